@@ -25,6 +25,9 @@ sources = [
     os.path.join(SRC, "pool.hip"),
     os.path.join(SRC, "norm.hip"),
     os.path.join(SRC, "softmax.hip"),
+    os.path.join(SRC, "layernorm.hip"),
+    os.path.join(SRC, "logprobs.hip"),
+    os.path.join(SRC, "newton_schulz.hip"),
 ]
 
 setup(

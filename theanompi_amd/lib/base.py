@@ -160,7 +160,7 @@ class GPUProcess:
             "verbose": self.verbose,
         }
         for key in ("batch_size", "epochs", "dtype", "n_iters", "val_iters",
-                    "image_size", "classes"):
+                    "image_size", "classes", "optimizer"):
             v = _env_opt(key)
             if v is not None:
                 config[key] = v

@@ -11,24 +11,32 @@ pass of the fused HIP kernel N12 over each flat fp32 master buffer,
 optionally writing the bf16 working copy in the same pass.
 """
 
+import math
+
 import torch
 
 from theanompi_amd import ops as _ops
+from theanompi_amd.ops import functional as OF
 
 
 class ParamRec:
     """One trainable: fp32 master + vel (+ optional bf16 mirror)."""
 
-    __slots__ = ("master", "vel", "bf16_out", "name", "lr_mult", "wd_mult")
+    __slots__ = ("master", "vel", "bf16_out", "name", "lr_mult", "wd_mult",
+                 "matrix", "span")
 
     def __init__(self, master, name="", lr_mult=1.0, wd_mult=1.0,
-                 bf16_out=None):
+                 bf16_out=None, matrix=None, span=None):
         self.master = master          # fp32 tensor with .grad after bwd
         self.vel = torch.zeros_like(master.data)
         self.bf16_out = bf16_out      # bf16 tensor refreshed by the step
         self.name = name
         self.lr_mult = lr_mult
         self.wd_mult = wd_mult
+        # (batch, rows, cols) if the parameter is one or more matrices
+        # that Muon orthogonalises, and their longer side without padding
+        self.matrix = matrix
+        self.span = span
 
 
 class SGDMomentum:
@@ -197,3 +205,84 @@ class SGDMomentum:
         else:
             for r in self.recs:
                 self._dispatch(r, r.vel, 2)
+
+
+class Muon(SGDMomentum):
+    """Orthogonalised momentum for the records that are matrices
+    (``ParamRec.matrix``), SGD + momentum for the others (biases and
+    normalisation parameters), under every rule:
+
+      phase 1:  vel = mu*vel - grad
+      phase 2:  w = (1 - lr*wd)*w + lr * rms*sqrt(longer side) * NS(vel)
+
+    NS are ``steps`` Newton-Schulz products (ops.functional.
+    orthogonalize); its entries' root mean square is about
+    1/sqrt(longer side), so an update's is about lr*rms whatever the
+    matrix's shape.  Between the phases the cdd exchange averages the
+    momenta, and every worker orthogonalises the average.  A merged
+    weight (several 1x1 convolutions over one input) is one matrix."""
+
+    def __init__(self, recs, lr=0.02, momentum=0.95, weight_decay=0.0,
+                 grad_arena=None, steps=5, rms=0.2):
+        super().__init__(recs, lr, momentum, weight_decay, grad_arena)
+        self.steps = steps
+        self.rms = rms
+        self._mats = [r for r in self.recs if r.matrix is not None]
+        self._rest = SGDMomentum(
+            [r for r in self.recs if r.matrix is None], lr, momentum,
+            weight_decay)
+
+    def make_persistent(self):
+        super().make_persistent()
+        self._rest.persistent_grads = True
+        self._rest.invalidate()
+
+    def invalidate(self):
+        super().invalidate()
+        self._rest.invalidate()
+
+    def _update(self, phase):
+        recs = self._mats if phase == 2 else [
+            r for r in self._mats if r.master.grad is not None]
+        ws, gs, vs, outs, lrs, wds, scales = [], [], [], [], [], [], []
+        for r in recs:
+            ws.append(r.master.data.view(r.matrix))
+            gs.append(None if phase == 2 else
+                      r.master.grad.contiguous().view(r.matrix))
+            vs.append(r.vel.view(r.matrix))
+            outs.append(r.bf16_out if phase != 1 else None)
+            lrs.append(self.lr * r.lr_mult)
+            wds.append(self.weight_decay * r.wd_mult)
+            scales.append(self.rms * math.sqrt(r.span or max(r.matrix[1:])))
+        OF.muon_update(ws, gs, vs, outs, lrs, wds, self.momentum, scales,
+                       phase, self.steps)
+
+    def _sync(self):
+        # lr, momentum and decay are changed on this object
+        rest = self._rest
+        rest.lr, rest.momentum = self.lr, self.momentum
+        rest.weight_decay = self.weight_decay
+        return rest
+
+    def step(self):
+        self._sync().step()
+        self._update(0)
+
+    def phase1(self):
+        self._sync().phase1()
+        self._update(1)
+
+    def phase2(self):
+        self._sync().phase2()
+        self._update(2)
+
+
+OPTIMIZERS = {"sgd": SGDMomentum, "muon": Muon}
+
+
+def build_optimizer(name, recs, **kwargs):
+    """The optimizer of that name ('sgd' or 'muon') over ``recs``."""
+    if name not in OPTIMIZERS:
+        raise ValueError(f"unknown optimizer {name!r}: one of "
+                         f"{', '.join(sorted(OPTIMIZERS))}")
+    return OPTIMIZERS[name](recs, **kwargs)

@@ -11,7 +11,7 @@ from contextlib import contextmanager as _contextmanager
 import torch
 
 from theanompi_amd.lib import helper_funcs
-from theanompi_amd.lib.opt import ParamRec, SGDMomentum
+from theanompi_amd.lib.opt import ParamRec, build_optimizer
 from theanompi_amd.models import layers as L
 from theanompi_amd.ops import functional as OF
 
@@ -91,14 +91,16 @@ class BaseModel:
         for name, mod in self.module.named_modules():
             if isinstance(mod, (L.Conv2d, L.Linear)):
                 bf16 = getattr(mod, "w_bf16", None)
+                matrix, span = mod.weight_matrix()
                 self.recs.append(ParamRec(mod.weight, name + ".W",
-                                          bf16_out=bf16))
+                                          bf16_out=bf16, matrix=matrix,
+                                          span=span))
                 if mod.bias is not None:
                     self.recs.append(ParamRec(mod.bias, name + ".b",
                                               wd_mult=0.0))
                 if mod.gpu:
                     self._post_step_layers.append(mod)
-            elif isinstance(mod, L.BatchNorm2d):
+            elif isinstance(mod, (L.BatchNorm2d, L.LayerNorm)):
                 self.recs.append(ParamRec(mod.gamma, name + ".gamma",
                                           wd_mult=0.0))
                 self.recs.append(ParamRec(mod.beta, name + ".beta",
@@ -207,10 +209,11 @@ class BaseModel:
         """Reference compiled Theano functions here (minutes); we build the
         optimizer and warm the kernels (instant)."""
         self.sync_type = sync_type
-        self.opt = SGDMomentum(self.recs, lr=self.current_lr,
-                               grad_arena=self.grad_arena,
-                               momentum=self.momentum,
-                               weight_decay=self.weight_decay)
+        self.opt = build_optimizer(self.config.get("optimizer", "sgd"),
+                                   self.recs, lr=self.current_lr,
+                                   grad_arena=self.grad_arena,
+                                   momentum=self.momentum,
+                                   weight_decay=self.weight_decay)
 
     def sync_tensors(self):
         """What the BSP exchanger moves, by sync mode."""

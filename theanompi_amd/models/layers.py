@@ -452,6 +452,24 @@ class _Base(nn.Module):
         reference's per-layer W-then-b order."""
         return []
 
+    def weight_matrix(self):
+        """((batch, rows, cols) of the weight as stored, the longer side
+        without padding): what Muon orthogonalises.  Convolutions: a
+        group's output channels by taps x input channels."""
+        if self.gpu:
+            plan = self.plan
+            taps = plan.R * plan.S
+            c = getattr(self, "Cg_logical", plan.Cg)
+            if isinstance(self, Linear):
+                c = self.n_in
+            return plan.flat_shape(), max(plan.Kg, taps * c)
+        w = self.weight
+        if w.dim() == 2:
+            return (1, *w.shape), max(w.shape)
+        g = self.groups
+        cols = w[0].numel()
+        return (g, w.shape[0] // g, cols), max(w.shape[0] // g, cols)
+
     def _dgrad_single_plan(self):
         """The sole dgrad plan when the layer has exactly one stride
         class WITH a halo (the pre-padded dual-relu-backward target);
@@ -973,6 +991,30 @@ class BatchNorm2d(_Base):
                  lambda v: self.gamma.data.copy_(v)),
                 ("beta", lambda: self.beta.data,
                  lambda v: self.beta.data.copy_(v))]
+
+
+class LayerNorm(_Base):
+    """Normalisation of each position over its channels; on the GPU the
+    physical padding behind ``n_features`` stays zero."""
+
+    def __init__(self, n_features, eps=1e-5, device="cpu"):
+        super().__init__()
+        dev = torch.device(device)
+        self.n = n_features
+        c = cpad_for(n_features) if dev.type == "cuda" else n_features
+        self.gamma = nn.Parameter(torch.zeros(c, device=dev))
+        self.gamma.data[:n_features] = 1.0
+        self.beta = nn.Parameter(torch.zeros(c, device=dev))
+        self.eps = eps
+
+    def forward(self, x):
+        return OF.layernorm(x, self.gamma, self.beta, self.eps, self.n)
+
+    def logical_params(self):
+        return [("gamma", lambda: self.gamma.data[:self.n],
+                 lambda v: self.gamma.data[:self.n].copy_(v)),
+                ("beta", lambda: self.beta.data[:self.n],
+                 lambda v: self.beta.data[:self.n].copy_(v))]
 
 
 class Dropout(_Base):

@@ -29,7 +29,7 @@ import torch
 import torch.nn.functional as F
 
 from theanompi_amd.lib import helper_funcs
-from theanompi_amd.lib.opt import ParamRec, SGDMomentum
+from theanompi_amd.lib.opt import ParamRec, build_optimizer
 from theanompi_amd.models.data.synthetic import SyntheticData
 
 
@@ -80,7 +80,8 @@ class ContractAdapter:
         self.module = self.module_factory().to(self.device)
         self.module.train()
         self.data = self.data_factory()
-        self.recs = [ParamRec(p, name)
+        self.recs = [ParamRec(p, name, matrix=(1, p.shape[0], p[0].numel())
+                              if p.dim() > 1 else None)
                      for name, p in self.module.named_parameters()]
         self.params = [r.master for r in self.recs]
         self.vels = [r.vel for r in self.recs]
@@ -90,9 +91,10 @@ class ContractAdapter:
 
     def compile_iter_fns(self, sync_type="cdd"):
         self.sync_type = sync_type
-        self.opt = SGDMomentum(self.recs, lr=self.current_lr,
-                               momentum=self.momentum,
-                               weight_decay=self.weight_decay)
+        self.opt = build_optimizer(self.config.get("optimizer", "sgd"),
+                                   self.recs, lr=self.current_lr,
+                                   momentum=self.momentum,
+                                   weight_decay=self.weight_decay)
 
     # -- contract: train / validate ---------------------------------------------
 

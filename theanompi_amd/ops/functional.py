@@ -16,6 +16,7 @@ including conv (reference: the ops of Theano-MPI's layer library
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from theanompi_amd import ops as _ops
 
@@ -106,6 +107,70 @@ def softmax_xent_ref(logits, labels, n_classes=None):
     probs = F.softmax(logits.float(), dim=1)
     loss = F.cross_entropy(logits.float(), labels)
     return loss, probs
+
+
+def layernorm_ref(x, gamma, beta, eps=1e-5, n_features=None):
+    """Normalisation over the last dimension's first ``n_features``
+    channels, statistics in at least fp32; zeros behind them."""
+    n = n_features or x.shape[-1]
+    wide = torch.promote_types(x.dtype, torch.float32)
+    xf = x[..., :n].to(wide)
+    d = xf - xf.mean(dim=-1, keepdim=True)
+    var = (d * d).mean(dim=-1, keepdim=True)
+    y = d / torch.sqrt(var + eps) * gamma[:n] + beta[:n]
+    return pad_channels(y, x.shape[-1]).to(x.dtype)
+
+
+def label_logprobs_ref(logits, labels, n_classes=None, top=0):
+    """See :func:`label_logprobs`."""
+    n = n_classes or logits.shape[1]
+    wide = torch.promote_types(logits.dtype, torch.float32)
+    z = logits[:, :n].to(wide)
+    masked = z == float("-inf")
+    empty = masked.all(dim=1, keepdim=True)
+    logp = torch.log_softmax(torch.where(empty, torch.zeros_like(z), z),
+                             dim=1)
+    p = logp.exp()
+    entropy = -(p * logp.masked_fill(p == 0, 0.0)).sum(dim=1)
+    entropy = entropy.masked_fill(empty[:, 0], 0.0)
+    logp = logp.masked_fill(empty, float("-inf"))
+    given = logp.gather(1, labels.clamp(0, n - 1)[:, None])[:, 0]
+    given = given * torch.ones_like(given).masked_fill(labels >= n,
+                                                       float("nan"))
+    given = given.masked_fill(labels < 0, 0.0)
+    # a stable sort leaves equal values in the order of their index
+    best = z.detach().sort(dim=1, descending=True, stable=True)
+    best = best.indices[:, :top].contiguous()
+    return given, entropy, logp.gather(1, best), best
+
+
+#: the quintic whose iteration takes singular values towards 1
+NS_QUINTIC = (3.4445, -4.775, 2.0315)
+
+
+def orthogonalize_ref(x, steps=5):
+    """See :func:`orthogonalize`."""
+    y = x.to(torch.promote_types(x.dtype, torch.float32))
+    tall = y.shape[-2] > y.shape[-1]
+    if tall:
+        y = y.transpose(-2, -1)
+    norm = y.double().square().sum(dim=(-2, -1), keepdim=True).sqrt()
+    y = (y / (norm + 1e-7)).to(y.dtype)
+    a, b, c = NS_QUINTIC
+    for _ in range(steps):
+        gram = y @ y.transpose(-2, -1)
+        y = a * y + (b * gram + c * (gram @ gram)) @ y
+    return (y.transpose(-2, -1) if tall else y).to(x.dtype).contiguous()
+
+
+def muon_update_ref(w, g, v, out, keep, rate, momentum, phase, steps):
+    """One matrix (or batch) of :func:`muon_update`."""
+    if phase != 2:
+        v.mul_(momentum).sub_(g)
+    if phase != 1:
+        w.mul_(keep).add_(orthogonalize_ref(v, steps), alpha=rate)
+        if out is not None:
+            out.copy_(w)
 
 
 # ---------------------------------------------------------------------------
@@ -346,6 +411,45 @@ class _SoftmaxXentFn(torch.autograd.Function):
         return dlogits, None, None
 
 
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps, n):
+        y, stat = _ops.ext().ln_fwd(x, gamma, beta, n, eps)
+        # stat = per-row mean and 1/std: the backward re-reads x
+        ctx.save_for_backward(x, gamma, stat)
+        ctx.n = n
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gamma, stat = ctx.saved_tensors
+        dx, dgamma, dbeta = _ops.ext().ln_bwd(dy, x, gamma, stat, ctx.n)
+        return dx, dgamma, dbeta, None, None
+
+
+class _LabelLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, n, top):
+        logp, entropy, top_logp, top_idx, stat = _ops.ext().lp_fwd(
+            logits, labels, n, top)
+        ctx.save_for_backward(logits, labels, top_idx, stat)
+        ctx.n = n
+        ctx.mark_non_differentiable(top_idx)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top_logp, top_idx
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogp, dentropy, dtop, _):
+        logits, labels, top_idx, stat = ctx.saved_tensors
+        if dlogp is None and dentropy is None and dtop is None:
+            return None, None, None, None
+        dx = _ops.ext().lp_bwd(logits, labels, top_idx, stat, dlogp,
+                               dentropy, dtop, ctx.n)
+        return dx, None, None, None
+
+
 # ---------------------------------------------------------------------------
 # public dispatchers
 # ---------------------------------------------------------------------------
@@ -431,3 +535,197 @@ def softmax_xent_err(logits, labels, n_classes=None):
         pred = logits[:, :n_classes].argmax(dim=1)
         err = (pred != labels).float().mean()
     return loss, probs, err
+
+
+def _check_float(t, name):
+    ok = (torch.float32, torch.float16, torch.bfloat16)
+    if t.dtype not in ok and (t.is_cuda or t.dtype != torch.float64):
+        raise TypeError(f"{name} must be float32, float16 or bfloat16, "
+                        f"not {t.dtype}")
+
+
+def _check_count(n, most, name):
+    if n is None:
+        return most
+    if isinstance(n, bool) or not isinstance(n, int) or not 1 <= n <= most:
+        raise ValueError(f"{name} must be a whole number from 1 to {most}, "
+                         f"not {n!r}")
+    return n
+
+
+def layernorm(x, gamma, beta, eps=1e-5, n_features=None):
+    """Layer normalisation over the last (channel) dimension.
+
+    ``x``: [..., C] in float32, float16 or bfloat16; rows may lie apart
+    (a channel slice of a wider buffer).  ``gamma``, ``beta``: float32
+    [C].  Only the first ``n_features`` channels count (default: all);
+    the physical padding behind them is not read, its outputs and
+    gradients are 0.  Statistics are kept in float32.  Returns x's shape
+    and type.  Differentiable once in x, gamma and beta; the sums of the
+    latter two have a fixed order, so a repeated call gives the same
+    bits."""
+    _check_float(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x needs at least one channel")
+    c = x.shape[-1]
+    for t, name in ((gamma, "gamma"), (beta, "beta")):
+        if t.shape != (c,):
+            raise ValueError(f"{name} must have shape ({c},), "
+                             f"not {tuple(t.shape)}")
+        if t.dtype != (torch.float64 if x.dtype == torch.float64
+                       else torch.float32):
+            raise TypeError(f"{name} must be float32, not {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must not be negative, not {eps}")
+    n = _check_count(n_features, c, "n_features")
+    if x.is_cuda:
+        return _LayerNormFn.apply(x, gamma.contiguous(), beta.contiguous(),
+                                  eps, n)
+    return layernorm_ref(x, gamma, beta, eps, n)
+
+
+#: alternatives that label_logprobs can name
+TOP_MAX = 32
+
+
+def label_logprobs(logits, labels, n_classes=None, top=0):
+    """Log probability of each row's given class, the entropy of the
+    row's distribution, and its most probable classes.
+
+    ``logits``: [B, C] in float32, float16 or bfloat16, of which the
+    first ``n_classes`` columns count; rows may lie apart.  ``labels``:
+    int64 [B]; below 0: no class is given (log probability 0), from
+    ``n_classes`` on: NaN.  Returns (logp [B], entropy [B], top_logp
+    [B, top], top_idx [B, top]): float32, and int64 class numbers, best
+    first, equal logits by ascending class.  Logits of -inf are masked
+    classes: probability 0, and no gradient unless the label or an
+    alternative names them.  A row of masked classes alone has logp
+    -inf, entropy 0 and gradient 0.  A NaN or +inf gives
+    NaN in its row.  Differentiable once in the logits, through logp,
+    entropy and top_logp."""
+    _check_float(logits, "logits")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be [rows, classes], not "
+                         f"{tuple(logits.shape)}")
+    if labels.dtype != torch.int64:
+        raise TypeError(f"labels must be int64, not {labels.dtype}")
+    if labels.shape != logits.shape[:1]:
+        raise ValueError(f"labels must have shape ({logits.shape[0]},), "
+                         f"not {tuple(labels.shape)}")
+    if labels.device != logits.device:
+        raise ValueError(f"labels are on {labels.device}, logits on "
+                         f"{logits.device}")
+    n = _check_count(n_classes, logits.shape[1], "n_classes")
+    if isinstance(top, bool) or not isinstance(top, int) \
+            or not 0 <= top <= min(n, TOP_MAX):
+        raise ValueError(f"top must be a whole number from 0 to "
+                         f"{min(n, TOP_MAX)}, not {top!r}")
+    if logits.is_cuda:
+        return _LabelLogprobsFn.apply(logits, labels.contiguous(), n, top)
+    return label_logprobs_ref(logits, labels, n, top)
+
+
+def _check_steps(steps):
+    if isinstance(steps, bool) or not isinstance(steps, int) \
+            or not 1 <= steps <= 64:
+        raise ValueError("steps must be a whole number from 1 to 64, "
+                         f"not {steps!r}")
+
+
+def orthogonalize(x, steps=5):
+    """Newton-Schulz products that take the singular values of a matrix
+    towards 1 (into about 0.7 to 1.2) and leave its singular vectors.
+
+    ``x``: [rows, cols] or [batch, rows, cols] in float32, float16 or
+    bfloat16.  X = x / (|x|_F + 1e-7), then ``steps`` times
+    X <- (a + b XX^T + c (XX^T)^2) X with (a, b, c) = NS_QUINTIC, on the
+    orientation that has the smaller XX^T; accuracy is float32's for all
+    types.  Returns a new tensor of x's shape and type, without a
+    gradient."""
+    _check_float(x, "x")
+    if x.dim() not in (2, 3):
+        raise ValueError("x must be [rows, cols] or [batch, rows, cols], "
+                         f"not {tuple(x.shape)}")
+    _check_steps(steps)
+    with torch.no_grad():
+        x = x.detach()
+        if x.is_cuda:
+            return _ops.ext().orthogonalize(x, steps)
+        return orthogonalize_ref(x, steps) if x.numel() else x.clone()
+
+
+def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
+                steps=5):
+    """Orthogonalised momentum update of a list of weights, in place:
+
+      v = momentum*v - g;   w = (1 - lr*wd)*w + lr*scale*orthogonalize(v)
+
+    ``ws``, ``gs``, ``vs``: float32, contiguous, [rows, cols] or [batch,
+    rows, cols] (each matrix of a batch on its own); ``outs``: bf16
+    working copies of w, or None in the place of one that is not kept.
+    ``phase``: 0 the whole update, 1 the momentum only, 2 the weights
+    only (g is not read), as in the SGD step.  On the GPU every matrix
+    of the list goes through each product in one launch."""
+    many = len(ws)
+    for name, part in (("gs", gs), ("vs", vs), ("outs", outs),
+                       ("lrs", lrs), ("wds", wds), ("scales", scales)):
+        if len(part) != many:
+            raise ValueError(f"{name} has {len(part)} entries, ws {many}")
+    if phase not in (0, 1, 2):
+        raise ValueError(f"phase must be 0, 1 or 2, not {phase!r}")
+    _check_steps(steps)
+    if not many:
+        return
+    seen = set()
+    for i in range(many):
+        w = ws[i]
+        parts = [("w", w), ("v", vs[i])]
+        if phase != 2:
+            parts.append(("g", gs[i]))
+        for name, t in parts:
+            if t.dtype != torch.float32:
+                raise TypeError(f"{name} {i} must be float32, "
+                                f"not {t.dtype}")
+            if not t.is_contiguous() or t.shape != w.shape \
+                    or t.dim() not in (2, 3):
+                raise ValueError(
+                    f"{name} {i} must be a contiguous [rows, cols] or "
+                    "[batch, rows, cols] of its weight's shape")
+            if t.device != ws[0].device:
+                raise ValueError(f"{name} {i} is on {t.device}, the first "
+                                 f"weight on {ws[0].device}")
+        if outs[i] is not None:
+            if outs[i].dtype != torch.bfloat16:
+                raise TypeError(f"out {i} must be bfloat16, "
+                                f"not {outs[i].dtype}")
+            if not outs[i].is_contiguous() \
+                    or outs[i].numel() != w.numel() \
+                    or outs[i].device != w.device:
+                raise ValueError(f"out {i} must be contiguous, of its "
+                                 "weight's size and on its device")
+        if w.numel():
+            for t in (w, vs[i]):
+                if t.data_ptr() in seen:
+                    raise ValueError("a weight or momentum is in the "
+                                     "list twice")
+                seen.add(t.data_ptr())
+    keeps = [1.0 - lr * wd for lr, wd in zip(lrs, wds)]
+    rates = [lr * scale for lr, scale in zip(lrs, scales)]
+    with torch.no_grad():
+        if ws[0].is_cuda:
+            none = torch.empty(0, dtype=torch.bfloat16,
+                               device=ws[0].device)
+            _ops.ext().muon_update(
+                [w.detach() for w in ws], list(gs), list(vs),
+                [none if o is None else o for o in outs], keeps, rates,
+                float(momentum), phase, steps)
+            return
+        for i in range(many):
+            out = outs[i]
+            if ws[i].numel():
+                muon_update_ref(ws[i], gs[i], vs[i],
+                                out if out is None else out.view_as(ws[i]),
+                                keeps[i], rates[i], momentum, phase, steps)

@@ -15,6 +15,8 @@
 #include <unordered_map>
 #include <vector>
 
+#include "newton_schulz.hpp"
+
 // ---- extern "C" launchers from the .hip TUs --------------------------------
 
 struct GatherGemmArgs {
@@ -131,6 +133,28 @@ hipError_t launch_transpose_multi(const void*, int, int, int,
 hipError_t launch_tr_probe(const int*, float*, int, hipStream_t);
 hipError_t launch_splitk_finalize(float*, const float*, void*, long,
                                   int, int, hipStream_t);
+hipError_t launch_ln_fwd(const void*, const float*, const float*, void*,
+                         float*, float*, long, int, int, long, float, int,
+                         hipStream_t);
+hipError_t ln_bwd_plan(long, int, int, long*, int*);
+hipError_t launch_ln_bwd(const void*, const void*, const float*,
+                         const float*, const float*, void*, float*,
+                         float*, float*, long, long, int, int, long, long,
+                         int, hipStream_t);
+int lp_plan(long, long, int, int*, int*);
+hipError_t launch_lp_fwd(const void*, const long*, float*, float*, float*,
+                         long*, float*, float*, unsigned long long*, long,
+                         int, long, int, int, int, int, int, hipStream_t);
+hipError_t launch_lp_bwd(const void*, const long*, const long*,
+                         const float*, const float*, const float*,
+                         const float*, void*, long, int, int, long, int,
+                         int, hipStream_t);
+}
+
+extern "C" {
+hipError_t launch_ns_sum(NsArgs*, hipStream_t);
+hipError_t launch_ns_load(NsArgs*, hipStream_t);
+hipError_t launch_ns_gemm(NsArgs*, int, hipStream_t);
 }
 
 // pick a K-split so small-M GEMMs (FC layers at batch<=256) still fill
@@ -1074,6 +1098,348 @@ static void transpose_multi_run(torch::Tensor desc, long nseg,
                                    cur_stream()));
 }
 
+// ---- layer norm -------------------------------------------------------------
+
+static int kind_of(const torch::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be on GPU");
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return 0;
+    case torch::kFloat16: return 1;
+    case torch::kBFloat16: return 2;
+    default: TORCH_CHECK(false, name, " must be f32, f16 or bf16");
+  }
+  return -1;
+}
+
+static void check_same(const torch::Tensor& t, const torch::Tensor& x,
+                       const char* name) {
+  TORCH_CHECK(t.device() == x.device(), name, " is on another device");
+}
+
+// Rows of the last dimension at a uniform distance (a channel slice of a
+// wider buffer among them); anything else is laid out anew.
+static torch::Tensor as_rows(const torch::Tensor& t, long* ld) {
+  const long C = t.size(-1);
+  bool ok = C <= 1 || t.stride(-1) == 1;
+  long step = -1, span = 0;    // row distance; what a full index covers
+  for (long d = t.dim() - 2; ok && d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (step < 0) {
+      step = t.stride(d);
+      ok = step >= C;
+    } else {
+      ok = t.stride(d) == span;
+    }
+    span = t.stride(d) * t.size(d);
+  }
+  if (!ok) {
+    *ld = C;
+    return t.contiguous();
+  }
+  *ld = step < 0 ? C : step;
+  return t;
+}
+
+static std::vector<torch::Tensor> ln_fwd(torch::Tensor x,
+                                         torch::Tensor gamma,
+                                         torch::Tensor beta, long n,
+                                         double eps) {
+  const int kind = kind_of(x, "x");
+  check_f32(gamma, "gamma");
+  check_f32(beta, "beta");
+  check_same(gamma, x, "gamma");
+  check_same(beta, x, "beta");
+  TORCH_CHECK(x.dim() >= 1, "x needs a channel dimension");
+  const long C = x.size(-1);
+  TORCH_CHECK(gamma.numel() == C && beta.numel() == C,
+              "gamma and beta must have x's channels");
+  TORCH_CHECK(n >= 1 && n <= C && C < (1L << 30), "bad channel count");
+  c10::DeviceGuard guard(x.device());
+  long ld;
+  x = as_rows(x, &ld);
+  const long rows = x.numel() / C;
+  auto y = torch::empty(x.sizes(), x.options());
+  auto stat = torch::empty({2, rows}, gamma.options());
+  if (rows)
+    CHECK_HIP(launch_ln_fwd(x.data_ptr(), gamma.data_ptr<float>(),
+                            beta.data_ptr<float>(), y.data_ptr(),
+                            stat.data_ptr<float>(),
+                            stat.data_ptr<float>() + rows, rows, (int)C,
+                            (int)n, ld, (float)eps, kind, cur_stream()));
+  return {y, stat};
+}
+
+static std::vector<torch::Tensor> ln_bwd(torch::Tensor dy,
+                                         torch::Tensor x,
+                                         torch::Tensor gamma,
+                                         torch::Tensor stat, long n) {
+  const int kind = kind_of(x, "x");
+  TORCH_CHECK(dy.scalar_type() == x.scalar_type()
+                  && dy.sizes() == x.sizes(),
+              "dy must have x's shape and type");
+  check_f32(gamma, "gamma");
+  check_f32(stat, "stat");
+  check_same(dy, x, "dy");
+  c10::DeviceGuard guard(x.device());
+  const long C = x.size(-1), rows = x.numel() / C;
+  TORCH_CHECK(gamma.numel() == C && stat.numel() == 2 * rows
+                  && n >= 1 && n <= C,
+              "gamma / stat do not fit x");
+  long ldx, lddy;
+  x = as_rows(x, &ldx);
+  dy = as_rows(dy, &lddy);
+  auto dx = torch::empty(x.sizes(), x.options());
+  auto dgamma = torch::empty({C}, gamma.options());
+  auto dbeta = torch::empty({C}, gamma.options());
+  if (!rows) return {dx, dgamma.zero_(), dbeta.zero_()};
+  long blocks;
+  int shares;
+  CHECK_HIP(ln_bwd_plan(rows, (int)C, kind, &blocks, &shares));
+  torch::Tensor part;
+  if (shares) part = torch::empty({blocks * 2 * C}, gamma.options());
+  const float* st = stat.data_ptr<float>();
+  CHECK_HIP(launch_ln_bwd(dy.data_ptr(), x.data_ptr(),
+                          gamma.data_ptr<float>(), st, st + rows,
+                          dx.data_ptr(), dgamma.data_ptr<float>(),
+                          dbeta.data_ptr<float>(),
+                          shares ? part.data_ptr<float>() : nullptr,
+                          blocks, rows, (int)C, (int)n, ldx, lddy, kind,
+                          cur_stream()));
+  return {dx, dgamma, dbeta};
+}
+
+// ---- class log probabilities ------------------------------------------------
+
+static std::vector<torch::Tensor> lp_fwd(torch::Tensor x,
+                                         torch::Tensor labels, long n,
+                                         long k) {
+  const int kind = kind_of(x, "logits");
+  TORCH_CHECK(x.dim() == 2, "logits must be [rows, classes]");
+  const long rows = x.size(0), C = x.size(1);
+  TORCH_CHECK(labels.scalar_type() == torch::kInt64
+                  && labels.is_contiguous() && labels.dim() == 1
+                  && labels.size(0) == rows,
+              "labels must be contiguous int64 [rows]");
+  check_same(labels, x, "labels");
+  TORCH_CHECK(n >= 1 && n <= C && C < (1L << 30), "bad n_classes");
+  TORCH_CHECK(k >= 0 && k <= n && k <= 32, "bad number of alternatives");
+  c10::DeviceGuard guard(x.device());
+  long ld;
+  x = as_rows(x, &ld);
+  auto f32 = x.options().dtype(torch::kFloat32);
+  auto i64 = x.options().dtype(torch::kInt64);
+  auto logp = torch::empty({rows}, f32);
+  auto entropy = torch::empty({rows}, f32);
+  auto top_logp = torch::empty({rows, k}, f32);
+  auto top_idx = torch::empty({rows, k}, i64);
+  auto stat = torch::empty({rows, 3}, f32);
+  if (rows) {
+    int lanes, nv;
+    const long segs = lp_plan(rows, n, kind, &lanes, &nv);
+    TORCH_CHECK(segs > 0, "n_classes ", n, " is over what a row may have");
+    TORCH_CHECK(rows * segs < (1L << 31), "too many rows");
+    torch::Tensor psum, pkey;
+    if (segs > 1) {
+      psum = torch::empty({rows * segs * 3}, f32);
+      pkey = torch::empty({rows * segs * k}, i64);
+    }
+    CHECK_HIP(launch_lp_fwd(
+        x.data_ptr(), labels.data_ptr<long>(), logp.data_ptr<float>(),
+        entropy.data_ptr<float>(), top_logp.data_ptr<float>(),
+        top_idx.data_ptr<long>(), stat.data_ptr<float>(),
+        segs > 1 ? psum.data_ptr<float>() : nullptr,
+        segs > 1 ? (unsigned long long*)pkey.data_ptr() : nullptr, rows,
+        (int)n, ld, (int)segs, lanes, nv, (int)k, kind, cur_stream()));
+  }
+  return {logp, entropy, top_logp, top_idx, stat};
+}
+
+static torch::Tensor lp_bwd(torch::Tensor x, torch::Tensor labels,
+                            torch::Tensor top_idx, torch::Tensor stat,
+                            c10::optional<torch::Tensor> dlogp,
+                            c10::optional<torch::Tensor> dentropy,
+                            c10::optional<torch::Tensor> dtop, long n) {
+  const int kind = kind_of(x, "logits");
+  c10::DeviceGuard guard(x.device());
+  const long rows = x.size(0), C = x.size(1), k = top_idx.size(1);
+  TORCH_CHECK(labels.numel() == rows && stat.numel() == 3 * rows
+                  && top_idx.numel() == rows * k && n >= 1 && n <= C,
+              "saved tensors do not fit the logits");
+  long ld;
+  x = as_rows(x, &ld);
+  auto dx = torch::empty({rows, C}, x.options());
+  auto grad = [&](c10::optional<torch::Tensor>& t, long numel)
+      -> const float* {
+    if (!t.has_value() || !t->defined() || numel == 0) return nullptr;
+    TORCH_CHECK(t->numel() == numel
+                    && t->scalar_type() == torch::kFloat32,
+                "bad gradient");
+    t = t->contiguous();
+    return t->data_ptr<float>();
+  };
+  const float* dl = grad(dlogp, rows);
+  const float* dh = grad(dentropy, rows);
+  const float* dt = grad(dtop, rows * k);
+  if (rows)
+    CHECK_HIP(launch_lp_bwd(x.data_ptr(), labels.data_ptr<long>(),
+                            top_idx.data_ptr<long>(),
+                            stat.data_ptr<float>(), dl, dh, dt,
+                            dx.data_ptr(), rows, (int)n, (int)C, ld,
+                            (int)k, kind, cur_stream()));
+  return dx;
+}
+
+// ---- Newton-Schulz / orthogonalised momentum --------------------------------
+
+// Fills in shapes and workspace of `a` (count problems that have m, n,
+// batch and pointers to their data), and returns the workspace.
+static torch::Tensor ns_workspace(NsArgs& a,
+                                  const torch::TensorOptions& opts) {
+  const long tile = NS_TILE;
+  long total = 0;
+  auto take = [&](long bytes) {
+    const long at = total;
+    total += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  std::vector<long> at;
+  for (int i = 0; i < a.count; ++i) {
+    NsProb& p = a.p[i];
+    p.mp = (int)((p.m + tile - 1) / tile * tile);
+    p.np = (int)((p.n + tile - 1) / tile * tile);
+    const long len = (long)p.m * p.n;
+    long parts = (len + 4095) / 4096;
+    p.parts = (int)(parts < 256 ? parts : 256);
+    const long x = 4L * p.batch * p.mp * p.np;
+    const long s = 4L * p.batch * p.mp * p.mp;
+    at.push_back(take(x));
+    at.push_back(take(x));
+    at.push_back(take(s));
+    at.push_back(take(s));
+    at.push_back(take(8L * p.batch * p.parts));
+    at.push_back(take(4L * p.batch));
+  }
+  auto ws = torch::empty({total}, opts.dtype(torch::kUInt8));
+  char* base = (char*)ws.data_ptr();
+  for (int i = 0; i < a.count; ++i) {
+    NsProb& p = a.p[i];
+    p.X[0] = base + at[i * 6];
+    p.X[1] = base + at[i * 6 + 1];
+    p.A = base + at[i * 6 + 2];
+    p.B = base + at[i * 6 + 3];
+    p.part = (double*)(base + at[i * 6 + 4]);
+    p.shift = (float*)(base + at[i * 6 + 5]);
+  }
+  return ws;
+}
+
+static void ns_run(NsArgs& a, long steps, hipStream_t stream) {
+  a.steps = (int)steps;
+  CHECK_HIP(launch_ns_sum(&a, stream));
+  if (a.phase == 1) return;
+  CHECK_HIP(launch_ns_load(&a, stream));
+  for (int s = 0; s < (int)steps; ++s) {
+    a.step = s;
+    a.last = s + 1 == (int)steps;
+    for (int mode = 0; mode < 3; ++mode)
+      CHECK_HIP(launch_ns_gemm(&a, mode, stream));
+  }
+}
+
+static void ns_shape(NsProb& p, long rows, long cols, long batch) {
+  TORCH_CHECK(rows < (1L << 24) && cols < (1L << 24)
+                  && batch < (1L << 24),
+              "matrix too large");
+  p.tall = rows > cols;
+  p.m = (int)(p.tall ? cols : rows);
+  p.n = (int)(p.tall ? rows : cols);
+  p.batch = (int)batch;
+}
+
+static torch::Tensor orthogonalize(torch::Tensor x, long steps) {
+  TORCH_CHECK(x.dim() == 2 || x.dim() == 3,
+              "x must be [rows, cols] or [batch, rows, cols]");
+  TORCH_CHECK(steps >= 1 && steps <= 64, "bad number of steps");
+  const int kind = kind_of(x, "x");
+  c10::DeviceGuard guard(x.device());
+  x = x.contiguous();
+  auto out = torch::empty_like(x);
+  if (!x.numel()) return out;
+  NsArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.count = 1;
+  NsProb& p = a.p[0];
+  p.in = x.data_ptr();
+  p.out = out.data_ptr();
+  p.kind = kind;
+  ns_shape(p, x.size(-2), x.size(-1), x.dim() == 3 ? x.size(0) : 1);
+  auto ws = ns_workspace(a, x.options());
+  ns_run(a, steps, cur_stream());
+  return out;
+}
+
+// w, v (and the bf16 copies) in place.  Phases as sgd_step's: 0 = full,
+// 1 = momentum only, 2 = weights from the momentum.
+static void muon_update(std::vector<torch::Tensor> ws,
+                        std::vector<torch::Tensor> gs,
+                        std::vector<torch::Tensor> vs,
+                        std::vector<torch::Tensor> outs,
+                        std::vector<double> keeps,
+                        std::vector<double> rates, double mu, long phase,
+                        long steps) {
+  const size_t n = ws.size();
+  TORCH_CHECK(gs.size() == n && vs.size() == n && outs.size() == n
+                  && keeps.size() == n && rates.size() == n,
+              "muon_update: lists of different lengths");
+  TORCH_CHECK(phase >= 0 && phase <= 2 && steps >= 1 && steps <= 64,
+              "muon_update: bad phase or number of steps");
+  if (!n) return;
+  for (size_t i = 0; i < n; ++i) {
+    check_f32(ws[i], "w");
+    check_f32(vs[i], "v");
+    check_same(ws[i], ws[0], "w");
+    check_same(vs[i], ws[0], "v");
+    TORCH_CHECK(ws[i].dim() == 2 || ws[i].dim() == 3,
+                "w must be [rows, cols] or [batch, rows, cols]");
+    TORCH_CHECK(vs[i].sizes() == ws[i].sizes(), "v must have w's shape");
+    if (phase != 2) {
+      check_f32(gs[i], "g");
+      check_same(gs[i], ws[0], "g");
+      TORCH_CHECK(gs[i].sizes() == ws[i].sizes(),
+                  "g must have w's shape");
+    }
+    if (outs[i].numel()) {
+      check_bf16(outs[i], "out");
+      check_same(outs[i], ws[0], "out");
+      TORCH_CHECK(outs[i].numel() == ws[i].numel(),
+                  "out must have w's shape");
+    }
+  }
+  c10::DeviceGuard guard(ws[0].device());
+  size_t i = 0;
+  while (i < n) {
+    NsArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.phase = (int)phase;
+    a.mu = (float)mu;
+    for (; i < n && a.count < NS_MAXP; ++i) {
+      if (!ws[i].numel()) continue;
+      NsProb& p = a.p[a.count++];
+      p.w = ws[i].data_ptr<float>();
+      p.v = vs[i].data_ptr<float>();
+      p.g = phase != 2 ? gs[i].data_ptr<float>() : nullptr;
+      p.copy = outs[i].numel() ? outs[i].data_ptr() : nullptr;
+      p.keep = (float)keeps[i];
+      p.rate = (float)rates[i];
+      ns_shape(p, ws[i].size(-2), ws[i].size(-1),
+               ws[i].dim() == 3 ? ws[i].size(0) : 1);
+    }
+    if (!a.count) break;
+    auto buf = ns_workspace(a, ws[0].options());
+    ns_run(a, steps, cur_stream());
+  }
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("halo_pad", &halo_pad_sym);
   m.def("halo_pad_lrtb", &halo_pad);
@@ -1137,4 +1503,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gather_multi_run", &gather_multi_run);
   m.def("transpose_multi_make", &transpose_multi_make);
   m.def("transpose_multi_run", &transpose_multi_run);
+  m.def("ln_fwd", &ln_fwd);
+  m.def("ln_bwd", &ln_bwd);
+  m.def("lp_fwd", &lp_fwd);
+  m.def("lp_bwd", &lp_bwd);
+  m.def("orthogonalize", &orthogonalize);
+  m.def("muon_update", &muon_update);
 }

@@ -1,0 +1,486 @@
+// Log probabilities of given classes with the entropy and the top
+// alternatives of each row, and the gradient of the logits.
+//
+//   M = max x   s = sum exp(x-M)   t = sum exp(x-M)(x-M)
+//   logp_j = x_j - M - log s       H = log s - t/s
+//   top: the k largest x, equal values by ascending index
+//   dx_j = p_j * (-(dlogp + sum dtop) - dH*(logp_j + H))
+//          + [j == label]*dlogp + sum_i [j == top_i]*dtop_i
+//
+// Memory bound: the forward reads the logits once, the backward reads
+// them and writes their gradient.  A block holds its part of a row (a
+// segment) in registers, takes maximum and sums from there and writes
+// one partial result; rows of more than one segment are joined by a
+// second kernel, in a fixed order.
+//
+// A class at -inf is masked: probability 0, nothing to the entropy, and
+// p_j = 0 in its gradient.  A row of nothing else has logp -inf, entropy 0
+// and gradient 0.  Labels below 0 say that a row has no given class (logp
+// 0, no gradient from it); a label from n on is never read and gives NaN.
+
+#include "common.hpp"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
+
+constexpr int KMAX = 32;       // alternatives
+constexpr int MAXSEG = 256;    // segments a row
+
+// what is kept of a row for the backward pass
+struct RowStat { float M, logs, H; };
+
+// floats in an order that unsigned integers have: NaN above all, -0 as 0
+DEV unsigned ordered(float f) {
+  if (f != f) return 0xffffffffu;
+  const unsigned u = __float_as_uint(f + 0.f);
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+
+// value and index in one key: larger value first, then lower index
+DEV unsigned long long top_key(float f, int idx) {
+  return ((unsigned long long)ordered(f) << 32) | (unsigned)~idx;
+}
+DEV int key_index(unsigned long long k) { return (int)~(unsigned)k; }
+
+DEV float wave_max(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+    v = fmaxf(v, __shfl_xor(v, off, 64));
+  return v;
+}
+DEV float wave_sum(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+DEV unsigned long long wave_max_key(unsigned long long v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const unsigned long long o = __shfl_xor(v, off, 64);
+    if (o > v) v = o;
+  }
+  return v;
+}
+
+// one lane's NV vectors of a row, as loaded
+template <typename T, int LANES, int NV>
+struct Part {
+  static constexpr int N = 16 / sizeof(T);
+  union { u32x4 u; T t[N]; } c[NV];
+  int first, n;                       // first column; columns of the row
+
+  DEV int col(int i, int j) const { return first + i * LANES * N + j; }
+  DEV bool has(int i, int j) const { return col(i, j) < n; }
+  // what is behind the row is at -inf, as masked classes are
+  DEV float get(int i, int j) const { return (float)c[i].t[j]; }
+
+  DEV void load(const T* row, int seg0, int n_) {
+    first = seg0 + (int)threadIdx.x * N;
+    n = n_;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (col(i, N - 1) < n) {
+        c[i].u = ((const any16*)(row + col(i, 0)))->v;
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          c[i].t[j] = has(i, j) ? row[col(i, j)] : (T)-__builtin_inff();
+      }
+    }
+  }
+};
+
+// What a row's sums give.  s is 0 where every class is masked.
+DEV void finish_row(const float M, const float s, const float t,
+                    RowStat& st) {
+  if (s == 0.f) {
+    st.M = -__builtin_inff();
+    st.logs = 0.f;
+    st.H = 0.f;
+  } else {
+    // a NaN among masked classes alone must not pass for an empty row
+    st.M = s == s ? M : s;
+    st.logs = logf(s);
+    st.H = st.logs - t / s;
+  }
+}
+
+DEV float logp_of(const RowStat& st, float x) {
+  return st.M == -__builtin_inff() ? -__builtin_inff()
+                                   : (x - st.M) - st.logs;
+}
+
+template <typename T>
+DEV void write_row(const T* row, const long* labels, RowStat* stat,
+                   float* logp, float* entropy, long r, int n,
+                   const RowStat& st) {
+  stat[r] = st;
+  const long lab = labels[r];
+  logp[r] = lab < 0 ? 0.f
+            : lab < n ? logp_of(st, (float)row[lab])
+                      : __builtin_nanf("");
+  entropy[r] = st.H;
+}
+
+// One segment of one row.  Where a row has one segment only (segs == 1)
+// its results are final; else psum [row][seg][3] and pkey [row][seg][k]
+// go to lp_join_k.
+template <typename T, int LANES, int NV>
+__global__ __launch_bounds__(LANES) void lp_fwd_k(
+    const T* __restrict__ x, const long* __restrict__ labels,
+    float* __restrict__ logp, float* __restrict__ entropy,
+    float* __restrict__ top_logp, long* __restrict__ top_idx,
+    RowStat* __restrict__ stat, float* __restrict__ psum,
+    unsigned long long* __restrict__ pkey, int n, long ldx, int segs,
+    int k) {
+  constexpr int N = 16 / sizeof(T);
+  constexpr int WAVES = LANES / 64;
+  __shared__ float red[3][WAVES];
+  __shared__ unsigned long long kred[2][WAVES];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long r = blockIdx.x / segs;
+  const int seg = (int)(blockIdx.x % segs);
+  const T* row = x + r * ldx;
+  Part<T, LANES, NV> p;
+  p.load(row, seg * LANES * NV * N, n);
+
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) m = fmaxf(m, p.get(i, j));
+  m = wave_max(m);
+  if (WAVES > 1) {
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, red[0][w]);
+  }
+  // a maximum of -inf (nothing but masked classes) cannot be taken off
+  const float m0 = m == -__builtin_inff() ? 0.f : m;
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = p.get(i, j) - m0;
+      const float e = __expf(d);
+      s += e;
+      t += e > 0.f ? e * d : 0.f;
+    }
+  s = wave_sum(s);
+  t = wave_sum(t);
+  if (WAVES > 1) {
+    if (lane == 0) { red[1][wave] = s; red[2][wave] = t; }
+    __syncthreads();
+    s = t = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) { s += red[1][w]; t += red[2][w]; }
+  }
+  RowStat st;
+  finish_row(m, s, t, st);
+  if (threadIdx.x == 0) {
+    if (segs == 1) {
+      write_row(row, labels, stat, logp, entropy, r, n, st);
+    } else {
+      float* q = psum + (r * segs + seg) * 3;
+      q[0] = m;
+      q[1] = s;
+      q[2] = t;
+    }
+  }
+  // k times the best of what comes after the one before
+  unsigned long long last = ~0ull;
+  for (int a = 0; a < k; ++a) {
+    unsigned long long best = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const unsigned long long key = top_key(p.get(i, j), p.col(i, j));
+        if (p.has(i, j) && key < last && key > best) best = key;
+      }
+    best = wave_max_key(best);
+    if (WAVES > 1) {
+      if (lane == 0) kred[a & 1][wave] = best;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+        if (kred[a & 1][w] > best) best = kred[a & 1][w];
+    }
+    last = best;
+    if (threadIdx.x == 0) {
+      if (segs == 1) {
+        const int idx = key_index(best);
+        top_idx[r * k + a] = idx;
+        top_logp[r * k + a] = logp_of(st, (float)row[idx]);
+      } else {
+        pkey[(r * segs + seg) * k + a] = best;   // 0: no more there
+      }
+    }
+  }
+}
+
+// one wave a row: the segments' sums and their sorted lists
+template <typename T>
+__global__ __launch_bounds__(64) void lp_join_k(
+    const T* __restrict__ x, const long* __restrict__ labels,
+    float* __restrict__ logp, float* __restrict__ entropy,
+    float* __restrict__ top_logp, long* __restrict__ top_idx,
+    RowStat* __restrict__ stat, const float* __restrict__ psum,
+    const unsigned long long* __restrict__ pkey, int n, long ldx,
+    int segs, int k) {
+  constexpr int H = MAXSEG / 64;
+  const long r = blockIdx.x;
+  const int lane = threadIdx.x;
+  const T* row = x + r * ldx;
+  float m[H], s[H], t[H], M = -__builtin_inff();
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const int g = lane + h * 64;
+    const float* q = psum + (r * segs + g) * 3;
+    m[h] = g < segs ? q[0] : -__builtin_inff();
+    s[h] = g < segs ? q[1] : 0.f;
+    t[h] = g < segs ? q[2] : 0.f;
+    M = fmaxf(M, m[h]);
+  }
+  M = wave_max(M);
+  float S = 0.f, U = 0.f;
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    // a segment of masked classes has no maximum to be taken off; its
+    // sum is 0, or NaN where it has a NaN
+    const float d = m[h] == -__builtin_inff() ? 0.f : m[h] - M;
+    const float e = __expf(d);
+    S += e * s[h];
+    U += e > 0.f ? e * (t[h] + d * s[h]) : 0.f;   // d may be -3e38
+  }
+  S = wave_sum(S);
+  U = wave_sum(U);
+  RowStat st;
+  finish_row(M, S, U, st);
+  if (lane == 0) write_row(row, labels, stat, logp, entropy, r, n, st);
+  // each lane's segments' next best
+  unsigned long long head[H];
+  int at[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const int g = lane + h * 64;
+    at[h] = 0;
+    head[h] = g < segs && k > 0 ? pkey[(r * segs + g) * k] : 0;
+  }
+  for (int a = 0; a < k; ++a) {
+    unsigned long long best = 0;
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      if (head[h] > best) best = head[h];
+    best = wave_max_key(best);
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      if (head[h] == best) {
+        const int g = lane + h * 64;
+        ++at[h];
+        head[h] = g < segs && at[h] < k
+                      ? pkey[(r * segs + g) * k + at[h]] : 0;
+      }
+    if (lane == 0) {
+      const int idx = key_index(best);
+      top_idx[r * k + a] = idx;
+      top_logp[r * k + a] = logp_of(st, (float)row[idx]);
+    }
+  }
+}
+
+// dx of BLOCK*NV vectors of a row: every class as if it were not given,
+// then the few that are.
+template <typename T, int NV>
+__global__ __launch_bounds__(256) void lp_bwd_k(
+    const T* __restrict__ x, const long* __restrict__ labels,
+    const long* __restrict__ top_idx, const RowStat* __restrict__ stat,
+    const float* __restrict__ dlogp, const float* __restrict__ dentropy,
+    const float* __restrict__ dtop, T* __restrict__ dx, int n, int C,
+    long ldx, int segs, int k) {
+  constexpr int N = 16 / sizeof(T);
+  const long r = blockIdx.x / segs;
+  const int seg = (int)(blockIdx.x % segs);
+  const int seg0 = seg * 256 * NV * N;
+  const int seg1 = seg0 + 256 * NV * N;
+  const T* row = x + r * ldx;
+  T* out = dx + r * C;
+  const RowStat st = stat[r];
+  const long lab = labels[r];
+  const bool empty = st.M == -__builtin_inff();
+  const float dl = !dlogp || lab < 0 ? 0.f
+                   : lab < n ? dlogp[r] : __builtin_nanf("");
+  const float dh = dentropy ? dentropy[r] : 0.f;
+  float all = dl;
+  if (dtop)
+    for (int a = 0; a < k; ++a) all += dtop[r * k + a];
+  const float c0 = -all - dh * st.H;
+
+  auto plain = [&](float v) -> float {
+    if (empty) return 0.f;
+    const float lp = (v - st.M) - st.logs;
+    const float p = __expf(lp);
+    return p == 0.f ? 0.f : p * (c0 - dh * lp);
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = seg0 + (i * 256 + (int)threadIdx.x) * N;
+    union { u32x4 u; T t[N]; } v;
+    if (c + N <= n) {
+      v.u = ((const any16*)(row + c))->v;
+#pragma unroll
+      for (int j = 0; j < N; ++j) v.t[j] = (T)plain((float)v.t[j]);
+      ((any16*)(out + c))->v = v.u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (c + j < C)
+          out[c + j] = c + j < n ? (T)plain((float)row[c + j]) : (T)0.f;
+    }
+  }
+  if (empty) return;
+  __syncthreads();                 // the block's own stores come first
+  const int a = (int)threadIdx.x;  // 0: the label; from 1: alternatives
+  if (a <= k) {
+    const bool isl = a == 0;
+    long j = isl ? lab : top_idx[r * k + a - 1];
+    if ((isl && (!dlogp || lab < 0 || lab >= n)) || j < seg0 || j >= seg1)
+      return;
+    // the label among the alternatives is the label's to write
+    float add = isl ? dl : dtop ? dtop[r * k + a - 1] : 0.f;
+    if (isl) {
+      if (dtop)
+        for (int b = 0; b < k; ++b)
+          if (top_idx[r * k + b] == j) add += dtop[r * k + b];
+    } else if (!dtop || (dlogp && j == lab)) {
+      return;
+    }
+    out[j] = (T)(plain((float)row[j]) + add);
+  }
+}
+
+struct FwdArgs {
+  const void* x;
+  const long* labels;
+  float *logp, *entropy, *top_logp;
+  long* top_idx;
+  float* stat;
+  float* psum;
+  unsigned long long* pkey;
+  long rows;
+  int n;
+  long ldx;
+  int segs, k, lanes, nv;
+};
+
+template <typename T, int LANES, int NV>
+void fwd_one(const FwdArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((lp_fwd_k<T, LANES, NV>),
+                     dim3((unsigned)(a.rows * a.segs)), dim3(LANES), 0,
+                     stream, (const T*)a.x, a.labels, a.logp, a.entropy,
+                     a.top_logp, a.top_idx, (RowStat*)a.stat, a.psum,
+                     a.pkey, a.n, a.ldx, a.segs, a.k);
+}
+
+template <typename T>
+hipError_t fwd(const FwdArgs& a, hipStream_t stream) {
+  if (a.lanes == 64) {
+    if (a.nv == 1) fwd_one<T, 64, 1>(a, stream);
+    else fwd_one<T, 64, 2>(a, stream);
+  } else {
+    if (a.nv == 1) fwd_one<T, 256, 1>(a, stream);
+    else if (a.nv == 2) fwd_one<T, 256, 2>(a, stream);
+    else if (a.nv == 4) fwd_one<T, 256, 4>(a, stream);
+    else fwd_one<T, 256, 8>(a, stream);
+  }
+  HIP_KERNEL_ASSERT_OK(hipGetLastError());
+  if (a.segs > 1)
+    hipLaunchKernelGGL(lp_join_k<T>, dim3((unsigned)a.rows), dim3(64), 0,
+                       stream, (const T*)a.x, a.labels, a.logp, a.entropy,
+                       a.top_logp, a.top_idx, (RowStat*)a.stat, a.psum,
+                       a.pkey, a.n, a.ldx, a.segs, a.k);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t bwd(const void* x, const long* labels, const long* top_idx,
+               const float* stat, const float* dlogp,
+               const float* dentropy, const float* dtop, void* dx,
+               long rows, int n, int C, long ldx, int k,
+               hipStream_t stream) {
+  constexpr int N = 16 / sizeof(T);
+#define LP_BWD(NV)                                                        \
+  do {                                                                    \
+    const int per = 256 * NV * N, segs = (C + per - 1) / per;             \
+    hipLaunchKernelGGL((lp_bwd_k<T, NV>), dim3((unsigned)(rows * segs)),  \
+                       dim3(256), 0, stream, (const T*)x, labels,         \
+                       top_idx, (const RowStat*)stat, dlogp, dentropy,    \
+                       dtop, (T*)dx, n, C, ldx, segs, k);                 \
+  } while (0)
+  if (C <= 256 * N) LP_BWD(1);
+  else if (C <= 512 * N) LP_BWD(2);
+  else LP_BWD(4);
+#undef LP_BWD
+  return hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+// How a row of n classes is cut: lanes a block, vectors a lane, segments
+// a row.  Returns segments, or 0 where n is over what they can hold.
+int lp_plan(long rows, long n, int kind, int* lanes, int* nv) {
+  const long N = kind == 0 ? 4 : 8;
+  const long v = (n + N - 1) / N;          // vectors a row
+  if (v <= 128) {
+    *lanes = 64;
+    *nv = v <= 64 ? 1 : 2;
+    return 1;
+  }
+  *lanes = 256;
+  *nv = 1;
+  while (*nv < 8 && v > 256L * *nv) {
+    const long segs = (v + 256L * *nv - 1) / (256L * *nv);
+    if (rows * segs <= 1024 && segs <= 64) break;
+    *nv *= 2;
+  }
+  const long segs = (v + 256L * *nv - 1) / (256L * *nv);
+  return segs <= MAXSEG ? (int)segs : 0;
+}
+
+// kind: 0 f32, 1 f16, 2 bf16
+hipError_t launch_lp_fwd(const void* x, const long* labels, float* logp,
+                         float* entropy, float* top_logp, long* top_idx,
+                         float* stat, float* psum,
+                         unsigned long long* pkey, long rows, int n,
+                         long ldx, int segs, int lanes, int nv, int k,
+                         int kind, hipStream_t stream) {
+  const FwdArgs a = {x, labels, logp, entropy, top_logp, top_idx, stat,
+                     psum, pkey, rows, n, ldx, segs, k, lanes, nv};
+  if (kind == 0) return fwd<float>(a, stream);
+  if (kind == 1) return fwd<_Float16>(a, stream);
+  return fwd<__bf16>(a, stream);
+}
+
+hipError_t launch_lp_bwd(const void* x, const long* labels,
+                         const long* top_idx, const float* stat,
+                         const float* dlogp, const float* dentropy,
+                         const float* dtop, void* dx, long rows, int n,
+                         int C, long ldx, int k, int kind,
+                         hipStream_t stream) {
+  if (kind == 0)
+    return bwd<float>(x, labels, top_idx, stat, dlogp, dentropy, dtop, dx,
+                      rows, n, C, ldx, k, stream);
+  if (kind == 1)
+    return bwd<_Float16>(x, labels, top_idx, stat, dlogp, dentropy, dtop,
+                         dx, rows, n, C, ldx, k, stream);
+  return bwd<__bf16>(x, labels, top_idx, stat, dlogp, dentropy, dtop, dx,
+                     rows, n, C, ldx, k, stream);
+}
+
+}  // extern "C"

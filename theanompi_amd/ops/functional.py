@@ -16,7 +16,6 @@ including conv (reference: the ops of Theano-MPI's layer library
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from theanompi_amd import ops as _ops
 
@@ -175,6 +174,7 @@ def muon_update_ref(w, g, v, out, keep, rate, momentum, phase, steps):
 
 # ---------------------------------------------------------------------------
 # GPU autograd wrappers (stateless ops). Each calls theanompi_amd._C.
+# (layernorm and label_logprobs have their nodes there, in bindings.cpp.)
 # ---------------------------------------------------------------------------
 
 class _MaxPool2dFn(torch.autograd.Function):
@@ -411,45 +411,6 @@ class _SoftmaxXentFn(torch.autograd.Function):
         return dlogits, None, None
 
 
-class _LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gamma, beta, eps, n):
-        y, stat = _ops.ext().ln_fwd(x, gamma, beta, n, eps)
-        # stat = per-row mean and 1/std: the backward re-reads x
-        ctx.save_for_backward(x, gamma, stat)
-        ctx.n = n
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, gamma, stat = ctx.saved_tensors
-        dx, dgamma, dbeta = _ops.ext().ln_bwd(dy, x, gamma, stat, ctx.n)
-        return dx, dgamma, dbeta, None, None
-
-
-class _LabelLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, n, top):
-        logp, entropy, top_logp, top_idx, stat = _ops.ext().lp_fwd(
-            logits, labels, n, top)
-        ctx.save_for_backward(logits, labels, top_idx, stat)
-        ctx.n = n
-        ctx.mark_non_differentiable(top_idx)
-        ctx.set_materialize_grads(False)
-        return logp, entropy, top_logp, top_idx
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dlogp, dentropy, dtop, _):
-        logits, labels, top_idx, stat = ctx.saved_tensors
-        if dlogp is None and dentropy is None and dtop is None:
-            return None, None, None, None
-        dx = _ops.ext().lp_bwd(logits, labels, top_idx, stat, dlogp,
-                               dentropy, dtop, ctx.n)
-        return dx, None, None, None
-
-
 # ---------------------------------------------------------------------------
 # public dispatchers
 # ---------------------------------------------------------------------------
@@ -582,8 +543,8 @@ def layernorm(x, gamma, beta, eps=1e-5, n_features=None):
         raise ValueError(f"eps must not be negative, not {eps}")
     n = _check_count(n_features, c, "n_features")
     if x.is_cuda:
-        return _LayerNormFn.apply(x, gamma.contiguous(), beta.contiguous(),
-                                  eps, n)
+        return _ops.ext().layernorm(x, gamma.contiguous(),
+                                    beta.contiguous(), eps, n)
     return layernorm_ref(x, gamma, beta, eps, n)
 
 
@@ -624,7 +585,8 @@ def label_logprobs(logits, labels, n_classes=None, top=0):
         raise ValueError(f"top must be a whole number from 0 to "
                          f"{min(n, TOP_MAX)}, not {top!r}")
     if logits.is_cuda:
-        return _LabelLogprobsFn.apply(logits, labels.contiguous(), n, top)
+        return tuple(_ops.ext().label_logprobs(
+            logits, labels.contiguous(), n, top))
     return label_logprobs_ref(logits, labels, n, top)
 
 

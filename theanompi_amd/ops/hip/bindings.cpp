@@ -3,6 +3,7 @@
 // lives in the .hip files (hand-written CDNA4 kernels).
 
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <ATen/hip/HIPContext.h>
 #include <c10/hip/HIPStream.h>
@@ -1116,6 +1117,20 @@ static void check_same(const torch::Tensor& t, const torch::Tensor& x,
   TORCH_CHECK(t.device() == x.device(), name, " is on another device");
 }
 
+// Gradients that are differentiable no further: a second derivative
+// raises instead of coming out as 0.
+static torch::autograd::variable_list once(
+    std::vector<torch::Tensor> grads,
+    std::initializer_list<torch::Tensor> none) {
+  if (torch::GradMode::is_enabled()) {
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        "this operator is differentiable once", (int)grads.size());
+    grads = (*error)(std::move(grads));
+  }
+  grads.insert(grads.end(), none.begin(), none.end());
+  return grads;
+}
+
 // Rows of the last dimension at a uniform distance (a channel slice of a
 // wider buffer among them); anything else is laid out anew.
 static torch::Tensor as_rows(const torch::Tensor& t, long* ld) {
@@ -1208,6 +1223,36 @@ static std::vector<torch::Tensor> ln_bwd(torch::Tensor dy,
   return {dx, dgamma, dbeta};
 }
 
+// The autograd node is built here rather than in Python: forward and
+// backward of a small row count cost less on the device than two trips
+// through Python cost the host (92 us a training pass at 128 x 4096).
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx,
+                               const torch::Tensor& x,
+                               const torch::Tensor& gamma,
+                               const torch::Tensor& beta, double eps,
+                               int64_t n) {
+    auto r = ln_fwd(x, gamma, beta, n, eps);
+    ctx->save_for_backward({x, gamma, r[1]});
+    ctx->saved_data["n"] = n;
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list dy) {
+    const auto s = ctx->get_saved_variables();
+    auto r = ln_bwd(dy[0], s[0], s[1], s[2], ctx->saved_data["n"].toInt());
+    return once(r, {torch::Tensor(), torch::Tensor()});
+  }
+};
+
+static torch::Tensor layernorm(const torch::Tensor& x,
+                               const torch::Tensor& gamma,
+                               const torch::Tensor& beta, double eps,
+                               int64_t n) {
+  return LayerNormFn::apply(x, gamma, beta, eps, n);
+}
+
 // ---- class log probabilities ------------------------------------------------
 
 static std::vector<torch::Tensor> lp_fwd(torch::Tensor x,
@@ -1287,6 +1332,39 @@ static torch::Tensor lp_bwd(torch::Tensor x, torch::Tensor labels,
                             dx.data_ptr(), rows, (int)n, (int)C, ld,
                             (int)k, kind, cur_stream()));
   return dx;
+}
+
+struct LabelLogprobsFn : torch::autograd::Function<LabelLogprobsFn> {
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext* ctx, const torch::Tensor& logits,
+      const torch::Tensor& labels, int64_t n, int64_t k) {
+    auto r = lp_fwd(logits, labels, n, k);
+    ctx->save_for_backward({logits, labels, r[3], r[4]});
+    ctx->saved_data["n"] = n;
+    ctx->mark_non_differentiable({r[3]});
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1], r[2], r[3]};
+  }
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list d) {
+    const auto s = ctx->get_saved_variables();
+    auto opt = [](const torch::Tensor& t) {
+      return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt;
+    };
+    torch::Tensor none;
+    if (!d[0].defined() && !d[1].defined() && !d[2].defined())
+      return {none, none, none, none};
+    auto dx = lp_bwd(s[0], s[1], s[2], s[3], opt(d[0]), opt(d[1]),
+                     opt(d[2]), ctx->saved_data["n"].toInt());
+    return once({dx}, {none, none, none});
+  }
+};
+
+static std::vector<torch::Tensor> label_logprobs(
+    const torch::Tensor& logits, const torch::Tensor& labels, int64_t n,
+    int64_t k) {
+  return LabelLogprobsFn::apply(logits, labels, n, k);
 }
 
 // ---- Newton-Schulz / orthogonalised momentum --------------------------------
@@ -1503,10 +1581,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gather_multi_run", &gather_multi_run);
   m.def("transpose_multi_make", &transpose_multi_make);
   m.def("transpose_multi_run", &transpose_multi_run);
-  m.def("ln_fwd", &ln_fwd);
-  m.def("ln_bwd", &ln_bwd);
-  m.def("lp_fwd", &lp_fwd);
-  m.def("lp_bwd", &lp_bwd);
+  m.def("layernorm", &layernorm);
+  m.def("label_logprobs", &label_logprobs);
   m.def("orthogonalize", &orthogonalize);
   m.def("muon_update", &muon_update);
 }

@@ -129,6 +129,54 @@ DEV void glds16(const void* gsrc, void* lds_base) {
                                    16, 0, 0);
 }
 
+// Sums and maxima over aligned groups of W lanes (2 to 64), on every lane
+// of the group, without LDS: data-parallel moves within 16 lanes (pairs,
+// quads, then mirrors of 8 and of 16, which exchange the halves once
+// these are uniform), lane swaps of 16 and 32.  The order is fixed.
+template <int CTRL>
+DEV unsigned dpp_move(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf,
+                                               false);
+}
+
+template <int W, typename F>
+DEV unsigned lane_reduce(unsigned v, F f) {
+  if constexpr (W >= 2) v = f(v, dpp_move<0xB1>(v));    // lane ^ 1
+  if constexpr (W >= 4) v = f(v, dpp_move<0x4E>(v));    // lane ^ 2
+  if constexpr (W >= 8) v = f(v, dpp_move<0x141>(v));   // 7 - lane
+  if constexpr (W >= 16) v = f(v, dpp_move<0x140>(v));  // 15 - lane
+  if constexpr (W >= 32) {
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(r[0], r[1]);
+  }
+  if constexpr (W >= 64) {
+    auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = f(r[0], r[1]);
+  }
+  return v;
+}
+
+template <int W>
+DEV float lane_sum(float v) {
+  return __uint_as_float(lane_reduce<W>(
+      __float_as_uint(v), [](unsigned a, unsigned b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+      }));
+}
+template <int W>
+DEV float lane_max(float v) {
+  return __uint_as_float(lane_reduce<W>(
+      __float_as_uint(v), [](unsigned a, unsigned b) {
+        return __float_as_uint(
+            fmaxf(__uint_as_float(a), __uint_as_float(b)));
+      }));
+}
+template <int W>
+DEV unsigned lane_max(unsigned v) {
+  return lane_reduce<W>(v,
+                        [](unsigned a, unsigned b) { return a > b ? a : b; });
+}
+
 #define HIP_KERNEL_ASSERT_OK(expr)                                          \
   do {                                                                      \
     hipError_t _e = (expr);                                                 \

@@ -75,9 +75,7 @@ template <int TPR, int K>
 DEV void row_sum(float* v, float* red, int& turn) {
   constexpr int W = TPR < 64 ? TPR : 64;
 #pragma unroll
-  for (int off = W / 2; off > 0; off >>= 1)
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], off, 64);
+  for (int k = 0; k < K; ++k) v[k] = lane_sum<W>(v[k]);
   if constexpr (TPR > 64) {
     constexpr int WAVES = TPR / 64;
     float* r = red + turn * (WAVES * 2);

@@ -28,7 +28,11 @@ struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
 constexpr int KMAX = 32;       // alternatives
 constexpr int MAXSEG = 256;    // segments a row
 
-// what is kept of a row for the backward pass
+constexpr int CAP = 256;       // candidates a block may collect
+constexpr float LOG2E = 1.44269504f;
+
+// What is kept of a row for the backward pass; M = -inf: a row of masked
+// classes.
 struct RowStat { float M, logs, H; };
 
 // floats in an order that unsigned integers have: NaN above all, -0 as 0
@@ -37,34 +41,50 @@ DEV unsigned ordered(float f) {
   const unsigned u = __float_as_uint(f + 0.f);
   return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
+DEV float unordered(unsigned u) {
+  return __uint_as_float(u ^ ((u >> 31) ? 0x80000000u : 0xffffffffu));
+}
 
 // value and index in one key: larger value first, then lower index
 DEV unsigned long long top_key(float f, int idx) {
   return ((unsigned long long)ordered(f) << 32) | (unsigned)~idx;
 }
 DEV int key_index(unsigned long long k) { return (int)~(unsigned)k; }
+DEV float key_value(unsigned long long k) {
+  return unordered((unsigned)(k >> 32));
+}
 
-DEV float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    v = fmaxf(v, __shfl_xor(v, off, 64));
-  return v;
-}
-DEV float wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
-}
+// the largest of the wave's keys, on every lane
 DEV unsigned long long wave_max_key(unsigned long long v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const unsigned long long o = __shfl_xor(v, off, 64);
-    if (o > v) v = o;
-  }
-  return v;
+  const unsigned hi = (unsigned)(v >> 32);
+  const unsigned top = lane_max<64>(hi);
+  const unsigned low = lane_max<64>(hi == top ? (unsigned)v : 0u);
+  return (unsigned long long)top << 32 | low;
 }
 
-// one lane's NV vectors of a row, as loaded
+// The k-th largest (from 1) of the wave's 64 values, bit by bit: how many
+// lanes reach a value is a count of a ballot.  LOW: low bits that the
+// type leaves 0.
+template <int LOW>
+DEV float wave_kth(float v, int k) {
+  const unsigned u = ordered(v);
+  unsigned best = 0;
+#pragma unroll
+  for (int b = 31; b >= LOW; --b) {
+    const unsigned t = best | (1u << b);
+    if (__popcll(__ballot(u >= t)) >= k) best = t;
+  }
+  // negative numbers have their low bits the other way round
+  if (LOW > 0 && !(best >> 31)) best |= (1u << LOW) - 1u;
+  return unordered(best);
+}
+
+template <typename T> struct LowBits { static constexpr int V = 0; };
+template <> struct LowBits<_Float16> { static constexpr int V = 13; };
+template <> struct LowBits<__bf16> { static constexpr int V = 16; };
+
+// One lane's NV vectors of a row, as loaded; what is behind the row is at
+// -inf, as masked classes are.
 template <typename T, int LANES, int NV>
 struct Part {
   static constexpr int N = 16 / sizeof(T);
@@ -73,38 +93,63 @@ struct Part {
 
   DEV int col(int i, int j) const { return first + i * LANES * N + j; }
   DEV bool has(int i, int j) const { return col(i, j) < n; }
-  // what is behind the row is at -inf, as masked classes are
   DEV float get(int i, int j) const { return (float)c[i].t[j]; }
 
+  // an element by a number that is not known at compile time
+  DEV float pick(int i, int j) const {
+    const u32x4 u = c[i].u;
+    const int w = j * (int)sizeof(T) / 4;
+    const unsigned lo = w & 1 ? u[1] : u[0], hi = w & 1 ? u[3] : u[2];
+    const unsigned v = w & 2 ? hi : lo;
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(v);
+    } else {
+      const unsigned short h = (unsigned short)(j & 1 ? v >> 16 : v);
+      return (float)__builtin_bit_cast(T, h);
+    }
+  }
+
+  // All loads are issued before the first is waited for: vectors that
+  // the row does not fill load its start instead, and are overwritten.
   DEV void load(const T* row, int seg0, int n_) {
     first = seg0 + (int)threadIdx.x * N;
     n = n_;
+    if (n >= N) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (col(i, N - 1) < n) {
-        c[i].u = ((const any16*)(row + col(i, 0)))->v;
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          c[i].t[j] = has(i, j) ? row[col(i, j)] : (T)-__builtin_inff();
-      }
+      for (int i = 0; i < NV; ++i)
+        c[i].u = ((const any16*)(row + (has(i, N - 1) ? col(i, 0) : 0)))->v;
     }
+    if (seg0 + LANES * NV * N <= n) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (!has(i, N - 1)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) c[i].t[j] = (T)-__builtin_inff();
+      }
+    if (n % N == 0) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (has(i, 0) && !has(i, N - 1)) {
+#pragma unroll
+        for (int j = 0; j < N - 1; ++j)
+          if (has(i, j)) c[i].t[j] = row[col(i, j)];
+      }
   }
 };
 
-// What a row's sums give.  s is 0 where every class is masked.
-DEV void finish_row(const float M, const float s, const float t,
-                    RowStat& st) {
+// What a row's sums give.  s is 0 where every class is masked, and NaN
+// where a NaN or +inf is.
+DEV RowStat finish_row(float M, float s, float t) {
+  RowStat st;
   if (s == 0.f) {
     st.M = -__builtin_inff();
-    st.logs = 0.f;
-    st.H = 0.f;
+    st.logs = st.H = 0.f;
   } else {
-    // a NaN among masked classes alone must not pass for an empty row
     st.M = s == s ? M : s;
     st.logs = logf(s);
     st.H = st.logs - t / s;
   }
+  return st;
 }
 
 DEV float logp_of(const RowStat& st, float x) {
@@ -112,21 +157,25 @@ DEV float logp_of(const RowStat& st, float x) {
                                    : (x - st.M) - st.logs;
 }
 
-template <typename T>
-DEV void write_row(const T* row, const long* labels, RowStat* stat,
-                   float* logp, float* entropy, long r, int n,
-                   const RowStat& st) {
+DEV void write_row(RowStat* stat, float* logp, float* entropy, long r,
+                   int n, long lab, float xlab, const RowStat& st) {
   stat[r] = st;
-  const long lab = labels[r];
-  logp[r] = lab < 0 ? 0.f
-            : lab < n ? logp_of(st, (float)row[lab])
-                      : __builtin_nanf("");
+  logp[r] = lab < 0 ? 0.f : lab < n ? logp_of(st, xlab)
+                                    : __builtin_nanf("");
   entropy[r] = st.H;
 }
 
 // One segment of one row.  Where a row has one segment only (segs == 1)
 // its results are final; else psum [row][seg][3] and pkey [row][seg][k]
-// go to lp_join_k.
+// (sorted, 0 behind the last) go to lp_join_k.
+//
+// The top k in one pass: the k-th largest of a wave's 64 lane maxima is
+// a lower bound of the segment's k-th largest value, and so is the
+// largest of the waves' bounds.  Only what reaches it (a few more than
+// k) goes into a list in LDS, where a candidate's place is the number of
+// candidates before it.  A list that overflows (many equal values) and
+// rows with a NaN or +inf take the plain way: k times the best of what
+// comes after the one before.
 template <typename T, int LANES, int NV>
 __global__ __launch_bounds__(LANES) void lp_fwd_k(
     const T* __restrict__ x, const long* __restrict__ labels,
@@ -137,53 +186,104 @@ __global__ __launch_bounds__(LANES) void lp_fwd_k(
     int k) {
   constexpr int N = 16 / sizeof(T);
   constexpr int WAVES = LANES / 64;
-  __shared__ float red[3][WAVES];
-  __shared__ unsigned long long kred[2][WAVES];
+  constexpr float NINF = -__builtin_inff();
+  __shared__ float red[4][WAVES];
+  __shared__ unsigned long long list[CAP], kred[2][WAVES];
+  __shared__ int count;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const long r = blockIdx.x / segs;
   const int seg = (int)(blockIdx.x % segs);
+  const int seg0 = seg * LANES * NV * N;
   const T* row = x + r * ldx;
   Part<T, LANES, NV> p;
-  p.load(row, seg * LANES * NV * N, n);
+  p.load(row, seg0, n);
+  long lab = -1;
+  float xlab = 0.f;
+  if (threadIdx.x == 0) {
+    count = 0;
+    if (segs == 1) {
+      lab = labels[r];
+      if (lab >= 0 && lab < n) xlab = (float)row[lab];
+    }
+  }
 
-  float m = -__builtin_inff();
+  float vm[NV], m = NINF;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    vm[i] = NINF;
 #pragma unroll
-    for (int j = 0; j < N; ++j) m = fmaxf(m, p.get(i, j));
-  m = wave_max(m);
+    for (int j = 0; j < N; ++j) vm[i] = fmaxf(vm[i], p.get(i, j));
+    m = fmaxf(m, vm[i]);
+  }
+  float tau = k > 0 ? wave_kth<LowBits<T>::V>(m, k) : 0.f;
+  m = lane_max<64>(m);
   if (WAVES > 1) {
-    if (lane == 0) red[0][wave] = m;
+    if (lane == 0) { red[0][wave] = m; red[1][wave] = tau; }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, red[0][w]);
+    for (int w = 0; w < WAVES; ++w) {
+      m = fmaxf(m, red[0][w]);
+      tau = fmaxf(tau, red[1][w]);
+    }
+  } else {
+    __syncthreads();               // count
   }
   // a maximum of -inf (nothing but masked classes) cannot be taken off
-  const float m0 = m == -__builtin_inff() ? 0.f : m;
+  const float M = m == NINF ? 0.f : m;
   float s = 0.f, t = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float d = p.get(i, j) - m0;
-      const float e = __expf(d);
+      const float d = p.get(i, j) - M;
+      const float e = __builtin_amdgcn_exp2f(d * LOG2E);
       s += e;
-      t += e > 0.f ? e * d : 0.f;
+      t = fmaf(e, fmaxf(d, -200.f), t);     // e is 0 long before
     }
-  s = wave_sum(s);
-  t = wave_sum(t);
+  if (k > 0) {
+    const float least = fmaxf(tau, -__FLT_MAX__);    // above -inf
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (vm[i] >= least) {
+        unsigned hits = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          hits |= p.get(i, j) >= least ? 1u << j : 0u;
+        int at = atomicAdd(&count, __popc(hits));
+        while (hits) {
+          const int j = __ffs(hits) - 1;
+          hits &= hits - 1;
+          if (at < CAP) list[at] = top_key(p.pick(i, j), p.col(i, j));
+          ++at;
+        }
+      }
+    }
+    // fewer than k values above -inf, maybe: of the masked classes only
+    // the segment's first k can be called for
+    if (tau == NINF) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (p.get(0, j) == NINF && p.has(0, j) && p.col(0, j) - seg0 < k) {
+          const int at = atomicAdd(&count, 1);
+          if (at < CAP) list[at] = top_key(NINF, p.col(0, j));
+        }
+    }
+  }
+  s = lane_sum<64>(s);
+  t = lane_sum<64>(t);
   if (WAVES > 1) {
-    if (lane == 0) { red[1][wave] = s; red[2][wave] = t; }
+    if (lane == 0) { red[2][wave] = s; red[3][wave] = t; }
     __syncthreads();
     s = t = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) { s += red[1][w]; t += red[2][w]; }
+    for (int w = 0; w < WAVES; ++w) { s += red[2][w]; t += red[3][w]; }
+  } else {
+    __syncthreads();               // list
   }
-  RowStat st;
-  finish_row(m, s, t, st);
+  const RowStat st = finish_row(M, s, t);
   if (threadIdx.x == 0) {
     if (segs == 1) {
-      write_row(row, labels, stat, logp, entropy, r, n, st);
+      write_row(stat, logp, entropy, r, n, lab, xlab, st);
     } else {
       float* q = psum + (r * segs + seg) * 3;
       q[0] = m;
@@ -191,17 +291,33 @@ __global__ __launch_bounds__(LANES) void lp_fwd_k(
       q[2] = t;
     }
   }
-  // k times the best of what comes after the one before
+  auto put = [&](int place, unsigned long long key) {
+    if (segs == 1) {
+      top_idx[r * k + place] = key_index(key);
+      top_logp[r * k + place] = logp_of(st, key_value(key));
+    } else {
+      pkey[(r * segs + seg) * k + place] = key;
+    }
+  };
+  const int have = count;
+  if (have <= CAP && s == s) {
+    for (int a = threadIdx.x; a < have; a += LANES) {
+      const unsigned long long key = list[a];
+      int place = 0;
+      for (int b = 0; b < have; ++b) place += list[b] > key;
+      if (place < k) put(place, key);
+    }
+    for (int a = have + threadIdx.x; a < k; a += LANES) put(a, 0);
+    return;
+  }
   unsigned long long last = ~0ull;
   for (int a = 0; a < k; ++a) {
     unsigned long long best = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const unsigned long long key = top_key(p.get(i, j), p.col(i, j));
-        if (p.has(i, j) && key < last && key > best) best = key;
-      }
+    for (int col = seg0 + (int)threadIdx.x;
+         col < n && col < seg0 + LANES * NV * N; col += LANES) {
+      const unsigned long long key = top_key((float)row[col], col);
+      if (key < last && key > best) best = key;
+    }
     best = wave_max_key(best);
     if (WAVES > 1) {
       if (lane == 0) kred[a & 1][wave] = best;
@@ -211,15 +327,7 @@ __global__ __launch_bounds__(LANES) void lp_fwd_k(
         if (kred[a & 1][w] > best) best = kred[a & 1][w];
     }
     last = best;
-    if (threadIdx.x == 0) {
-      if (segs == 1) {
-        const int idx = key_index(best);
-        top_idx[r * k + a] = idx;
-        top_logp[r * k + a] = logp_of(st, (float)row[idx]);
-      } else {
-        pkey[(r * segs + seg) * k + a] = best;   // 0: no more there
-      }
-    }
+    if (threadIdx.x == 0) put(a, best);
   }
 }
 
@@ -236,7 +344,11 @@ __global__ __launch_bounds__(64) void lp_join_k(
   const long r = blockIdx.x;
   const int lane = threadIdx.x;
   const T* row = x + r * ldx;
+  const long lab = labels[r];
+  const float xlab = lab >= 0 && lab < n ? (float)row[lab] : 0.f;
   float m[H], s[H], t[H], M = -__builtin_inff();
+  unsigned long long head[H];      // each lane's segments' next best
+  int at[H];
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     const int g = lane + h * 64;
@@ -245,32 +357,24 @@ __global__ __launch_bounds__(64) void lp_join_k(
     s[h] = g < segs ? q[1] : 0.f;
     t[h] = g < segs ? q[2] : 0.f;
     M = fmaxf(M, m[h]);
-  }
-  M = wave_max(M);
-  float S = 0.f, U = 0.f;
-#pragma unroll
-  for (int h = 0; h < H; ++h) {
-    // a segment of masked classes has no maximum to be taken off; its
-    // sum is 0, or NaN where it has a NaN
-    const float d = m[h] == -__builtin_inff() ? 0.f : m[h] - M;
-    const float e = __expf(d);
-    S += e * s[h];
-    U += e > 0.f ? e * (t[h] + d * s[h]) : 0.f;   // d may be -3e38
-  }
-  S = wave_sum(S);
-  U = wave_sum(U);
-  RowStat st;
-  finish_row(M, S, U, st);
-  if (lane == 0) write_row(row, labels, stat, logp, entropy, r, n, st);
-  // each lane's segments' next best
-  unsigned long long head[H];
-  int at[H];
-#pragma unroll
-  for (int h = 0; h < H; ++h) {
-    const int g = lane + h * 64;
     at[h] = 0;
     head[h] = g < segs && k > 0 ? pkey[(r * segs + g) * k] : 0;
   }
+  M = lane_max<64>(M);
+  float S = 0.f, U = 0.f;
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    // a segment of masked classes has nothing to be taken off
+    const float d = m[h] == -__builtin_inff() ? 0.f : m[h] - M;
+    const float e = __builtin_amdgcn_exp2f(d * LOG2E);
+    S += e * s[h];
+    U += e > 0.f ? e * (t[h] + d * s[h]) : 0.f;   // d may be -3e38
+  }
+  S = lane_sum<64>(S);
+  U = lane_sum<64>(U);
+  const RowStat st = finish_row(M, S, U);
+  if (lane == 0)
+    write_row(stat, logp, entropy, r, n, lab, xlab, st);
   for (int a = 0; a < k; ++a) {
     unsigned long long best = 0;
 #pragma unroll
@@ -286,9 +390,8 @@ __global__ __launch_bounds__(64) void lp_join_k(
                       ? pkey[(r * segs + g) * k + at[h]] : 0;
       }
     if (lane == 0) {
-      const int idx = key_index(best);
-      top_idx[r * k + a] = idx;
-      top_logp[r * k + a] = logp_of(st, (float)row[idx]);
+      top_idx[r * k + a] = key_index(best);
+      top_logp[r * k + a] = logp_of(st, key_value(best));
     }
   }
 }
@@ -323,8 +426,9 @@ __global__ __launch_bounds__(256) void lp_bwd_k(
   auto plain = [&](float v) -> float {
     if (empty) return 0.f;
     const float lp = (v - st.M) - st.logs;
-    const float p = __expf(lp);
-    return p == 0.f ? 0.f : p * (c0 - dh * lp);
+    // p is 0 long before -200, where the product must not be 0 * inf
+    return __builtin_amdgcn_exp2f(lp * LOG2E)
+           * (c0 - dh * fmaxf(lp, -200.f));
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {

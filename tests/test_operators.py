@@ -557,11 +557,46 @@ def test_orthogonalize_gpu(shape, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("steps", [1, 2, 3, 8])
-def test_orthogonalize_gpu_steps(steps):
-    x = ns_inputs((90, 150), torch.float32, dev())
+@pytest.mark.parametrize("shape", [(90, 150), (40, 330)], ids=str)
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 8])
+def test_orthogonalize_gpu_steps(steps, shape):
+    x = ns_inputs(shape, torch.float32, dev())
     assert off(OF.orthogonalize(x, steps),
                ns_formula(x, steps)) < NS_TOL * max(1, steps / 5)
+
+
+def ns_recurrence(x, steps=5):
+    """The definition in 64 bits, where a singular value decomposition
+    would take minutes."""
+    x = x.double()
+    x = x / (torch.linalg.vector_norm(x) + 1e-7)
+    a, b, c = OF.NS_QUINTIC
+    for _ in range(steps):
+        g = x @ x.t()
+        x = a * x + (b * g + c * g @ g) @ x
+    return x
+
+
+# One shape for each way through the general kernels: k cut into runs and
+# not, tiles of 64, 128 and 256, two steps at a time (n >= 2m) and one,
+# and the padding of m and n within a tile.
+@gpu
+@pytest.mark.parametrize("shape,steps", [
+    ((70, 5000), 5), ((700, 1100), 5), ((1300, 4650), 5), ((1300, 4650), 4),
+    ((2500, 2500), 5), ((2050, 8200), 5), ((4097, 4100), 3)], ids=str)
+def test_orthogonalize_gpu_large(shape, steps):
+    x = ns_inputs(shape, torch.float32, dev())
+    want = ns_recurrence(x, steps)
+    assert off(OF.orthogonalize(x, steps), want) < NS_TOL
+    tall = x.t().contiguous()
+    assert off(OF.orthogonalize(tall, steps).t(), want) < NS_TOL
+
+
+@gpu
+def test_orthogonalize_gpu_same_bits_again():
+    for shape in ((64, 576), (300, 2000), (1300, 4650)):
+        x = ns_inputs(shape, torch.float32, dev())
+        assert torch.equal(OF.orthogonalize(x), OF.orthogonalize(x))
 
 
 @gpu
@@ -660,6 +695,28 @@ def test_muon_update_cpu(phase):
 def test_muon_update_gpu(phase):
     muon_check([(16, 27), (64, 576), (10, 256), (256, 10), (1, 1),
                 (3, 48, 70), (130, 130)], dev(), phase)
+
+
+@gpu
+@pytest.mark.parametrize("shapes", [
+    [(16, 27), (64, 576), (10, 256), (2, 3, 50)],      # few rows alone
+    [(16, 27), (128, 700), (1300, 4700), (64, 64)]], ids=["few", "mixed"])
+def test_muon_update_gpu_kinds(shapes):
+    """Lists whose matrices take the same kernels and several kinds."""
+    muon_check([s for s in shapes if s[0] < 1000], dev())
+    if len(shapes[2]) == 2 and shapes[2][0] > 1000:
+        ws, gs, vs, outs = muon_inputs(shapes, dev())
+        want = [(w.double() * 0.998, 0.9 * v.double() - g.double())
+                for w, g, v in zip(ws, gs, vs)]
+        OF.muon_update(ws, gs, vs, outs, [0.02] * 4, [0.1] * 4, 0.9,
+                       [5.0] * 4)
+        for w, v, (keep, vel) in zip(ws, vs, want):
+            close(v, vel, 3 * U * (vel.abs() + 0.02), "v")
+            o = ns_recurrence(vel if vel.shape[0] <= vel.shape[1]
+                              else vel.t())
+            diff = w.double() - (keep + 0.1 * o)
+            assert float(diff.norm()) <= (
+                6 * U * float(keep.norm()) + 0.1 * NS_TOL * float(o.norm()))
 
 
 @gpu

@@ -156,6 +156,7 @@ extern "C" {
 hipError_t launch_ns_sum(NsArgs*, hipStream_t);
 hipError_t launch_ns_load(NsArgs*, hipStream_t);
 hipError_t launch_ns_gemm(NsArgs*, int, hipStream_t);
+hipError_t launch_ns_few(NsArgs*, hipStream_t);
 }
 
 // pick a K-split so small-M GEMMs (FC layers at batch<=256) still fill
@@ -1369,17 +1370,29 @@ static std::vector<torch::Tensor> label_logprobs(
 
 // ---- Newton-Schulz / orthogonalised momentum --------------------------------
 
+// Which kernels a matrix takes: 0, those for few rows; else the tile of
+// the general ones, larger where there is work enough for all compute
+// units.
+static int ns_tile(const NsProb& p) {
+  if (p.m <= 64) return 0;
+  const long size = (long)p.batch * p.m * p.n;
+  return size >= (1L << 24) ? 256 : size >= 6000000 ? 128 : 64;
+}
+
 // Fills in shapes and workspace of `a` (count problems that have m, n,
 // batch and pointers to their data), and returns the workspace.
 static torch::Tensor ns_workspace(NsArgs& a,
                                   const torch::TensorOptions& opts) {
-  const long tile = NS_TILE;
+  const long tile = a.tile ? a.tile : 64;
   long total = 0;
   auto take = [&](long bytes) {
     const long at = total;
     total += (bytes + 255) / 256 * 256;
     return at;
   };
+  long blocks = 0;                   // of 64 columns, few rows
+  for (int i = 0; i < a.count; ++i)
+    blocks += (long)a.p[i].batch * ((a.p[i].n + 63) / 64);
   std::vector<long> at;
   for (int i = 0; i < a.count; ++i) {
     NsProb& p = a.p[i];
@@ -1387,40 +1400,92 @@ static torch::Tensor ns_workspace(NsArgs& a,
     p.np = (int)((p.n + tile - 1) / tile * tile);
     const long len = (long)p.m * p.n;
     long parts = (len + 4095) / 4096;
-    p.parts = (int)(parts < 256 ? parts : 256);
-    const long x = 4L * p.batch * p.mp * p.np;
-    const long s = 4L * p.batch * p.mp * p.mp;
-    at.push_back(take(x));
-    at.push_back(take(x));
-    at.push_back(take(s));
-    at.push_back(take(s));
+    p.parts = (int)(parts < 2048 ? parts : 2048);
+    at.push_back(take(4L * p.batch * p.mp * p.np));
+    at.push_back(take(4L * p.batch * p.mp * p.np));
     at.push_back(take(8L * p.batch * p.parts));
     at.push_back(take(4L * p.batch));
+    if (a.tile) {
+      for (int k = 0; k < 3; ++k)
+        at.push_back(take(4L * p.batch * p.mp * p.mp));
+    } else {
+      // about as many blocks as compute units, and no more than 16 a
+      // matrix, whose shares each of them adds up
+      const long cols = p.np / 64;
+      long groups = blocks <= 256 ? cols : (cols * 256 + blocks - 1) / blocks;
+      p.groups = (int)(groups < 16 ? groups : 16);
+      for (int k = 0; k < 3; ++k)
+        at.push_back(take(k < 2 ? 4L * p.batch * p.groups * 64 * 64 : 0));
+    }
   }
+  const long partial = take(a.tile ? NS_SLOTS * tile * tile * 4 : 0);
   auto ws = torch::empty({total}, opts.dtype(torch::kUInt8));
   char* base = (char*)ws.data_ptr();
+  a.partial = (float*)(base + partial);
   for (int i = 0; i < a.count; ++i) {
     NsProb& p = a.p[i];
-    p.X[0] = base + at[i * 6];
-    p.X[1] = base + at[i * 6 + 1];
-    p.A = base + at[i * 6 + 2];
-    p.B = base + at[i * 6 + 3];
-    p.part = (double*)(base + at[i * 6 + 4]);
-    p.shift = (float*)(base + at[i * 6 + 5]);
+    const long* o = &at[i * 7];
+    p.X[0] = base + o[0];
+    p.X[1] = base + o[1];
+    p.part = (double*)(base + o[2]);
+    p.shift = (float*)(base + o[3]);
+    if (a.tile) {
+      for (int k = 0; k < 3; ++k) p.S[k] = base + o[4 + k];
+    } else {
+      p.share[0] = (float*)(base + o[4]);
+      p.share[1] = (float*)(base + o[5]);
+    }
   }
   return ws;
 }
 
-static void ns_run(NsArgs& a, long steps, hipStream_t stream) {
+// The whole iteration for the matrices of `a`, which take the same
+// kernels.
+static void ns_run(NsArgs& a, long steps,
+                   const torch::TensorOptions& opts) {
+  auto ws = ns_workspace(a, opts);
+  auto stream = cur_stream();
   a.steps = (int)steps;
   CHECK_HIP(launch_ns_sum(&a, stream));
   if (a.phase == 1) return;
   CHECK_HIP(launch_ns_load(&a, stream));
-  for (int s = 0; s < (int)steps; ++s) {
-    a.step = s;
-    a.last = s + 1 == (int)steps;
-    for (int mode = 0; mode < 3; ++mode)
-      CHECK_HIP(launch_ns_gemm(&a, mode, stream));
+  if (!a.tile) {
+    a.pair = -1;
+    CHECK_HIP(launch_ns_few(&a, stream));
+    for (int left = (int)steps; left > 0; ++a.step) {
+      a.pair = left >= 2;
+      left -= 1 + a.pair;
+      a.last = left == 0;
+      CHECK_HIP(launch_ns_few(&a, stream));
+    }
+    return;
+  }
+  // Two steps at a time cost a Gram matrix and an X product less and
+  // three products of m x m more: at m = 4096 406 + 750 us against 650,
+  // at n = 9216.  They pay from about n = 2m on, where the device is full.
+  bool pairs = a.tile >= 128;
+  for (int i = 0; i < a.count; ++i)
+    pairs = pairs && a.p[i].n >= 2L * a.p[i].m;
+  auto product = [&](int mode, int s1, int s2, int to, int poly) {
+    a.s1 = s1;
+    a.s2 = s2;
+    a.to = to;
+    a.poly = poly;
+    CHECK_HIP(launch_ns_gemm(&a, mode, stream));
+  };
+  for (int left = (int)steps; left > 0; ++a.step) {
+    const bool two = pairs && left >= 2;
+    left -= two ? 2 : 1;
+    a.last = left == 0;
+    product(0, 0, 0, 0, 0);              // S0 = A
+    product(1, 0, 0, 1, 1);              // S1 = M
+    if (two) {
+      product(1, 1, 0, 2, 0);            // S2 = M A
+      product(1, 1, 2, 0, 0);            // S0 = A' = M A M
+      product(1, 0, 0, 2, 1);            // S2 = M'
+      product(1, 2, 1, 0, 0);            // S0 = M' M
+    }
+    product(2, two ? 0 : 1, 0, 0, 0);
   }
 }
 
@@ -1451,8 +1516,8 @@ static torch::Tensor orthogonalize(torch::Tensor x, long steps) {
   p.out = out.data_ptr();
   p.kind = kind;
   ns_shape(p, x.size(-2), x.size(-1), x.dim() == 3 ? x.size(0) : 1);
-  auto ws = ns_workspace(a, x.options());
-  ns_run(a, steps, cur_stream());
+  a.tile = ns_tile(p);
+  ns_run(a, steps, x.options());
   return out;
 }
 
@@ -1494,27 +1559,45 @@ static void muon_update(std::vector<torch::Tensor> ws,
     }
   }
   c10::DeviceGuard guard(ws[0].device());
-  size_t i = 0;
-  while (i < n) {
-    NsArgs a;
-    std::memset(&a, 0, sizeof(a));
-    a.phase = (int)phase;
-    a.mu = (float)mu;
-    for (; i < n && a.count < NS_MAXP; ++i) {
-      if (!ws[i].numel()) continue;
-      NsProb& p = a.p[a.count++];
-      p.w = ws[i].data_ptr<float>();
-      p.v = vs[i].data_ptr<float>();
-      p.g = phase != 2 ? gs[i].data_ptr<float>() : nullptr;
-      p.copy = outs[i].numel() ? outs[i].data_ptr() : nullptr;
-      p.keep = (float)keeps[i];
-      p.rate = (float)rates[i];
-      ns_shape(p, ws[i].size(-2), ws[i].size(-1),
-               ws[i].dim() == 3 ? ws[i].size(0) : 1);
+  // One pass for each kind of kernels, NS_MAXP matrices at a time.  Few
+  // rows have kernels of their own only where no others take the general
+  // ones: beside those they cost next to nothing (the 17 weights of a
+  // wide residual network: 231 us together, 278 us apart).
+  bool general = false;
+  auto kind = [&](const NsProb& p) {
+    const int tile = ns_tile(p);
+    return tile == 0 && general ? 64 : tile;
+  };
+  for (size_t i = 0; i < n; ++i) {
+    NsProb p;
+    ns_shape(p, ws[i].size(-2), ws[i].size(-1),
+             ws[i].dim() == 3 ? ws[i].size(0) : 1);
+    general = general || ns_tile(p) == 64;
+  }
+  for (int tile : {0, 64, 128, 256}) {
+    size_t i = 0;
+    while (i < n) {
+      NsArgs a;
+      std::memset(&a, 0, sizeof(a));
+      a.phase = (int)phase;
+      a.mu = (float)mu;
+      a.tile = tile;
+      for (; i < n && a.count < NS_MAXP; ++i) {
+        if (!ws[i].numel()) continue;
+        NsProb& p = a.p[a.count];
+        ns_shape(p, ws[i].size(-2), ws[i].size(-1),
+                 ws[i].dim() == 3 ? ws[i].size(0) : 1);
+        if (kind(p) != tile) continue;
+        ++a.count;
+        p.w = ws[i].data_ptr<float>();
+        p.v = vs[i].data_ptr<float>();
+        p.g = phase != 2 ? gs[i].data_ptr<float>() : nullptr;
+        p.copy = outs[i].numel() ? outs[i].data_ptr() : nullptr;
+        p.keep = (float)keeps[i];
+        p.rate = (float)rates[i];
+      }
+      if (a.count) ns_run(a, steps, ws[0].options());
     }
-    if (!a.count) break;
-    auto buf = ns_workspace(a, ws[0].options());
-    ns_run(a, steps, cur_stream());
   }
 }
 

@@ -2,7 +2,7 @@
 // update around it.
 //
 //   X = G / (|G|_F + 1e-7), on the orientation with m <= n rows
-//   steps times:   A = X X^T     B = a I + b A + c A A     X <- B X
+//   steps times:   A = X X^T     M = a I + b A + c A A     X <- M X
 //   with (a, b, c) = (3.4445, -4.775, 2.0315)
 //   update:  v = mu v - g    w = (1 - lr wd) w + lr scale NS(v)
 //
@@ -15,15 +15,16 @@
 // products, hi*hi + hi*lo + lo*hi, in fp32 accumulators: the accuracy of
 // fp32 at a third of the fp16 rate, five times the fp32 matrix rate.
 // The entries stay far below fp16's largest: singular values of X are at
-// most 1.21 over the whole iteration, those of B at most 3.45.
+// most 1.21 over the whole iteration, those of M at most 3.45.
 //
 // Layout: a "split" matrix of R rows and K columns (both padded to the
 // tile with zeros, which every step keeps) is [R][K/32][2][32] halves,
 // 32 hi then 32 lo: a 32-deep slice of a row is one 128-byte line.
-// A and B are symmetric: only tiles on and below the diagonal are
+// A, M and their products are symmetric: only tiles on and below the diagonal are
 // computed, each written twice.
 //
-// All matrices of a call go through each step in one launch; what a
+// Where n is large against m, two steps use X once (see ns_run): what X
+// X^T is after a step is A' = M A M, and X <- (M' M) X.  All matrices of a call go through each step in one launch; what a
 // kernel needs to know of them travels in its arguments, so a captured
 // graph holds it.
 
@@ -32,18 +33,19 @@
 
 namespace {
 
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
 typedef __attribute__((ext_vector_type(4))) _Float16 half4;
 typedef __attribute__((ext_vector_type(8))) _Float16 half8;
 typedef __attribute__((ext_vector_type(4))) __fp16 fp16x4;
 typedef __attribute__((address_space(3))) fp16x4 lds_fp16x4;
 
-constexpr int TILE = NS_TILE;
 constexpr float SCALE = 4096.f;   // of every split matrix
 constexpr float QA = 3.4445f, QB = -4.775f, QC = 2.0315f;
 
-DEV int find(const NsArgs& a, int block) {
+DEV int find(const NsArgs& a, int at) {
   int i = 0;
-  while (i + 1 < a.count && block >= a.start[i + 1]) ++i;
+  while (i + 1 < a.count && at >= a.start[i + 1]) ++i;
   return i;
 }
 
@@ -58,44 +60,69 @@ DEV void split(float v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(v - (float)hi);
 }
 
-// momentum (phase 0, 1) and the sum of squares, in 64 bits: no gradient
-// that fp32 holds is too small or too large for it
-__global__ __launch_bounds__(256) void ns_sum_k(const NsArgs a) {
-  const int i = find(a, blockIdx.x);
-  const NsProb& p = a.p[i];
-  const int b = blockIdx.x - a.start[i];
-  const int part = b % p.parts;
-  const long mat = b / p.parts;
-  const long len = (long)p.m * p.n;
-  double s = 0.0;
-  for (long e = part * 256L + threadIdx.x; e < len; e += p.parts * 256L) {
-    const long at = mat * len + e;
-    float f;
-    if (p.in) {
-      f = load_in(p, at);
-    } else if (a.phase == 2) {
-      f = p.v[at];
-    } else {
-      f = a.mu * p.v[at] - p.g[at];
-      p.v[at] = f;
-    }
-    s += (double)f * f;
-  }
-  if (a.phase == 1) return;
-  __shared__ double red[256];
+// sum over a block of 256, on every thread
+DEV double block_sum(double s, double* red) {
   red[threadIdx.x] = s;
   __syncthreads();
   for (int h = 128; h > 0; h >>= 1) {
     if ((int)threadIdx.x < h) red[threadIdx.x] += red[threadIdx.x + h];
     __syncthreads();
   }
-  if (threadIdx.x == 0) p.part[mat * p.parts + part] = red[0];
+  return red[0];
+}
+
+// momentum (phase 0, 1) and the sum of squares, in 64 bits: no gradient
+// that fp32 holds is too small or too large for it
+__global__ __launch_bounds__(256) void ns_sum_k(const NsArgs a) {
+  __shared__ double red[256];
+  const int i = find(a, blockIdx.x);
+  const NsProb& p = a.p[i];
+  const int b = blockIdx.x - a.start[i];
+  const int part = b % p.parts;
+  const long mat = b / p.parts;
+  const long len = (long)p.m * p.n, base = mat * len;
+  const long step = p.parts * 1024L;
+  double s = 0.0;
+  // four elements a thread and turn; rows meet 16 bytes only where the
+  // matrix does, and memory takes them where they are
+  for (long e = (part * 256L + threadIdx.x) * 4; e < len; e += step) {
+    const long at = base + e;
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool whole = e + 4 <= len;
+    if (p.in) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (e + j < len) f[j] = load_in(p, at + j);
+    } else if (whole) {
+      const f32x4 v = __builtin_bit_cast(f32x4, ((any16*)(p.v + at))->v);
+      if (a.phase == 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = v[j];
+      } else {
+        f32x4 g = __builtin_bit_cast(f32x4, ((const any16*)(p.g + at))->v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = g[j] = a.mu * v[j] - g[j];
+        ((any16*)(p.v + at))->v = __builtin_bit_cast(u32x4, g);
+      }
+    } else {
+      for (int j = 0; e + j < len; ++j) {
+        f[j] = p.v[at + j];
+        if (a.phase != 2) p.v[at + j] = f[j] = a.mu * f[j] - p.g[at + j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += (double)f[j] * f[j];
+  }
+  if (a.phase == 1) return;
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) p.part[mat * p.parts + part] = s;
 }
 
 // X / (|X| + 1e-7) as a split matrix, a 64 x 64 tile a block, turned if
 // the matrix is tall
 __global__ __launch_bounds__(256) void ns_load_k(const NsArgs a) {
   __shared__ float tile[64][65];
+  __shared__ double red[256];
   const int i = find(a, blockIdx.x);
   const NsProb& p = a.p[i];
   const int tiles = (p.mp / 64) * (p.np / 64);
@@ -103,8 +130,22 @@ __global__ __launch_bounds__(256) void ns_load_k(const NsArgs a) {
   const long mat = b / tiles;
   b %= tiles;
   const int r0 = b / (p.np / 64) * 64, c0 = b % (p.np / 64) * 64;
+  // rows and columns as stored
+  const int sr0 = p.tall ? c0 : r0, sc0 = p.tall ? r0 : c0;
+  const int rows = p.tall ? p.n : p.m, cols = p.tall ? p.m : p.n;
+  const long base = mat * rows * (long)cols;
+  float f[16];
+#pragma unroll
+  for (int t = 0; t < 16; ++t) {
+    const int r = sr0 + t * 4 + (threadIdx.x >> 6);
+    const int c = sc0 + (threadIdx.x & 63);
+    const long at = base + (long)r * cols + c;
+    f[t] = r < rows && c < cols ? (p.in ? load_in(p, at) : p.v[at]) : 0.f;
+  }
   double sum = 0.0;
-  for (int k = 0; k < p.parts; ++k) sum += p.part[mat * p.parts + k];
+  for (int k = threadIdx.x; k < p.parts; k += 256)
+    sum += p.part[mat * p.parts + k];
+  sum = block_sum(sum, red);
   // A norm far below 1e-7 leaves X far below 1, and fp16 would lose it:
   // it is kept 2^e times as large, e so that `steps` growths by QA end
   // below 1 all the same.
@@ -115,236 +156,752 @@ __global__ __launch_bounds__(256) void ns_load_k(const NsArgs a) {
   if (e < 0) e = 0;
   const double inv = ldexp((double)SCALE * inv0, e);
   if (b == 0 && threadIdx.x == 0) p.shift[mat] = (float)ldexp(1.0, -e);
-  // rows and columns as stored
-  const int sr0 = p.tall ? c0 : r0, sc0 = p.tall ? r0 : c0;
-  const int rows = p.tall ? p.n : p.m, cols = p.tall ? p.m : p.n;
-  const long base = mat * rows * (long)cols;
-  for (int t = threadIdx.x; t < 4096; t += 256) {
-    const int r = sr0 + t / 64, c = sc0 + t % 64;
-    float f = 0.f;
-    if (r < rows && c < cols) {
-      const long at = base + (long)r * cols + c;
-      f = p.in ? load_in(p, at) : p.v[at];
-      f = (float)(f * inv);
-    }
-    tile[t / 64][t % 64] = f;
-  }
+#pragma unroll
+  for (int t = 0; t < 16; ++t)
+    tile[t * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] =
+        (float)(f[t] * inv);
   __syncthreads();
   _Float16* X = (_Float16*)p.X[0] + mat * 2 * p.mp * (long)p.np;
-  for (int t = threadIdx.x; t < 4096; t += 256) {
-    const int r = t / 64, c = t % 64;
-    _Float16 hi, lo;
-    split(p.tall ? tile[c][r] : tile[r][c], hi, lo);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    // 8 columns a thread: 16 bytes of hi, 16 of lo
+    const int r = t * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
+    half8 hi, lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      _Float16 h, l;
+      split(p.tall ? tile[c + j][r] : tile[r][c + j], h, l);
+      hi[j] = h;
+      lo[j] = l;
+    }
     _Float16* d = X + ((long)(r0 + r) * p.np + c0) * 2 + c / 32 * 64 + c % 32;
-    d[0] = hi;
-    d[32] = lo;
+    *(half8*)d = hi;
+    *(half8*)(d + 32) = lo;
   }
 }
 
-enum { GRAM, POLY, APPLY };
+enum { GRAM, SQUARE, APPLY };
 
-// C = Aop * Bop.  Aop: rows of a split matrix, k along them.  Bop: the
-// same (GRAM, POLY), or k down the rows of a split matrix (APPLY).
-// Two LDS buffers: the next 32-deep slice is on its way (16 bytes a
-// lane, straight to LDS) while the present one is multiplied.
-template <int MODE, int BT>
-__global__ __launch_bounds__(256) void ns_gemm_k(const NsArgs a) {
-  constexpr int F = BT / 32;                 // 16-wide fragments a wave
-  __shared__ __align__(16) _Float16 As[2][BT * 64];
-  __shared__ __align__(16) _Float16 Bs[2][BT * 64];
-  const int i = find(a, blockIdx.x);
-  const NsProb& p = a.p[i];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int b = blockIdx.x - a.start[i], ti, tj;
-  long mat;
-  if (MODE == APPLY) {
-    const int tn = p.np / BT, tiles = p.mp / BT * tn;
-    mat = b / tiles;
-    b %= tiles;
-    ti = b / tn;
-    tj = b % tn;
-  } else {
-    const int t = p.mp / BT, tiles = t * (t + 1) / 2;
-    mat = b / tiles;
-    b %= tiles;
-    ti = 0;
-    while ((ti + 1) * (ti + 2) / 2 <= b) ++ti;
-    tj = b - ti * (ti + 1) / 2;
+template <int V> struct Int { static constexpr int value = V; };
+
+// what lanes of a wave hand each other through LDS stays in order
+DEV void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// N values of row R from column c on, into a split matrix
+template <int N>
+DEV void store_split(_Float16* m, int ld, int R, int c, const float* f) {
+  _Float16* d = m + ((long)R * ld + c / 32 * 32) * 2 + c % 32;
+#pragma unroll
+  for (int k = 0; k < N; k += 8) {
+    half8 hi, lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      _Float16 h, l;
+      split(f[k + j], h, l);
+      hi[j] = h;
+      lo[j] = l;
+    }
+    *(half8*)(d + k) = hi;
+    *(half8*)(d + k + 32) = lo;
   }
+}
+
+// the same into the result: N values of row R as stored, of `cols`
+template <int N>
+DEV void store_result(const NsProb& p, long at, int c, int cols,
+                      const float* f) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (c + j >= cols) break;
+    if (p.w) {
+      const float w = p.keep * p.w[at + j] + p.rate * f[j];
+      p.w[at + j] = w;
+      if (p.copy) ((__bf16*)p.copy)[at + j] = (__bf16)w;
+    } else if (p.kind == 0) {
+      ((float*)p.out)[at + j] = f[j];
+    } else if (p.kind == 1) {
+      ((_Float16*)p.out)[at + j] = (_Float16)f[j];
+    } else {
+      ((__bf16*)p.out)[at + j] = (__bf16)f[j];
+    }
+  }
+}
+
+// 32-deep slices of split matrices in LDS, in 16-byte pieces.  ROWS rows
+// from row0, k to k + 32 along them: piece q of row r holds the row's
+// piece q ^ (r & 7), so that a column of fragments spreads over the banks.
+template <int ROWS, int THREADS>
+DEV void stage_rows(const _Float16* m, int ld, int row0, int k,
+                    _Float16* lds) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+  for (int it = 0; it < ROWS * 8 / THREADS; ++it) {
+    const int q = it * THREADS + wave * 64 + lane;
+    const int r = q >> 3, s = (q & 7) ^ (r & 7);
+    glds16(m + ((long)(row0 + r) * ld + k) * 2 + s * 8,
+           lds + (it * THREADS + wave * 64) * 8);
+  }
+}
+
+// Rows k to k + 32, COLS columns from c0: pair q of pieces of row k holds
+// the row's pair q ^ swap_of(k).
+DEV int swap_of(int k) { return (k & 3) | ((k >> 3) & 1) << 2; }
+
+template <int COLS, int THREADS>
+DEV void stage_cols(const _Float16* m, int ld, int k, int c0,
+                    _Float16* lds) {
+  constexpr int PER = COLS / 4;                // pieces a row
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+  for (int it = 0; it < COLS * 8 / THREADS; ++it) {
+    const int q = it * THREADS + wave * 64 + lane;
+    const int r = q / PER, s = (q % PER) ^ (swap_of(r) << 1);
+    glds16(m + ((long)(k + r) * ld + c0) * 2 + s * 8,
+           lds + (it * THREADS + wave * 64) * 8);
+  }
+}
+
+// A lane's 8 k-values of row r of a stage_rows slice: hi (part 0) or lo
+// (part 1).
+DEV half8 frag_rows(const _Float16* lds, int r, int part) {
+  const int lane = threadIdx.x & 63;
+  const int s = (part * 4 + (lane >> 4)) ^ (r & 7);
+  return *(const half8*)(lds + r * 64 + s * 8);
+}
+
+// The same of column c + (lane & 15) of a stage_cols slice, by transposing
+// reads of four k each: lane l of a group of 16 gets column l, rows from
+// the addresses of lanes 4j + l/4.
+template <int COLS>
+DEV half8 frag_cols(const _Float16* lds, int c, int part) {
+  const int lane = threadIdx.x & 63;
+  const int pair = c / 32 * 4 + part * 2 + c % 32 / 16;
+  half8 f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int k = 8 * (lane >> 4) + 4 * h + ((lane & 15) >> 2);
+    const _Float16* at = lds + k * COLS * 2 + (pair ^ swap_of(k)) * 16
+                         + 4 * (lane & 3);
+    const half4 v = __builtin_bit_cast(
+        half4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_fp16x4*)at));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[h * 4 + j] = v[j];
+  }
+  return f;
+}
+
+// Where a tile of a product lies.  Of symmetric matrices (GRAM, SQUARE) the
+// tiles on and below the diagonal, row by row.
+template <int MODE, int BT>
+struct Tile {
+  long mat;
+  int ti, tj;
+
+  DEV Tile(const NsProb& p, int b) {
+    if (MODE == APPLY) {
+      const int tn = p.np / BT, tiles = p.mp / BT * tn;
+      mat = b / tiles;
+      b %= tiles;
+      ti = b / tn;
+      tj = b % tn;
+    } else {
+      const int t = p.mp / BT, tiles = t * (t + 1) / 2;
+      mat = b / tiles;
+      b %= tiles;
+      ti = (int)((sqrtf(8.f * b + 1.f) - 1.f) * 0.5f);
+      if (ti * (ti + 1) / 2 > b) --ti;
+      if ((ti + 1) * (ti + 2) / 2 <= b) ++ti;
+      tj = b - ti * (ti + 1) / 2;
+    }
+  }
+};
+
+// What is done with finished sums: 16 rows of a wave's part of a tile,
+// from row0, FN fragments wide, from col0.  The wave turns them around in
+// its strip of LDS, so that a lane has N neighbours of one row (or, for
+// the other half of a symmetric matrix, of one column) to store.
+template <int MODE, int FN>
+DEV void finish(const NsArgs& a, const NsProb& p, long mat, bool mirror,
+                int row0, int col0, float shift, const f32x4 (&acc)[FN],
+                float* strip) {
+  constexpr int N = FN * 4, W = FN * 16 + 4;
+  const int lane = threadIdx.x & 63;
+  const int lr = lane >> 2, lc = (lane & 3) * N;           // row-wise
+  const int xc = lane % (FN * 16), xr = lane / (FN * 16) * N;
+  const bool result = MODE == APPLY && a.last;
+  // what takes a sum to the scale of the split matrix or of the result
+  const float unit = MODE == GRAM ? shift * shift / SCALE
+                     : result ? shift / (SCALE * SCALE) : 1.f / SCALE;
+  // lane: column lane&15 of a fragment, rows 4*(lane>>4) + r
+#pragma unroll
+  for (int v = 0; v < FN; ++v)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      strip[(4 * (lane >> 4) + r) * W + v * 16 + (lane & 15)] =
+          acc[v][r] * unit;
+  wave_order();
+  float f[N];
+  if (result && p.tall) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = strip[(xr + j) * W + xc];
+    const int R = col0 + xc, c = row0 + xr;
+    if (R < p.n)
+      store_result<N>(p, (mat * p.n + R) * (long)p.m + c, c, p.m, f);
+    wave_order();
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] = strip[lr * W + lc + j];
+  const int R = row0 + lr, c = col0 + lc;
+  if (result) {
+    if (R < p.m)
+      store_result<N>(p, (mat * p.m + R) * (long)p.n + c, c, p.n, f);
+  } else if (MODE == APPLY) {
+    store_split<N>((_Float16*)p.X[(a.step + 1) & 1]
+                       + mat * 2 * p.mp * (long)p.np,
+                   p.np, R, c, f);
+  } else {
+    const long at = mat * 2 * p.mp * (long)p.mp;
+    const bool poly = MODE == SQUARE && a.poly;
+    if (poly) {
+      const _Float16* q = (const _Float16*)p.S[a.s1] + at
+                          + ((long)R * p.mp + c / 32 * 32) * 2 + c % 32;
+#pragma unroll
+      for (int k = 0; k < N; k += 8) {
+        const half8 hi = *(const half8*)(q + k);
+        const half8 lo = *(const half8*)(q + k + 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          f[k + j] = QC * f[k + j] + QB * ((float)hi[j] + (float)lo[j]);
+          if (R == c + k + j) f[k + j] += QA * SCALE;
+        }
+      }
+    }
+    _Float16* d = (_Float16*)p.S[a.to] + at;
+    store_split<N>(d, p.mp, R, c, f);
+    if (mirror) {
+      if (poly) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) strip[lr * W + lc + j] = f[j];
+        wave_order();
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = strip[(xr + j) * W + xc];
+      store_split<N>(d, p.mp, col0 + xc, row0 + xr, f);
+    }
+  }
+  wave_order();
+}
+
+// C = Aop * Bop, BT x BT a block.  Aop: rows of a split matrix, k along
+// them.  Bop: the same (GRAM, SQUARE), or k down the rows of a split matrix
+// (APPLY).  A ring of S LDS buffers: S - 1 slices of 32 DEEP k are on
+// their way (16 bytes a lane, straight to LDS) while one is multiplied.
+//
+// The first skip[i] tiles of a matrix are one block's each; k of the
+// others is cut into parts[i] runs, whose sums go to a.partial, one place
+// a run, for ns_join_k to add.
+template <int MODE, int BT, int WM, int WN, int S, int DEEP>
+__global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
+  constexpr int THREADS = 64 * WM * WN;
+  constexpr int FM = BT / WM / 16, FN = BT / WN / 16;  // fragments a wave
+  constexpr bool PING = BT == 256;
+  constexpr int HALVES = BT * 128;           // a 32-deep slice in LDS
+  constexpr int LOADS = DEEP * BT * 16 / THREADS;          // a lane
+  extern __shared__ __align__(16) _Float16 lds[];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wr = wave / WN * (BT / WM), wc = wave % WN * (BT / WN);
+  const bool single = (int)blockIdx.x < a.whole;
+  const int run = (int)blockIdx.x - a.whole;
+  int i = 0, tile, first = 0, steps;
+  if (single) {
+    while (i + 1 < a.count && (int)blockIdx.x >= a.tile0[i + 1]) ++i;
+  } else {
+    while (i + 1 < a.count && run >= a.start[i + 1]) ++i;
+  }
+  const NsProb& p = a.p[i];
+  const int slices = (MODE == GRAM ? p.np : p.mp) / (32 * DEEP);
+  if (single) {
+    tile = (int)blockIdx.x - a.tile0[i];
+    steps = slices;
+  } else {
+    const int parts = a.parts[i];
+    tile = a.skip[i] + (run - a.start[i]) / parts;
+    const int part = (run - a.start[i]) % parts;
+    first = (int)((long)slices * part / parts);
+    steps = (int)((long)slices * (part + 1) / parts) - first;
+  }
+  const Tile<MODE, BT> at(p, tile);
+  const long mat = at.mat;
+  const int r0 = at.ti * BT, c0 = at.tj * BT;
+  const float shift = p.shift[mat];
   const _Float16* X = (const _Float16*)p.X[a.step & 1]
                       + mat * 2 * p.mp * (long)p.np;
-  const _Float16* S = (const _Float16*)(MODE == APPLY ? p.B : p.A)
-                      + mat * 2 * p.mp * (long)p.mp;
-  const _Float16* Ag = MODE == GRAM ? X : S;
-  const _Float16* Bg = MODE == POLY ? S : X;
+  const long sq = mat * 2 * p.mp * (long)p.mp;
+  const _Float16* Ag = MODE == GRAM ? X : (const _Float16*)p.S[a.s1] + sq;
+  const _Float16* Bg = MODE == SQUARE ? (const _Float16*)p.S[a.s2] + sq : X;
   const int K = MODE == GRAM ? p.np : p.mp;
-  const int r0 = ti * BT, c0 = tj * BT;
 
-  // 16-byte pieces; LDS piece q of row r holds the row's piece
-  // q ^ (r & 7), so that a column of fragments spreads over the banks
-  auto stage_rows = [&](const _Float16* g, int row0, int t,
-                        _Float16* lds) {
-#pragma unroll
-    for (int it = 0; it < BT / 32; ++it) {
-      const int q = it * 256 + wave * 64 + lane;
-      const int r = q >> 3, s = (q & 7) ^ (r & 7);
-      glds16(g + ((long)(row0 + r) * K + t * 32) * 2 + s * 8,
-             lds + (it * 256 + wave * 64) * 8);
-    }
-  };
-  // k rows of BT columns: 32-byte pairs of pieces, pair q of row k holds
-  // the row's pair q ^ swap(k)
-  auto swap_of = [](int k) { return (k & 3) | ((k >> 3) & 1) << 2; };
-  auto stage_k = [&](int t, _Float16* lds) {
-    constexpr int PER = BT / 4;              // pieces a row
-#pragma unroll
-    for (int it = 0; it < BT / 32; ++it) {
-      const int q = it * 256 + wave * 64 + lane;
-      const int k = q / PER, s = (q % PER) ^ (swap_of(k) << 1);
-      glds16(Bg + ((long)(t * 32 + k) * p.np + c0) * 2 + s * 8,
-             lds + (it * 256 + wave * 64) * 8);
-    }
-  };
   auto stage = [&](int t, int buf) {
-    stage_rows(Ag, r0, t, As[buf]);
-    if (MODE == APPLY)
-      stage_k(t, Bs[buf]);
-    else
-      stage_rows(Bg, c0, t, Bs[buf]);
-  };
-  // 8 k-values of row r: hi (part 0) or lo (part 1)
-  auto frag_rows = [&](const _Float16* lds, int r, int part) -> half8 {
-    const int s = (part * 4 + (lane >> 4)) ^ (r & 7);
-    return *(const half8*)(lds + r * 64 + s * 8);
-  };
-  // the same of a column: transposing reads of four k each (lane l of a
-  // group of 16 gets column l, rows from the addresses of lanes 4j+l/4)
-  auto frag_cols = [&](const _Float16* lds, int c, int part) -> half8 {
-    const int pair = c / 32 * 4 + part * 2 + c % 32 / 16;
-    half8 f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = 8 * (lane >> 4) + 4 * h + ((lane & 15) >> 2);
-      const _Float16* at = lds + k * BT * 2 + (pair ^ swap_of(k)) * 16
-                           + 4 * (lane & 3);
-      const half4 v = __builtin_bit_cast(
-          half4,
-          __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_fp16x4*)at));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[h * 4 + j] = v[j];
+    for (int d = 0; d < DEEP; ++d) {
+      _Float16* to = lds + (buf * DEEP + d) * HALVES;
+      const int k = (t * DEEP + d) * 32;
+      stage_rows<BT, THREADS>(Ag, K, r0, k, to);
+      if (MODE == APPLY)
+        stage_cols<BT, THREADS>(Bg, p.np, k, c0, to + BT * 64);
+      else
+        stage_rows<BT, THREADS>(Bg, K, c0, k, to + BT * 64);
     }
-    return f;
   };
 
-  const int wr = (wave >> 1) * (BT / 2), wc = (wave & 1) * (BT / 2);
-  f32x4 acc[F][F];
+  f32x4 acc[FM][FN];
 #pragma unroll
-  for (int u = 0; u < F; ++u)
+  for (int u = 0; u < FM; ++u)
 #pragma unroll
-    for (int v = 0; v < F; ++v) acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int steps = K / 32;
-  stage(0, 0);
-  for (int t = 0; t < steps; ++t) {
+    for (int v = 0; v < FN; ++v) acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (PING) {
+    // Two groups of four waves, one of each on every SIMD, half a beat
+    // apart: while one reads its fragments (and asks for the next
+    // slice), the other multiplies.  Beats of a group: fragments of B
+    // and of the upper half of A; their products; the lower half of A;
+    // their products.
+    const bool late = wave >= 4;
+    half8 fa[2][FM / 2], fb[2][FN];
+    auto beat = [] {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto read_a = [&](const _Float16* la, int h) {
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int u = 0; u < FM / 2; ++u)
+          fa[part][u] = frag_rows(
+              la, wr + (h * (FM / 2) + u) * 16 + (lane & 15), part);
+    };
+    auto multiply = [&](auto h) {
+      constexpr int H = decltype(h)::value * (FM / 2);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int term = 0; term < 3; ++term)
+#pragma unroll
+        for (int u = 0; u < FM / 2; ++u)
+#pragma unroll
+          for (int v = 0; v < FN; ++v)
+            acc[H + u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                fa[term == 2][u], fb[term == 1][v], acc[H + u][v], 0, 0,
+                0);
+      __builtin_amdgcn_s_setprio(0);
+    };
+    stage(first, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < steps) stage(t + 1, (t + 1) & 1);
-    const _Float16 *la = As[t & 1], *lb = Bs[t & 1];
-    half8 fa[2][F], fb[2][F];
+    beat();
+    if (late) beat();
+    for (int t = 0; t < steps; ++t) {
+      const _Float16* la = lds + (t & 1) * HALVES;
+      const _Float16* lb = la + BT * 64;
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int v = 0; v < FN; ++v)
+          fb[part][v] =
+              MODE == APPLY
+                  ? frag_cols<BT>(lb, wc + v * 16, part)
+                  : frag_rows(lb, wc + v * 16 + (lane & 15), part);
+      read_a(la, 0);
+      // the other buffer's last readers, the late group in its third
+      // beat of the slice before, are past that beat's barrier
+      if (t + 1 < steps) stage(first + t + 1, (t + 1) & 1);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      beat();
+      multiply(Int<0>());
+      beat();
+      read_a(la, 1);
+      // the next slice is read first in the beat after next
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      beat();
+      multiply(Int<1>());
+      beat();
+    }
+    if (!late) beat();
+  } else {
+    for (int t = 0; t < S - 1 && t < steps; ++t) stage(first + t, t);
+    int buf = 0;
+    for (int t = 0; t < steps; ++t) {
+      // Slice t has landed when only the S - 2 after it are
+      // outstanding.  The barrier is the bare one: a full one would
+      // wait for them too.
+      if (t + S - 1 <= steps)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((S - 2)
+                                                           * LOADS)
+                     : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      // all fragments first: read one by one, each read's latency
+      // stood before its products
+      half8 fa[DEEP][2][FM], fb[DEEP][2][FN];
+#pragma unroll
+      for (int d = 0; d < DEEP; ++d) {
+        const _Float16* la = lds + (buf * DEEP + d) * HALVES;
+        const _Float16* lb = la + BT * 64;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+#pragma unroll
+          for (int v = 0; v < FN; ++v)
+            fb[d][part][v] =
+                MODE == APPLY
+                    ? frag_cols<BT>(lb, wc + v * 16, part)
+                    : frag_rows(lb, wc + v * 16 + (lane & 15), part);
+#pragma unroll
+          for (int u = 0; u < FM; ++u)
+            fa[d][part][u] =
+                frag_rows(la, wr + u * 16 + (lane & 15), part);
+        }
+      }
+      // into the buffer that every wave was done with at that barrier
+      if (t + S - 1 < steps)
+        stage(first + t + S - 1, buf == 0 ? S - 1 : buf - 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+        for (int term = 0; term < 3; ++term)
+#pragma unroll
+          for (int u = 0; u < FM; ++u)
+#pragma unroll
+            for (int v = 0; v < FN; ++v)
+              acc[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  fa[d][term == 2][u], fb[d][term == 1][v], acc[u][v], 0,
+                  0, 0);
+      buf = buf + 1 == S ? 0 : buf + 1;
+    }
+  }
+  __syncthreads();                  // the ring is free again
+  if (steps < slices) {
+    f32x4* to = (f32x4*)(a.partial + (long)run * BT * BT);
+#pragma unroll
+    for (int u = 0; u < FM; ++u)
+#pragma unroll
+      for (int v = 0; v < FN; ++v)
+        to[((wave * FM + u) * FN + v) * 64 + lane] = acc[u][v];
+    return;
+  }
+  float* strip = (float*)lds + wave * 16 * (FN * 16 + 4);
+#pragma unroll
+  for (int u = 0; u < FM; ++u)
+    finish<MODE, FN>(a, p, mat, at.ti != at.tj, r0 + wr + u * 16, c0 + wc,
+                     shift, acc[u], strip);
+}
+
+// The runs of tiles that were cut, added up in the order of k: a wave
+// takes 16 rows of what one wave of ns_gemm_k left.
+template <int MODE, int BT, int WM, int WN>
+__global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
+  constexpr int FM = BT / WM / 16, FN = BT / WN / 16;
+  constexpr int STRIPS = WM * WN * FM;       // of a tile
+  __shared__ __align__(16) float strips[4][16 * (FN * 16 + 4)];
+  const int lane = threadIdx.x & 63;
+  int job = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
+  int i = 0;
+  for (; i < a.count; ++i) {
+    const int jobs = a.parts[i] > 1
+                         ? (a.start[i + 1] - a.start[i]) / a.parts[i]
+                               * STRIPS : 0;
+    if (job < jobs) break;
+    job -= jobs;
+  }
+  if (i == a.count) return;
+  const NsProb& p = a.p[i];
+  const int cut = job / STRIPS, wave = job % STRIPS / FM, u = job % FM;
+  const Tile<MODE, BT> at(p, a.skip[i] + cut);
+  const f32x4* from = (const f32x4*)a.partial
+                      + (long)(a.start[i] + cut * a.parts[i]) * BT * BT / 4
+                      + (wave * FM + u) * FN * 64 + lane;
+  f32x4 acc[FN];
+#pragma unroll
+  for (int v = 0; v < FN; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int j = 0; j < a.parts[i]; ++j)
+#pragma unroll
+    for (int v = 0; v < FN; ++v)
+      acc[v] += from[(long)j * (BT * BT / 4) + v * 64];
+  finish<MODE, FN>(a, p, at.mat, at.ti != at.tj,
+                   at.ti * BT + wave / WN * (BT / WM) + u * 16,
+                   at.tj * BT + wave % WN * (BT / WN), p.shift[at.mat], acc,
+                   strips[threadIdx.x >> 6]);
+}
+
+// ---- matrices of at most 64 rows ------------------------------------------
+//
+// Everything that is m x m fits into LDS, so two steps of the iteration
+// need X once: with A = X X^T, M = aI + bA + cAA, A' = M A M (what X X^T
+// is after a step) and M' = aI + bA' + cA'A', X <- (M' M) X.  More than
+// two steps at a time would let M' M's entries outgrow fp16 (its norm is
+// at most 3.4445^k) and lose weak directions to rounding.
+//
+// `groups` blocks a matrix have a range of X's columns each.  Every block
+// adds up A from all blocks' shares and does the m x m work itself, which
+// costs less than a launch; then it multiplies its columns and leaves its
+// share of the next A.  At 64 x 576 five launches of 97 us become six
+// kernels: see the table of measurements.
+
+constexpr int FEW = 64;
+constexpr int SLICE = FEW * 64;               // halves of 32 columns
+
+// P Q for symmetric 64 x 64 P, Q in LDS (two slices each): a wave's 32 x
+// 32 part.  The lanes' columns are rows of P, so that a lane has four
+// neighbours of a row of the result (kept transposed instead, the errors
+// of the chain of products came out twice as large).
+DEV void few_product(const _Float16* P, const _Float16* Q, int wr, int wc,
+                     f32x4 (&acc)[2][2]) {
+  const int l = threadIdx.x & 15;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+    half8 f[2][2], g[2][2];
 #pragma unroll
     for (int part = 0; part < 2; ++part)
 #pragma unroll
-      for (int u = 0; u < F; ++u) {
-        fa[part][u] = frag_rows(la, wr + u * 16 + (lane & 15), part);
-        fb[part][u] =
-            MODE == APPLY
-                ? frag_cols(lb, wc + u * 16, part)
-                : frag_rows(lb, wc + u * 16 + (lane & 15), part);
+      for (int u = 0; u < 2; ++u) {
+        f[part][u] = frag_rows(Q + d * SLICE, wr + u * 16 + l, part);
+        g[part][u] = frag_rows(P + d * SLICE, wc + u * 16 + l, part);
       }
 #pragma unroll
     for (int term = 0; term < 3; ++term)
 #pragma unroll
-      for (int u = 0; u < F; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int v = 0; v < F; ++v)
+        for (int v = 0; v < 2; ++v)
           acc[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              fa[term == 2][u], fb[term == 1][v], acc[u][v], 0, 0, 0);
+              f[term == 2][u], g[term == 1][v], acc[u][v], 0, 0, 0);
   }
+}
 
-  // what takes an accumulator to the scale of the split matrix (or, in
-  // the end, of the result)
-  const float shift = p.shift[mat];
-  const float unit = MODE == GRAM ? shift * shift / SCALE
-                     : MODE == APPLY && a.last
-                         ? shift / (SCALE * SCALE) : 1.f / SCALE;
-  // lane: column lane&15 of a fragment, rows 4*(lane>>4) + r
+// four neighbours of row r from column c on into a stage_rows slice pair
+DEV void few_put(_Float16* lds, int r, int c, const f32x4& val) {
+  half4 hi, lo;
 #pragma unroll
-  for (int u = 0; u < F; ++u)
+  for (int j = 0; j < 4; ++j) {
+    _Float16 h, l;
+    split(val[j], h, l);
+    hi[j] = h;
+    lo[j] = l;
+  }
+  _Float16* at = lds + c / 32 * SLICE + r * 64 + c % 8;
+  const int q = c % 32 / 8;
+  *(half4*)(at + ((q ^ (r & 7)) * 8)) = hi;
+  *(half4*)(at + (((q + 4) ^ (r & 7)) * 8)) = lo;
+}
+
+// a wave's part of a product into LDS
+DEV void few_store(_Float16* lds, int wr, int wc, const f32x4 (&val)[2][2]) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int v = 0; v < F; ++v) {
-      const int row = r0 + wr + u * 16 + 4 * (lane >> 4);
-      const int col = c0 + wc + v * 16 + (lane & 15);
-      if (MODE == APPLY && a.last) {
-        const int rows = p.tall ? p.n : p.m, cols = p.tall ? p.m : p.n;
+  for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (row + r >= p.m || col >= p.n) continue;
-          const float o = acc[u][v][r] * unit;
-          const long at = mat * rows * (long)cols
-                          + (p.tall ? (long)col * cols + row + r
-                                    : (long)(row + r) * cols + col);
-          if (p.w) {
-            const float w = p.keep * p.w[at] + p.rate * o;
-            p.w[at] = w;
-            if (p.copy) ((__bf16*)p.copy)[at] = (__bf16)w;
-          } else if (p.kind == 0) {
-            ((float*)p.out)[at] = o;
-          } else if (p.kind == 1) {
-            ((_Float16*)p.out)[at] = (_Float16)o;
-          } else {
-            ((__bf16*)p.out)[at] = (__bf16)o;
-          }
-        }
-      } else if (MODE == APPLY) {
-        _Float16* d = (_Float16*)p.X[(a.step + 1) & 1]
-                      + mat * 2 * p.mp * (long)p.np;
+    for (int v = 0; v < 2; ++v)
+      few_put(lds, wc + v * 16 + (lane & 15),
+              wr + u * 16 + 4 * (lane >> 4), val[u][v]);
+}
+
+// aI + b A + c AA (all as kept, SCALE times) from A and the sums of AA
+DEV void few_poly(const f32x4 (&A)[2][2], f32x4 (&acc)[2][2], int wr,
+                  int wc) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          _Float16 hi, lo;
-          split(acc[u][v][r] * unit, hi, lo);
-          _Float16* q = d + (long)(row + r) * p.np * 2 + col / 32 * 64
-                        + col % 32;
-          q[0] = hi;
-          q[32] = lo;
-        }
-      } else {
-        _Float16* d = (_Float16*)(MODE == GRAM ? p.A : p.B)
-                      + mat * 2 * p.mp * (long)p.mp;
-        half4 hi4, lo4;
+  for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float val = acc[u][v][r] * unit;
-          if (MODE == POLY) {
-            const _Float16* q = S + (long)(row + r) * p.mp * 2
-                                + col / 32 * 64 + col % 32;
-            val = QC * val + QB * ((float)q[0] + (float)q[32]);
-            if (row + r == col) val += QA * SCALE;
-          }
-          _Float16 hi, lo;
-          split(val, hi, lo);
-          _Float16* q = d + (long)(row + r) * p.mp * 2 + col / 32 * 64
-                        + col % 32;
-          q[0] = hi;
-          q[32] = lo;
-          hi4[r] = hi;
-          lo4[r] = lo;
-        }
-        if (ti != tj) {
-          _Float16* q = d + (long)col * p.mp * 2 + row / 32 * 64 + row % 32;
-          *(half4*)q = hi4;
-          *(half4*)(q + 32) = lo4;
-        }
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool diagonal = wr + u * 16 + 4 * (lane >> 4) + r
+                              == wc + v * 16 + (lane & 15);
+        acc[u][v][r] = QC / SCALE * acc[u][v][r] + QB * A[u][v][r]
+                       + (diagonal ? QA * SCALE : 0.f);
       }
+}
+
+DEV void few_scale(f32x4 (&acc)[2][2], float by) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) acc[u][v] *= by;
+}
+
+// FIRST: the shares of A = X X^T.  Else two steps (or one, if a.pair is
+// 0), and the shares of the next A unless they are the last.
+template <bool FIRST>
+__global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
+  __shared__ __align__(16) _Float16 P[2 * SLICE], Q[2 * SLICE],
+      T[2 * SLICE];
+  const int i = find(a, blockIdx.x);
+  const NsProb& p = a.p[i];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
+  const int b = blockIdx.x - a.start[i], g = b % p.groups;
+  const long mat = b / p.groups;
+  const float shift = p.shift[mat];
+  const _Float16* X = (const _Float16*)p.X[a.step & 1]
+                      + mat * 2 * FEW * (long)p.np;
+  const int blocks = p.np / FEW;               // of 64 columns
+  const int b0 = (int)((long)blocks * g / p.groups);
+  const int b1 = (int)((long)blocks * (g + 1) / p.groups);
+  f32x4 acc[2][2], sum[2][2];
+
+  if (!FIRST) {
+    // A, in the lanes that hold its places and in LDS
+    const f32x4* from = (const f32x4*)p.share[a.step & 1]
+                        + (mat * p.groups) * (FEW * FEW / 4)
+                        + wave * 256 + lane;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) sum[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < p.groups; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+          sum[u][v] += from[j * (FEW * FEW / 4) + (u * 2 + v) * 64];
+    few_scale(sum, shift * shift / SCALE);
+    few_store(P, wr, wc, sum);                 // P = A
+    __syncthreads();
+    few_product(P, P, wr, wc, acc);
+    few_poly(sum, acc, wr, wc);
+    few_store(Q, wr, wc, acc);                 // Q = M
+    __syncthreads();
+    if (a.pair) {
+      few_product(Q, P, wr, wc, acc);
+      few_scale(acc, 1.f / SCALE);
+      few_store(T, wr, wc, acc);               // T = M A
+      __syncthreads();
+      few_product(Q, T, wr, wc, sum);
+      few_scale(sum, 1.f / SCALE);
+      few_store(P, wr, wc, sum);               // P = A' = M A M
+      __syncthreads();
+      few_product(P, P, wr, wc, acc);
+      few_poly(sum, acc, wr, wc);
+      few_store(T, wr, wc, acc);               // T = M'
+      __syncthreads();
+      few_product(T, Q, wr, wc, acc);
+      few_scale(acc, 1.f / SCALE);
+      few_store(P, wr, wc, acc);               // P = M' M
+      __syncthreads();
     }
+  }
+  const _Float16* mul = a.pair ? P : Q;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) sum[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c = b0; c < b1; ++c) {
+    if (FIRST) {
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+        stage_rows<FEW, 256>(X, p.np, 0, c * FEW + d * 32, T + d * SLICE);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+        stage_cols<FEW, 256>(X, p.np, d * 32, c * FEW, T + d * SLICE);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      // X'^T = X^T (M' M): a lane has four columns of a row of X'
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        half8 f[2][2], m[2][2];
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            f[part][u] = frag_cols<FEW>(T + d * SLICE, wr + u * 16, part);
+            m[part][u] = frag_rows(mul + d * SLICE,
+                                   wc + u * 16 + (lane & 15), part);
+          }
+#pragma unroll
+        for (int term = 0; term < 3; ++term)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+              acc[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  f[term == 2][u], m[term == 1][v], acc[u][v], 0, 0, 0);
+      }
+      few_scale(acc, a.last ? shift / (SCALE * SCALE) : 1.f / SCALE);
+      __syncthreads();                         // T is read
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int R = wc + v * 16 + (lane & 15);
+          const int in = wr + u * 16 + 4 * (lane >> 4), C = c * FEW + in;
+          if (!a.last) {
+            few_put(T, R, in, acc[u][v]);
+            half4 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              _Float16 h, l;
+              split(acc[u][v][j], h, l);
+              hi[j] = h;
+              lo[j] = l;
+            }
+            _Float16* d = (_Float16*)p.X[(a.step + 1) & 1]
+                          + mat * 2 * FEW * (long)p.np
+                          + ((long)R * p.np + C / 32 * 32) * 2 + C % 32;
+            *(half4*)d = hi;
+            *(half4*)(d + 32) = lo;
+          } else {
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = acc[u][v][j];
+            if (R >= p.m) continue;
+            if (!p.tall) {
+              store_result<4>(p, (mat * p.m + R) * (long)p.n + C, C, p.n, f);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (C + j < p.n)
+                  store_result<1>(p, (mat * p.n + C + j) * (long)p.m + R, R,
+                                  p.m, f + j);
+            }
+          }
+        }
+      __syncthreads();
+    }
+    if (!a.last) {
+      few_product(T, T, wr, wc, acc);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) sum[u][v] += acc[u][v];
+      __syncthreads();                         // T is read
+    }
+  }
+  if (!a.last) {
+    f32x4* to = (f32x4*)p.share[FIRST ? a.step & 1 : (a.step + 1) & 1]
+                + (mat * p.groups + g) * (FEW * FEW / 4) + wave * 256 + lane;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) to[(u * 2 + v) * 64] = sum[u][v];
+  }
 }
 
 }  // namespace
@@ -374,26 +931,88 @@ hipError_t launch_ns_load(NsArgs* a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// one product of the iteration, for every matrix: mode 0 A = X X^T,
-// 1 B = aI + bA + cAA, 2 X <- B X
-hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
+// matrices of at most 64 rows: the first A (pair < 0), else one or two
+// steps
+hipError_t launch_ns_few(NsArgs* a, hipStream_t stream) {
   int at = 0;
   for (int i = 0; i < a->count; ++i) {
-    const NsProb& p = a->p[i];
-    const int t = p.mp / TILE;
     a->start[i] = at;
-    at += p.batch * (mode == APPLY ? t * (p.np / TILE) : t * (t + 1) / 2);
+    at += a->p[i].batch * a->p[i].groups;
   }
   a->start[a->count] = at;
-  if (mode == GRAM)
-    hipLaunchKernelGGL((ns_gemm_k<GRAM, TILE>), dim3(at), dim3(256), 0,
-                       stream, *a);
-  else if (mode == POLY)
-    hipLaunchKernelGGL((ns_gemm_k<POLY, TILE>), dim3(at), dim3(256), 0,
-                       stream, *a);
+  if (a->pair < 0)
+    hipLaunchKernelGGL(ns_few_k<true>, dim3(at), dim3(256), 0, stream, *a);
   else
-    hipLaunchKernelGGL((ns_gemm_k<APPLY, TILE>), dim3(at), dim3(256), 0,
-                       stream, *a);
+    hipLaunchKernelGGL(ns_few_k<false>, dim3(at), dim3(256), 0, stream, *a);
+  return hipGetLastError();
+}
+
+// One product, for every matrix: mode 0 S[to] = X X^T, 1 S[to] = S[s1]
+// S[s2] (with poly: aI + b S[s1] + c S[s1] S[s1]), 2 X <- S[s1] X.
+hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
+  const int bt = a->tile == 256 && mode != APPLY ? 128 : a->tile;
+  const int deep = bt == 64 ? 64 : 32;
+  const int slots = bt == 256 ? 256 : NS_SLOTS;   // blocks that run at once
+  const int least = 384 / deep;        // shortest run of k worth a join
+  long tiles = 0, rest = 0, runs = 0, joins = 0;
+  long n[NS_MAXP], s[NS_MAXP];
+  for (int i = 0; i < a->count; ++i) {
+    const NsProb& p = a->p[i];
+    const long t = p.mp / bt;
+    n[i] = p.batch * (mode == APPLY ? t * (p.np / bt) : t * (t + 1) / 2);
+    s[i] = (mode == GRAM ? p.np : p.mp) / deep;
+    a->tile0[i] = (int)tiles;
+    tiles += n[i];
+  }
+  if (tiles >= (1L << 30)) return hipErrorInvalidValue;
+  a->tile0[a->count] = (int)tiles;
+  a->whole = (int)(tiles / slots * slots);
+  // the rest: cut k so that it, too, gives every slot a run, in runs of
+  // `least` slices or more
+  rest = tiles - a->whole;
+  for (int i = 0; i < a->count; ++i) {
+    long skip = a->whole - a->tile0[i];
+    skip = skip < 0 ? 0 : skip > n[i] ? n[i] : skip;
+    a->skip[i] = (int)skip;
+    long parts = rest ? slots / rest : 1;
+    if (parts > s[i] / least) parts = s[i] / least;
+    if (parts < 2) parts = 1;
+    a->parts[i] = (int)parts;
+    a->start[i] = (int)runs;
+    runs += (n[i] - skip) * parts;
+    if (parts > 1) joins += (n[i] - skip);
+  }
+  a->start[a->count] = (int)runs;
+  if (runs > NS_SLOTS) return hipErrorInvalidValue;
+  const int blocks = a->whole + (int)runs;
+#define NS_GEMM(MODE, BT, WM, WN, S, DEEP)                               \
+  do {                                                                   \
+    constexpr int bytes = S * DEEP * BT * 256;                           \
+    static const hipError_t ok = hipFuncSetAttribute(                    \
+        (const void*)ns_gemm_k<MODE, BT, WM, WN, S, DEEP>,               \
+        hipFuncAttributeMaxDynamicSharedMemorySize, bytes);              \
+    HIP_KERNEL_ASSERT_OK(ok);                                            \
+    hipLaunchKernelGGL((ns_gemm_k<MODE, BT, WM, WN, S, DEEP>),           \
+                       dim3(blocks), dim3(64 * WM * WN), bytes, stream,  \
+                       *a);                                              \
+    if (joins) {                                                         \
+      const long strips = joins * (BT / 16 * WN);                        \
+      hipLaunchKernelGGL((ns_join_k<MODE, BT, WM, WN>),                  \
+                         dim3((unsigned)((strips + 3) / 4)), dim3(256),  \
+                         0, stream, *a);                                 \
+    }                                                                    \
+  } while (0)
+#define NS_MODES(...)                                  \
+  do {                                                 \
+    if (mode == GRAM) NS_GEMM(GRAM, __VA_ARGS__);      \
+    else if (mode == SQUARE) NS_GEMM(SQUARE, __VA_ARGS__); \
+    else NS_GEMM(APPLY, __VA_ARGS__);                  \
+  } while (0)
+  if (bt == 256) NS_MODES(256, 2, 4, 2, 1);
+  else if (bt == 128) NS_MODES(128, 2, 2, 2, 1);
+  else NS_MODES(64, 2, 2, 2, 2);
+#undef NS_MODES
+#undef NS_GEMM
   return hipGetLastError();
 }
 

@@ -2,8 +2,7 @@
 // by newton_schulz.hip and the bindings.
 #pragma once
 
-constexpr int NS_TILE = 64;    // output tile, and the padding of m and n
-constexpr int NS_MAXP = 24;    // shapes in one launch: 4 KB of arguments
+constexpr int NS_MAXP = 20;    // shapes in one launch: 4 KB of arguments
 
 // One shape: `batch` matrices one behind the other.
 struct NsProb {
@@ -14,18 +13,31 @@ struct NsProb {
   float* v;
   void* copy;
   void* X[2];          // split [mp][np], this step's and the next's
-  void* A;             // split [mp][mp]
-  void* B;
+  void* S[3];          // split [mp][mp]
   double* part;        // [batch][parts] sums of squares
   float* shift;        // [batch] X is kept 1/shift times as large
+  float* share[2];     // few rows: [batch][groups][64][64], of X X^T
   int m, n, mp, np;    // m <= n; padded
+  int groups;          // few rows: blocks a matrix
   int batch, parts, tall, kind;   // kind of in / out: 0 f32, 1 f16, 2 bf16
   float keep, rate;    // w = keep*w + rate*NS
 };
 
+constexpr int NS_SLOTS = 512;  // blocks of a product that share tiles
+
 struct NsArgs {
   NsProb p[NS_MAXP];
-  int start[NS_MAXP + 1];  // first block of each; their number at the end
-  int count, steps, step, last, phase;
+  // first block (in a product: first run) of each; the end's last
+  int start[NS_MAXP + 1];
+  // a product: first output tile of each, its tiles that are one block's,
+  // and the runs that k of its others is cut into
+  int tile0[NS_MAXP + 1], skip[NS_MAXP], parts[NS_MAXP];
+  // edge of an output tile, to which m and n are padded; 0: few rows
+  int tile;
+  int pair;                // few rows: two steps (1), one (0), first (-1)
+  int s1, s2, to, poly;    // a product: which S, and whether aI + bS is added
+  int count, steps, step, last, phase, whole;
   float mu;
+  float* partial;          // [NS_SLOTS][tile]
 };
+static_assert(sizeof(NsArgs) <= 4096, "arguments of a kernel");

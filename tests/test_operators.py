@@ -123,7 +123,7 @@ LN_SHAPES = [(1, 1), (1, 3), (7, 8), (33, 64), (5, 65), (2, 3, 127),
              (260, 128), (31, 256), (70, 257), (600, 300), (513, 512),
              (129, 1000), (40, 1001), (19, 2048), (11, 2049), (6, 4096),
              (5, 8191), (4, 16384), (3, 16385), (2, 33000), (2, 2, 5, 48),
-             (5000, 16)]
+             (5000, 16), (700, 9001), (530, 20000)]
 
 
 @gpu
@@ -196,6 +196,17 @@ def test_layernorm_gpu_nan_stays_in_its_row():
     y = OF.layernorm(x, gamma, beta)
     assert torch.isnan(y[3]).all() and torch.isnan(y[5]).all()
     assert torch.isfinite(y[[0, 1, 2, 4, 6, 7]]).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [5, 700])
+def test_layernorm_gpu_nan_leaves_padded_channels_alone(rows):
+    x, gamma, beta, dy = ln_inputs((rows, 48), torch.bfloat16, dev())
+    x[0, 3] = float("nan")
+    leaves = [t.requires_grad_(True) for t in (x, gamma, beta)]
+    y = OF.layernorm(*leaves, n_features=40)
+    for g in (y, *torch.autograd.grad(y, leaves, dy)):
+        assert not g[..., 40:].float().any()
 
 
 def test_layernorm_refusals():

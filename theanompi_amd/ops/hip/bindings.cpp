@@ -137,11 +137,11 @@ hipError_t launch_splitk_finalize(float*, const float*, void*, long,
 hipError_t launch_ln_fwd(const void*, const float*, const float*, void*,
                          float*, float*, long, int, int, long, float, int,
                          hipStream_t);
-hipError_t ln_bwd_plan(long, int, int, long*, int*);
+void ln_bwd_plan(long, int, int, long*, long*, int*);
 hipError_t launch_ln_bwd(const void*, const void*, const float*,
                          const float*, const float*, void*, float*,
-                         float*, float*, long, long, int, int, long, long,
-                         int, hipStream_t);
+                         float*, float*, long, long, int, long, int, int,
+                         long, long, int, hipStream_t);
 int lp_plan(long, long, int, int*, int*);
 hipError_t launch_lp_fwd(const void*, const long*, float*, float*, float*,
                          long*, float*, float*, unsigned long long*, long,
@@ -1208,19 +1208,19 @@ static std::vector<torch::Tensor> ln_bwd(torch::Tensor dy,
   auto dgamma = torch::empty({C}, gamma.options());
   auto dbeta = torch::empty({C}, gamma.options());
   if (!rows) return {dx, dgamma.zero_(), dbeta.zero_()};
-  long blocks;
-  int shares;
-  CHECK_HIP(ln_bwd_plan(rows, (int)C, kind, &blocks, &shares));
+  long blocks, shares;
+  int by_column;
+  ln_bwd_plan(rows, (int)C, kind, &blocks, &shares, &by_column);
   torch::Tensor part;
-  if (shares) part = torch::empty({blocks * 2 * C}, gamma.options());
+  if (shares) part = torch::empty({shares * 2 * C}, gamma.options());
   const float* st = stat.data_ptr<float>();
   CHECK_HIP(launch_ln_bwd(dy.data_ptr(), x.data_ptr(),
                           gamma.data_ptr<float>(), st, st + rows,
                           dx.data_ptr(), dgamma.data_ptr<float>(),
                           dbeta.data_ptr<float>(),
                           shares ? part.data_ptr<float>() : nullptr,
-                          blocks, rows, (int)C, (int)n, ldx, lddy, kind,
-                          cur_stream()));
+                          blocks, shares, by_column, rows, (int)C, (int)n,
+                          ldx, lddy, kind, cur_stream()));
   return {dx, dgamma, dbeta};
 }
 

@@ -28,30 +28,35 @@ struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
 template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
-  static DEV void load(const T* p, float* f) {
-    union { u32x4 u; T t[N]; } c;
-    c.u = ((const any16*)p)->v;
+  union { u32x4 u; T t[N]; };
+
+  // elements [start, start+N) of a row of n that counts; zeros behind it
+  DEV void load(const T* row, int start, int n) {
+    if (start + N <= n) {
+      u = ((const any16*)(row + start))->v;
+    } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = (float)c.t[j];
+      for (int j = 0; j < N; ++j)
+        t[j] = start + j < n ? row[start + j] : (T)0.f;
+    }
   }
-  static DEV void store(T* p, const float* f) {
-    union { u32x4 u; T t[N]; } c;
-#pragma unroll
-    for (int j = 0; j < N; ++j) c.t[j] = (T)f[j];
-    ((any16*)p)->v = c.u;
-  }
+  DEV float operator[](int j) const { return (float)t[j]; }
 };
 
-// elements [start, start+N) of a row of n that counts; zeros behind it
-template <typename T>
-DEV void load_row(const T* row, int start, int n, float* f) {
-  constexpr int N = Vec<T>::N;
+// N values of gamma or beta
+template <int N>
+DEV void load_param(const float* p, int start, int n, float* f) {
   if (start + N <= n) {
-    Vec<T>::load(row + start, f);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      const f32x4 v = __builtin_bit_cast(
+          f32x4, ((const any16*)(p + start + k))->v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[k + j] = v[j];
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      f[j] = start + j < n ? (float)row[start + j] : 0.f;
+    for (int j = 0; j < N; ++j) f[j] = start + j < n ? p[start + j] : 0.f;
   }
 }
 
@@ -60,7 +65,10 @@ template <typename T>
 DEV void store_row(T* row, int start, int n, int C, const float* f) {
   constexpr int N = Vec<T>::N;
   if (start + N <= n) {
-    Vec<T>::store(row + start, f);
+    Vec<T> v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v.t[j] = (T)f[j];
+    ((any16*)(row + start))->v = v.u;
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -77,10 +85,10 @@ DEV void row_sum(float* v, float* red, int& turn) {
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] = lane_sum<W>(v[k]);
   if constexpr (TPR > 64) {
-    constexpr int WAVES = TPR / 64;
-    float* r = red + turn * (WAVES * 2);
+    constexpr int WAVES = TPR / 64, ALL = TPR > 256 ? WAVES : 4;
+    float* r = red + turn * (ALL * 2);
     turn ^= 1;
-    const int wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, first = wave / WAVES * WAVES;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int k = 0; k < K; ++k) r[wave * K + k] = v[k];
@@ -89,7 +97,7 @@ DEV void row_sum(float* v, float* red, int& turn) {
     for (int k = 0; k < K; ++k) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) s += r[w * K + k];
+      for (int w = 0; w < WAVES; ++w) s += r[(first + w) * K + k];
       v[k] = s;
     }
   }
@@ -104,32 +112,38 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_k(
   constexpr int N = Vec<T>::N;
   constexpr int BLOCK = TPR > 256 ? TPR : 256;
   constexpr int RPB = BLOCK / TPR;
-  __shared__ float red[TPR > 64 ? TPR / 64 * 4 : 1];
+  __shared__ float red[TPR > 256 ? TPR / 16 : 16];
   int turn = 0;
   const int lane = threadIdx.x % TPR;
   const float inv_n = 1.f / (float)n;
+  const long step = (long)gridDim.x * RPB;
+  long r = (long)blockIdx.x * RPB + threadIdx.x / TPR;
+  Vec<T> next[NV];
+  auto fetch = [&](long row) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      next[i].load(x + (row < rows ? row : 0) * ldx, (lane + i * TPR) * N,
+                   row < rows ? n : 0);
+  };
+  fetch(r);
   float ga[NV][N], be[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int s = (lane + i * TPR) * N;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      ga[i][j] = s + j < n ? gamma[s + j] : 0.f;
-      be[i][j] = s + j < n ? beta[s + j] : 0.f;
-    }
+    load_param<N>(gamma, (lane + i * TPR) * N, n, ga[i]);
+    load_param<N>(beta, (lane + i * TPR) * N, n, be[i]);
   }
   for (long base = (long)blockIdx.x * RPB; base < rows;
-       base += (long)gridDim.x * RPB) {
-    const long r = base + threadIdx.x / TPR;
+       base += step, r += step) {
     const bool live = r < rows;
-    float f[NV][N], s[1] = {0.f};
+    Vec<T> v[NV];
+    float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      load_row(x + (live ? r : 0) * ldx, (lane + i * TPR) * N,
-               live ? n : 0, f[i]);
+      v[i] = next[i];
 #pragma unroll
-      for (int j = 0; j < N; ++j) s[0] += f[i][j];
+      for (int j = 0; j < N; ++j) s[0] += v[i][j];
     }
+    if (base + step < rows) fetch(r + step);   // while this one is summed
     row_sum<TPR, 1>(s, red, turn);
     const float m = s[0] * inv_n;
     s[0] = 0.f;
@@ -137,18 +151,19 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_k(
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        f[i][j] -= m;
-        s[0] += (lane + i * TPR) * N + j < n ? f[i][j] * f[i][j] : 0.f;
+        const float d = v[i][j] - m;
+        s[0] += (lane + i * TPR) * N + j < n ? d * d : 0.f;
       }
     row_sum<TPR, 1>(s, red, turn);
     const float rs = 1.f / sqrtf(s[0] * inv_n + eps);
     if (live) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        float f[N];
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          f[i][j] = f[i][j] * rs * ga[i][j] + be[i][j];
-        store_row(y + r * C, (lane + i * TPR) * N, n, C, f[i]);
+          f[j] = (v[i][j] - m) * rs * ga[i][j] + be[i][j];
+        store_row(y + r * C, (lane + i * TPR) * N, n, C, f);
       }
       if (lane == 0) {
         mean[r] = m;
@@ -172,28 +187,34 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_k(
   const float inv_n = 1.f / (float)n;
   for (long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = x + r * ldx;
-    float f[N], s[1] = {0.f};
+    float s[1] = {0.f};
+    Vec<T> v;
+#pragma unroll 2
     for (int c = threadIdx.x * N; c < n; c += 1024 * N) {
-      load_row(row, c, n, f);
+      v.load(row, c, n);
 #pragma unroll
-      for (int j = 0; j < N; ++j) s[0] += f[j];
+      for (int j = 0; j < N; ++j) s[0] += v[j];
     }
     row_sum<1024, 1>(s, red, turn);
     const float m = s[0] * inv_n;
     s[0] = 0.f;
+#pragma unroll 2
     for (int c = threadIdx.x * N; c < n; c += 1024 * N) {
-      load_row(row, c, n, f);
+      v.load(row, c, n);
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        s[0] += c + j < n ? (f[j] - m) * (f[j] - m) : 0.f;
+        s[0] += c + j < n ? (v[j] - m) * (v[j] - m) : 0.f;
     }
     row_sum<1024, 1>(s, red, turn);
     const float rs = 1.f / sqrtf(s[0] * inv_n + eps);
+#pragma unroll 2
     for (int c = threadIdx.x * N; c < C; c += 1024 * N) {
-      load_row(row, c, n, f);
+      float f[N], ga[N], be[N];
+      v.load(row, c, n);
+      load_param<N>(gamma, c, n, ga);
+      load_param<N>(beta, c, n, be);
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (c + j < n) f[j] = (f[j] - m) * rs * gamma[c + j] + beta[c + j];
+      for (int j = 0; j < N; ++j) f[j] = (v[j] - m) * rs * ga[j] + be[j];
       store_row(y + r * C, c, n, C, f);
     }
     if (threadIdx.x == 0) {
@@ -216,59 +237,79 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
   constexpr int BLOCK = TPR > 256 ? TPR : 256;
   constexpr int RPB = BLOCK / TPR;
   constexpr int WAVES = BLOCK / 64;
-  __shared__ float red[TPR > 64 ? TPR / 64 * 4 : 1];
+  __shared__ float red[TPR > 256 ? TPR / 16 : 16];
   int turn = 0;
   const int lane = threadIdx.x % TPR;
   const float inv_n = 1.f / (float)n;
-  float ga[NV][N], ag[NV][N], ab[NV][N];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int s = (lane + i * TPR) * N;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      ga[i][j] = s + j < n ? gamma[s + j] : 0.f;
-      ag[i][j] = ab[i][j] = 0.f;
-    }
-  }
-  for (long base = (long)blockIdx.x * RPB; base < rows;
-       base += (long)gridDim.x * RPB) {
-    const long r = base + threadIdx.x / TPR;
-    const bool live = r < rows;
-    const long rr = live ? r : 0;
-    const float m = mean[rr], rs = rstd[rr];
-    float g[NV][N], xh[NV][N], s[2] = {0.f, 0.f};
+  const long step = (long)gridDim.x * RPB;
+  long r = (long)blockIdx.x * RPB + threadIdx.x / TPR;
+  // the next row, as loaded: what is computed from it is computed twice
+  // rather than kept over the sums
+  Vec<T> nx[NV], ny[NV];
+  float nm, nr;
+  auto fetch = [&](long row) {
+    const bool there = row < rows;
+    const long rr = there ? row : 0;
+    nm = mean[rr];
+    nr = rstd[rr];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (lane + i * TPR) * N;
-      load_row(dy + rr * lddy, c, live ? n : 0, g[i]);
-      load_row(x + rr * ldx, c, live ? n : 0, xh[i]);
+      ny[i].load(dy + rr * lddy, c, there ? n : 0);
+      nx[i].load(x + rr * ldx, c, there ? n : 0);
+    }
+  };
+  fetch(r);
+  float ga[NV][N], ag[NV][N], ab[NV][N];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load_param<N>(gamma, (lane + i * TPR) * N, n, ga[i]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) ag[i][j] = ab[i][j] = 0.f;
+  }
+  for (long base = (long)blockIdx.x * RPB; base < rows;
+       base += step, r += step) {
+    const bool live = r < rows;
+    Vec<T> vx[NV], vy[NV];
+    const float m = nm, rs = nr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      vx[i] = nx[i];
+      vy[i] = ny[i];
+    }
+    if (base + step < rows) fetch(r + step);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        // behind the row's end dy and gamma are 0, and so is what a
-        // row that is not there would add
-        xh[i][j] = (live && c + j < n) ? (xh[i][j] - m) * rs : 0.f;
-        ag[i][j] += g[i][j] * xh[i][j];
-        ab[i][j] += g[i][j];
-        g[i][j] *= ga[i][j];
-        s[0] += g[i][j];
-        s[1] += g[i][j] * xh[i][j];
+        // behind the row's end dy and gamma are 0, and so is what a row
+        // that is not there adds; x is 0 there, and xh is finite
+        const float xh = (vx[i][j] - m) * rs, d = vy[i][j];
+        ag[i][j] += d * xh;
+        ab[i][j] += d;
+        s[0] += d * ga[i][j];
+        s[1] += d * ga[i][j] * xh;
       }
-    }
     row_sum<TPR, 2>(s, red, turn);
     const float c1 = s[0] * inv_n, c2 = s[1] * inv_n;
     if (live) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        float f[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          g[i][j] = rs * (g[i][j] - c1 - xh[i][j] * c2);
-        store_row(dx + r * C, (lane + i * TPR) * N, n, C, g[i]);
+        for (int j = 0; j < N; ++j) {
+          const float xh = (vx[i][j] - m) * rs;
+          f[j] = rs * (vy[i][j] * ga[i][j] - c1 - xh * c2);
+        }
+        store_row(dx + r * C, (lane + i * TPR) * N, n, C, f);
       }
     }
   }
   if (!part) return;
   float* pg = part + (long)blockIdx.x * 2 * C;
   float* pb = pg + C;
+  // channels behind n have no gradient, whatever a row's NaN makes of 0
   if constexpr (TPR >= 256) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -276,15 +317,16 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
       for (int j = 0; j < N; ++j) {
         const int c = (lane + i * TPR) * N + j;
         if (c < C) {
-          pg[c] = ag[i][j];
-          pb[c] = ab[i][j];
+          pg[c] = c < n ? ag[i][j] : 0.f;
+          pb[c] = c < n ? ab[i][j] : 0.f;
         }
       }
   } else {
     // the block's row groups are added up in a fixed order: within a
-    // wave by exchange, between waves in LDS
-    __shared__ float acc[2][WAVES][TPR * NV * N];
-    const int wave = threadIdx.x >> 6;
+    // wave by exchange, between waves (or pairs of them) in LDS
+    constexpr int SLOTS = TPR <= 64 ? WAVES : RPB;
+    __shared__ float acc[2][SLOTS][TPR * NV * N];
+    const int slot = TPR <= 64 ? threadIdx.x >> 6 : threadIdx.x / TPR;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -294,21 +336,21 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
           ag[i][j] += __shfl_xor(ag[i][j], off, 64);
           ab[i][j] += __shfl_xor(ab[i][j], off, 64);
         }
-        if ((threadIdx.x & 63) < TPR) {
-          acc[0][wave][(lane + i * TPR) * N + j] = ag[i][j];
-          acc[1][wave][(lane + i * TPR) * N + j] = ab[i][j];
+        if (TPR >= 64 || (threadIdx.x & 63) < TPR) {
+          acc[0][slot][(lane + i * TPR) * N + j] = ag[i][j];
+          acc[1][slot][(lane + i * TPR) * N + j] = ab[i][j];
         }
       }
     __syncthreads();
     for (int c = threadIdx.x; c < C; c += BLOCK) {
       float sg = 0.f, sb = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
+      for (int w = 0; w < SLOTS; ++w) {
         sg += acc[0][w][c];
         sb += acc[1][w][c];
       }
-      pg[c] = sg;
-      pb[c] = sb;
+      pg[c] = c < n ? sg : 0.f;
+      pb[c] = c < n ? sb : 0.f;
     }
   }
 }
@@ -326,55 +368,68 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide_k(
   for (long r = blockIdx.x; r < rows; r += gridDim.x) {
     const float m = mean[r], rs = rstd[r];
     const T *xr = x + r * ldx, *dr = dy + r * lddy;
-    float f[N], g[N], s[2] = {0.f, 0.f};
+    float s[2] = {0.f, 0.f}, ga[N];
+    Vec<T> g, v;
+#pragma unroll 2
     for (int c = threadIdx.x * N; c < n; c += 1024 * N) {
-      load_row(dr, c, n, g);
-      load_row(xr, c, n, f);
+      g.load(dr, c, n);
+      v.load(xr, c, n);
+      load_param<N>(gamma, c, n, ga);
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (c + j < n) {
-          g[j] *= gamma[c + j];
-          s[0] += g[j];
-          s[1] += g[j] * (f[j] - m) * rs;
-        }
+      for (int j = 0; j < N; ++j) {
+        s[0] += g[j] * ga[j];
+        s[1] += g[j] * ga[j] * ((v[j] - m) * rs);
+      }
     }
     row_sum<1024, 2>(s, red, turn);
     const float c1 = s[0] * inv_n, c2 = s[1] * inv_n;
+#pragma unroll 2
     for (int c = threadIdx.x * N; c < C; c += 1024 * N) {
-      load_row(dr, c, n, g);
-      load_row(xr, c, n, f);
+      float f[N];
+      g.load(dr, c, n);
+      v.load(xr, c, n);
+      load_param<N>(gamma, c, n, ga);
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (c + j < n)
-          g[j] = rs * (g[j] * gamma[c + j] - c1 - (f[j] - m) * rs * c2);
-      store_row(dx + r * C, c, n, C, g);
+        f[j] = rs * (g[j] * ga[j] - c1 - (v[j] - m) * rs * c2);
+      store_row(dx + r * C, c, n, C, f);
     }
   }
 }
 
 // dgamma / dbeta of a group of channels straight from x and dy: for few
 // rows and for rows too wide for ln_bwd_k.  8 lanes x 16 bytes across,
-// 32 rows down, then a fixed-order sum in LDS.
+// 32 rows down, then a fixed-order sum in LDS.  With `part`, of one of
+// gridDim.y ranges of rows, to be joined.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_cols_k(
     const T* __restrict__ dy, const T* __restrict__ x,
     const float* __restrict__ mean, const float* __restrict__ rstd,
-    float* __restrict__ dgamma, float* __restrict__ dbeta, long rows,
-    int C, int n, long ldx, long lddy) {
+    float* __restrict__ dgamma, float* __restrict__ dbeta,
+    float* __restrict__ part, long rows, int C, int n, long ldx,
+    long lddy) {
   constexpr int N = Vec<T>::N;
   __shared__ float acc[2][32][8 * N + 1];
+  const long r0 = rows * blockIdx.y / gridDim.y;
+  const long r1 = rows * (blockIdx.y + 1) / gridDim.y;
+  if (part) {
+    dgamma = part + (long)blockIdx.y * 2 * C;
+    dbeta = dgamma + C;
+  }
   const int lx = threadIdx.x & 7, ly = threadIdx.x >> 3;
   const int c = (blockIdx.x * 8 + lx) * N;
-  float ag[N], ab[N], f[N], g[N];
+  float ag[N], ab[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) ag[j] = ab[j] = 0.f;
-  for (long r = ly; r < rows; r += 32) {
+#pragma unroll 4
+  for (long r = r0 + ly; r < r1; r += 32) {
     const float m = mean[r], rs = rstd[r];
-    load_row(dy + r * lddy, c, n, g);
-    load_row(x + r * ldx, c, n, f);
+    Vec<T> g, v;
+    g.load(dy + r * lddy, c, n);
+    v.load(x + r * ldx, c, n);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      ag[j] += c + j < n ? g[j] * (f[j] - m) * rs : 0.f;
+      ag[j] += g[j] * ((v[j] - m) * rs);
       ab[j] += g[j];
     }
   }
@@ -390,7 +445,7 @@ __global__ __launch_bounds__(256) void ln_cols_k(
     float s = 0.f;
 #pragma unroll
     for (int r = 0; r < 32; ++r) s += acc[which][r][k];
-    (which ? dbeta : dgamma)[col] = s;
+    (which ? dbeta : dgamma)[col] = col < n ? s : 0.f;
   }
 }
 
@@ -419,30 +474,34 @@ __global__ __launch_bounds__(1024) void ln_join_k(
   }
 }
 
-// lanes a row and vectors a lane: the fewest lanes whose registers hold
-// the row with up to 2 vectors each, up to a wave; wider rows take a
-// block.  v: 16-byte vectors a row has.
-#define LN_PICK(v, CALL)              \
-  do {                                \
-    if ((v) <= 8) CALL(8, 1);         \
-    else if ((v) <= 16) CALL(16, 1);  \
-    else if ((v) <= 32) CALL(32, 1);  \
-    else if ((v) <= 64) CALL(64, 1);  \
-    else if ((v) <= 128) CALL(64, 2); \
+// Lanes a row and vectors a lane: one 16-byte vector a lane as long as a
+// block has lanes enough.  Two vectors on half the lanes, tried at 1024 to
+// 8192 bf16 channels, ran at 60 to 80 % of that.  v: vectors a row has.
+#define LN_PICK(v, CALL)               \
+  do {                                 \
+    if ((v) <= 8) CALL(8, 1);          \
+    else if ((v) <= 16) CALL(16, 1);   \
+    else if ((v) <= 32) CALL(32, 1);   \
+    else if ((v) <= 64) CALL(64, 1);   \
+    else if ((v) <= 128) CALL(128, 1); \
     else if ((v) <= 256) CALL(256, 1); \
-    else if ((v) <= 512) CALL(256, 2); \
-    else if ((v) <= 1024) CALL(512, 2); \
-    else CALL(1024, 2);               \
+    else if ((v) <= 512) CALL(512, 1); \
+    else if ((v) <= 1024) CALL(1024, 1); \
+    else CALL(1024, 2);                \
   } while (0)
 
-constexpr long WIDEST = 2048;   // vectors a row may have for registers
+// Vectors a row may have for registers.  The backward's sums for two
+// vectors do not fit the 128 that 1024 threads have each (spilled it took
+// 120 us at 2048 x 16384 bf16): rows over 1024 vectors take the wide
+// kernel and the column kernel, which read x and dy twice, in 71 us.
+constexpr long WIDEST_FWD = 2048, WIDEST_BWD = 1024;
 
 template <typename T>
 hipError_t fwd(const void* x, const float* gamma, const float* beta,
                void* y, float* mean, float* rstd, long rows, int C, int n,
                long ldx, float eps, hipStream_t stream) {
   const long v = (C + Vec<T>::N - 1) / Vec<T>::N;
-  if (v > WIDEST) {
+  if (v > WIDEST_FWD) {
     hipLaunchKernelGGL(ln_fwd_wide_k<T>,
                        dim3((unsigned)(rows < 4096 ? rows : 4096)),
                        dim3(1024), 0, stream, (const T*)x, gamma, beta,
@@ -468,10 +527,10 @@ template <typename T>
 hipError_t bwd(const void* dy, const void* x, const float* gamma,
                const float* mean, const float* rstd, void* dx,
                float* dgamma, float* dbeta, float* part, long blocks,
-               long rows, int C, int n, long ldx, long lddy,
-               hipStream_t stream) {
+               long shares, int by_column, long rows, int C, int n,
+               long ldx, long lddy, hipStream_t stream) {
   const long v = (C + Vec<T>::N - 1) / Vec<T>::N;
-  if (v > WIDEST) {
+  if (v > WIDEST_BWD) {
     hipLaunchKernelGGL(ln_bwd_wide_k<T>,
                        dim3((unsigned)(rows < 4096 ? rows : 4096)),
                        dim3(1024), 0, stream, (const T*)dy, (const T*)x,
@@ -482,23 +541,28 @@ hipError_t bwd(const void* dy, const void* x, const float* gamma,
     constexpr int block = TPR > 256 ? TPR : 256;                        \
     hipLaunchKernelGGL((ln_bwd_k<T, TPR, NV>), dim3((unsigned)blocks),  \
                        dim3(block), 0, stream, (const T*)dy,            \
-                       (const T*)x, gamma, mean, rstd, (T*)dx, part,    \
+                       (const T*)x, gamma, mean, rstd, (T*)dx,          \
+                       by_column ? nullptr : part,                      \
                        rows, C, n, ldx, lddy);                          \
   } while (0)
     LN_PICK(v, LN_BWD);
 #undef LN_BWD
   }
   HIP_KERNEL_ASSERT_OK(hipGetLastError());
-  if (part) {
+  if (by_column) {
+    constexpr int per = 8 * Vec<T>::N;
+    hipLaunchKernelGGL(ln_cols_k<T>,
+                       dim3((unsigned)((C + per - 1) / per),
+                            (unsigned)(shares ? shares : 1)),
+                       dim3(256), 0, stream, (const T*)dy, (const T*)x,
+                       mean, rstd, dgamma, dbeta, shares ? part : nullptr,
+                       rows, C, n, ldx, lddy);
+    HIP_KERNEL_ASSERT_OK(hipGetLastError());
+  }
+  if (shares)
     hipLaunchKernelGGL(ln_join_k, dim3((unsigned)((2 * C + 15) / 16)),
                        dim3(1024), 0, stream, part, dgamma, dbeta,
-                       (int)blocks, C);
-  } else {
-    constexpr int per = 8 * Vec<T>::N;
-    hipLaunchKernelGGL(ln_cols_k<T>, dim3((unsigned)((C + per - 1) / per)),
-                       dim3(256), 0, stream, (const T*)dy, (const T*)x,
-                       mean, rstd, dgamma, dbeta, rows, C, n, ldx, lddy);
-  }
+                       (int)shares, C);
   return hipGetLastError();
 }
 
@@ -521,40 +585,52 @@ hipError_t launch_ln_fwd(const void* x, const float* gamma,
                      stream);
 }
 
-// How the backward is launched: *blocks row blocks, and whether their
-// shares of dgamma / dbeta go through a [blocks][2C] buffer (else the
-// column kernel makes both from x and dy).
-hipError_t ln_bwd_plan(long rows, int C, int kind, long* blocks,
-                       int* shares) {
+// How the backward is launched: *blocks row blocks; dgamma and dbeta from
+// these, or (*by_column) from the column kernel; *shares parts of them to
+// be joined, [shares][2C] floats (0: there is nothing to join).
+void ln_bwd_plan(long rows, int C, int kind, long* blocks, long* shares,
+                 int* by_column) {
   const int N = kind == 0 ? 4 : 8;
   const long v = (C + N - 1) / N;
-  int block = 256, tpr = 1024;
+  int tpr = 1024;
 #define LN_TPR(TPR, NV) tpr = TPR
   LN_PICK(v, LN_TPR);
 #undef LN_TPR
-  if (tpr > 256) block = tpr;
-  const int rpb = block / tpr;
-  long grid = (rows + rpb - 1) / rpb;
-  const long most = 256L * (1024 / block);
+  const int block = tpr > 256 ? tpr : 256, rpb = block / tpr;
+  // 16 waves a compute unit; 32 for narrow rows in f32, whose vectors are
+  // half as many values (300000 x 100: 62 against 100 us; but 4099 x 1000
+  // f32 19 against 14, 802816 x 256 bf16 252 against 228)
+  const long most = 256L * (kind == 0 && v <= 64 ? 2048 : 1024) / block;
+  const long grid = (rows + rpb - 1) / rpb;
   *blocks = grid < most ? grid : most;
-  *shares = v <= WIDEST && rows > 512;
-  return hipSuccess;
+  *by_column = v > WIDEST_BWD || rows <= 512;
+  *shares = *blocks;
+  if (*by_column) {
+    const long across = (C + 8 * N - 1) / (8 * N);
+    long down = (rows + 127) / 128;
+    if (down > (1024 + across - 1) / across)
+      down = (1024 + across - 1) / across;
+    *shares = rows <= 512 ? 0 : down;
+  }
 }
 
 hipError_t launch_ln_bwd(const void* dy, const void* x,
                          const float* gamma, const float* mean,
                          const float* rstd, void* dx, float* dgamma,
-                         float* dbeta, float* part, long blocks, long rows,
-                         int C, int n, long ldx, long lddy, int kind,
+                         float* dbeta, float* part, long blocks,
+                         long shares, int by_column, long rows, int C,
+                         int n, long ldx, long lddy, int kind,
                          hipStream_t stream) {
   if (kind == 0)
     return bwd<float>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part,
-                      blocks, rows, C, n, ldx, lddy, stream);
+                      blocks, shares, by_column, rows, C, n, ldx, lddy, stream);
   if (kind == 1)
     return bwd<_Float16>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta,
-                         part, blocks, rows, C, n, ldx, lddy, stream);
+                         part, blocks, shares, by_column, rows, C, n, ldx,
+                         lddy, stream);
   return bwd<__bf16>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part,
-                     blocks, rows, C, n, ldx, lddy, stream);
+                     blocks, shares, by_column, rows, C, n, ldx, lddy,
+                     stream);
 }
 
 }  // extern "C"

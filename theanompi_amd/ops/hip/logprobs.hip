@@ -29,7 +29,7 @@ constexpr int KMAX = 32;       // alternatives
 constexpr int MAXSEG = 256;    // segments a row
 
 constexpr int CAP = 256;       // candidates a block may collect
-constexpr float LOG2E = 1.44269504f;
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
 
 // What is kept of a row for the backward pass; M = -inf: a row of masked
 // classes.
@@ -66,14 +66,19 @@ DEV unsigned long long wave_max_key(unsigned long long v) {
 // lanes reach a value is a count of a ballot.  LOW: low bits that the
 // type leaves 0.
 template <int LOW>
-DEV float wave_kth(float v, int k) {
-  const unsigned u = ordered(v);
+DEV unsigned wave_kth_bits(unsigned u, int k) {
   unsigned best = 0;
 #pragma unroll
   for (int b = 31; b >= LOW; --b) {
     const unsigned t = best | (1u << b);
     if (__popcll(__ballot(u >= t)) >= k) best = t;
   }
+  return best;
+}
+
+template <int LOW>
+DEV float wave_kth(float v, int k) {
+  unsigned best = wave_kth_bits<LOW>(ordered(v), k);
   // negative numbers have their low bits the other way round
   if (LOW > 0 && !(best >> 31)) best |= (1u << LOW) - 1u;
   return unordered(best);
@@ -230,16 +235,37 @@ __global__ __launch_bounds__(LANES) void lp_fwd_k(
   }
   // a maximum of -inf (nothing but masked classes) cannot be taken off
   const float M = m == NINF ? 0.f : m;
+  // y = (x - M) log2 e in one fused step, x log2 e - c; what c = M log2 e
+  // lost in rounding, the same for all, is put right afterwards
+  const float c = M * LOG2E, off = fmaf(M, LOG2E, -c);
   float s = 0.f, t = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float d = p.get(i, j) - M;
-      const float e = __builtin_amdgcn_exp2f(d * LOG2E);
+      const float y = fmaf(p.get(i, j), LOG2E, -c);
+      const float e = __builtin_amdgcn_exp2f(y);
       s += e;
-      t = fmaf(e, fmaxf(d, -200.f), t);     // e is 0 long before
+      t = fmaf(e, y, t);
     }
+  const float fix = __builtin_amdgcn_exp2f(-off);
+  t = (t - off * s) * fix * LN2;
+  s *= fix;
+  if (t != t) {
+    // A masked class (0 * -inf), a NaN, or an M near the largest number
+    // that c does not hold: once more, step by step.  Lanes without have
+    // the same sums from both.
+    s = t = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float d = p.get(i, j) - M;
+        const float e = __builtin_amdgcn_exp2f(d * LOG2E);
+        s += e;
+        t = fmaf(e, fmaxf(d, -200.f), t);     // e is 0 long before
+      }
+  }
   if (k > 0) {
     const float least = fmaxf(tau, -__FLT_MAX__);    // above -inf
 #pragma unroll
@@ -331,7 +357,10 @@ __global__ __launch_bounds__(LANES) void lp_fwd_k(
   }
 }
 
-// one wave a row: the segments' sums and their sorted lists
+// One wave a row: the segments' sums and their sorted lists.  As in
+// lp_fwd_k, what reaches a lower bound of the row's k-th value goes into
+// one list, where a key's place is the number of keys before it; picking
+// the best head k times took 0.5 us a pick.
 template <typename T>
 __global__ __launch_bounds__(64) void lp_join_k(
     const T* __restrict__ x, const long* __restrict__ labels,
@@ -340,32 +369,37 @@ __global__ __launch_bounds__(64) void lp_join_k(
     RowStat* __restrict__ stat, const float* __restrict__ psum,
     const unsigned long long* __restrict__ pkey, int n, long ldx,
     int segs, int k) {
-  constexpr int H = MAXSEG / 64;
+  constexpr int H = MAXSEG / 64, HELD = 1024;
+  constexpr float NINF = -__builtin_inff();
+  __shared__ unsigned long long held[HELD];
   const long r = blockIdx.x;
   const int lane = threadIdx.x;
   const T* row = x + r * ldx;
+  const unsigned long long* lists = pkey + r * segs * k;
   const long lab = labels[r];
   const float xlab = lab >= 0 && lab < n ? (float)row[lab] : 0.f;
-  float m[H], s[H], t[H], M = -__builtin_inff();
-  unsigned long long head[H];      // each lane's segments' next best
-  int at[H];
+  float m[H], s[H], t[H], M = NINF;
+  unsigned long long head[H], best = 0, least = 0;
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     const int g = lane + h * 64;
-    const float* q = psum + (r * segs + g) * 3;
-    m[h] = g < segs ? q[0] : -__builtin_inff();
-    s[h] = g < segs ? q[1] : 0.f;
-    t[h] = g < segs ? q[2] : 0.f;
+    const bool there = g < segs;
+    const float* q = psum + (r * segs + (there ? g : 0)) * 3;
+    m[h] = there ? q[0] : NINF;
+    s[h] = there ? q[1] : 0.f;
+    t[h] = there ? q[2] : 0.f;
+    head[h] = there && k > 0 ? lists[g * k] : 0;
+    const unsigned long long last = there && k > 0 ? lists[g * k + k - 1] : 0;
     M = fmaxf(M, m[h]);
-    at[h] = 0;
-    head[h] = g < segs && k > 0 ? pkey[(r * segs + g) * k] : 0;
+    if (head[h] > best) best = head[h];
+    if (last > least) least = last;
   }
   M = lane_max<64>(M);
   float S = 0.f, U = 0.f;
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     // a segment of masked classes has nothing to be taken off
-    const float d = m[h] == -__builtin_inff() ? 0.f : m[h] - M;
+    const float d = m[h] == NINF ? 0.f : m[h] - M;
     const float e = __builtin_amdgcn_exp2f(d * LOG2E);
     S += e * s[h];
     U += e > 0.f ? e * (t[h] + d * s[h]) : 0.f;   // d may be -3e38
@@ -375,8 +409,42 @@ __global__ __launch_bounds__(64) void lp_join_k(
   const RowStat st = finish_row(M, S, U);
   if (lane == 0)
     write_row(stat, logp, entropy, r, n, lab, xlab, st);
+  if (k == 0) return;
+  auto put = [&](int place, unsigned long long key) {
+    top_idx[r * k + place] = key_index(key);
+    top_logp[r * k + place] = logp_of(st, key_value(key));
+  };
+  // a full list's last key, and the k-th of the lanes' best heads, are
+  // bounds from below (0: there is none)
+  unsigned bound = lane_max<64>((unsigned)(least >> 32));
+  if (segs > k) {
+    const unsigned other = wave_kth_bits<0>((unsigned)(best >> 32), k);
+    if (other > bound) bound = other;
+  }
+  int have = 0;
+  for (int j0 = 0; j0 < segs * k; j0 += 64) {
+    const int j = j0 + lane;
+    const unsigned long long key = j < segs * k ? lists[j] : 0;
+    const bool in = key != 0 && (unsigned)(key >> 32) >= bound;
+    const unsigned long long who = __ballot(in);
+    const int at = have + __popcll(who & ((1ull << lane) - 1));
+    if (in && at < HELD) held[at] = key;
+    have += __popcll(who);
+  }
+  __syncthreads();
+  if (have <= HELD) {
+    for (int a = lane; a < have; a += 64) {
+      const unsigned long long key = held[a];
+      int place = 0;
+#pragma unroll 8
+      for (int b = 0; b < have; ++b) place += held[b] > key;
+      if (place < k) put(place, key);
+    }
+    return;
+  }
+  int at[H] = {};
   for (int a = 0; a < k; ++a) {
-    unsigned long long best = 0;
+    best = 0;
 #pragma unroll
     for (int h = 0; h < H; ++h)
       if (head[h] > best) best = head[h];
@@ -386,13 +454,9 @@ __global__ __launch_bounds__(64) void lp_join_k(
       if (head[h] == best) {
         const int g = lane + h * 64;
         ++at[h];
-        head[h] = g < segs && at[h] < k
-                      ? pkey[(r * segs + g) * k + at[h]] : 0;
+        head[h] = g < segs && at[h] < k ? lists[g * k + at[h]] : 0;
       }
-    if (lane == 0) {
-      top_idx[r * k + a] = key_index(best);
-      top_logp[r * k + a] = logp_of(st, key_value(best));
-    }
+    if (lane == 0) put(a, best);
   }
 }
 

@@ -137,11 +137,11 @@ hipError_t launch_splitk_finalize(float*, const float*, void*, long,
 hipError_t launch_ln_fwd(const void*, const float*, const float*, void*,
                          float*, float*, long, int, int, long, float, int,
                          hipStream_t);
-void ln_bwd_plan(long, int, int, long*, long*, int*);
+void ln_bwd_plan(long, int, int, long*, long*);
 hipError_t launch_ln_bwd(const void*, const void*, const float*,
                          const float*, const float*, void*, float*,
-                         float*, float*, long, long, int, long, int, int,
-                         long, long, int, hipStream_t);
+                         float*, float*, long, long, long, int, int, long,
+                         long, int, hipStream_t);
 int lp_plan(long, long, int, int*, int*);
 hipError_t launch_lp_fwd(const void*, const long*, float*, float*, float*,
                          long*, float*, float*, unsigned long long*, long,
@@ -1209,8 +1209,7 @@ static std::vector<torch::Tensor> ln_bwd(torch::Tensor dy,
   auto dbeta = torch::empty({C}, gamma.options());
   if (!rows) return {dx, dgamma.zero_(), dbeta.zero_()};
   long blocks, shares;
-  int by_column;
-  ln_bwd_plan(rows, (int)C, kind, &blocks, &shares, &by_column);
+  ln_bwd_plan(rows, (int)C, kind, &blocks, &shares);
   torch::Tensor part;
   if (shares) part = torch::empty({shares * 2 * C}, gamma.options());
   const float* st = stat.data_ptr<float>();
@@ -1219,8 +1218,8 @@ static std::vector<torch::Tensor> ln_bwd(torch::Tensor dy,
                           dx.data_ptr(), dgamma.data_ptr<float>(),
                           dbeta.data_ptr<float>(),
                           shares ? part.data_ptr<float>() : nullptr,
-                          blocks, shares, by_column, rows, (int)C, (int)n,
-                          ldx, lddy, kind, cur_stream()));
+                          blocks, shares, rows, (int)C, (int)n, ldx, lddy,
+                          kind, cur_stream()));
   return {dx, dgamma, dbeta};
 }
 
@@ -1233,6 +1232,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
                                const torch::Tensor& gamma,
                                const torch::Tensor& beta, double eps,
                                int64_t n) {
+    at::AutoDispatchBelowADInplaceOrView below;
     auto r = ln_fwd(x, gamma, beta, n, eps);
     ctx->save_for_backward({x, gamma, r[1]});
     ctx->saved_data["n"] = n;
@@ -1242,7 +1242,11 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
       torch::autograd::AutogradContext* ctx,
       torch::autograd::variable_list dy) {
     const auto s = ctx->get_saved_variables();
-    auto r = ln_bwd(dy[0], s[0], s[1], s[2], ctx->saved_data["n"].toInt());
+    std::vector<torch::Tensor> r;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      r = ln_bwd(dy[0], s[0], s[1], s[2], ctx->saved_data["n"].toInt());
+    }
     return once(r, {torch::Tensor(), torch::Tensor()});
   }
 };
@@ -1284,18 +1288,16 @@ static std::vector<torch::Tensor> lp_fwd(torch::Tensor x,
     const long segs = lp_plan(rows, n, kind, &lanes, &nv);
     TORCH_CHECK(segs > 0, "n_classes ", n, " is over what a row may have");
     TORCH_CHECK(rows * segs < (1L << 31), "too many rows");
-    torch::Tensor psum, pkey;
-    if (segs > 1) {
-      psum = torch::empty({rows * segs * 3}, f32);
-      pkey = torch::empty({rows * segs * k}, i64);
-    }
+    torch::Tensor parts;           // keys, then sums, of every segment
+    if (segs > 1)
+      parts = torch::empty({rows * segs * (k + 2)}, i64);
+    auto* pkey = segs > 1 ? (unsigned long long*)parts.data_ptr() : nullptr;
+    auto* psum = segs > 1 ? (float*)(pkey + rows * segs * k) : nullptr;
     CHECK_HIP(launch_lp_fwd(
         x.data_ptr(), labels.data_ptr<long>(), logp.data_ptr<float>(),
         entropy.data_ptr<float>(), top_logp.data_ptr<float>(),
         top_idx.data_ptr<long>(), stat.data_ptr<float>(),
-        segs > 1 ? psum.data_ptr<float>() : nullptr,
-        segs > 1 ? (unsigned long long*)pkey.data_ptr() : nullptr, rows,
-        (int)n, ld, (int)segs, lanes, nv, (int)k, kind, cur_stream()));
+        psum, pkey, rows, (int)n, ld, (int)segs, lanes, nv, (int)k, kind, cur_stream()));
   }
   return {logp, entropy, top_logp, top_idx, stat};
 }
@@ -1339,6 +1341,7 @@ struct LabelLogprobsFn : torch::autograd::Function<LabelLogprobsFn> {
   static torch::autograd::variable_list forward(
       torch::autograd::AutogradContext* ctx, const torch::Tensor& logits,
       const torch::Tensor& labels, int64_t n, int64_t k) {
+    at::AutoDispatchBelowADInplaceOrView below;
     auto r = lp_fwd(logits, labels, n, k);
     ctx->save_for_backward({logits, labels, r[3], r[4]});
     ctx->saved_data["n"] = n;
@@ -1356,8 +1359,12 @@ struct LabelLogprobsFn : torch::autograd::Function<LabelLogprobsFn> {
     torch::Tensor none;
     if (!d[0].defined() && !d[1].defined() && !d[2].defined())
       return {none, none, none, none};
-    auto dx = lp_bwd(s[0], s[1], s[2], s[3], opt(d[0]), opt(d[1]),
-                     opt(d[2]), ctx->saved_data["n"].toInt());
+    torch::Tensor dx;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      dx = lp_bwd(s[0], s[1], s[2], s[3], opt(d[0]), opt(d[1]), opt(d[2]),
+                  ctx->saved_data["n"].toInt());
+    }
     return once({dx}, {none, none, none});
   }
 };

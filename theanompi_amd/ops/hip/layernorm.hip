@@ -224,15 +224,68 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_k(
   }
 }
 
-// dx, and this block's share of dgamma / dbeta: part[block][2][C] (null:
-// the column kernel makes them)
-template <typename T, int TPR, int NV>
+// dgamma / dbeta of a group of channels straight from x and dy, over rows
+// r0 to r1, by a block's first 256 threads: for few rows and for rows too
+// wide for ln_bwd_k.  8 lanes x 16 bytes across, 32 rows down, then a
+// fixed-order sum in LDS.
+template <typename T>
+DEV void ln_cols(const T* __restrict__ dy, const T* __restrict__ x,
+                 const float* __restrict__ mean,
+                 const float* __restrict__ rstd, float* dgamma,
+                 float* dbeta, int group, long r0, long r1, int C, int n,
+                 long ldx, long lddy) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float acc[2][32][8 * N + 1];
+  const int lx = threadIdx.x & 7, ly = threadIdx.x >> 3;
+  const int c = (group * 8 + lx) * N;
+  if (threadIdx.x < 256) {
+    float ag[N], ab[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) ag[j] = ab[j] = 0.f;
+#pragma unroll 4
+    for (long r = r0 + ly; r < r1; r += 32) {
+      const float m = mean[r], rs = rstd[r];
+      Vec<T> g, v;
+      g.load(dy + r * lddy, c, n);
+      v.load(x + r * ldx, c, n);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        ag[j] += g[j] * ((v[j] - m) * rs);
+        ab[j] += g[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      acc[0][ly][lx * N + j] = ag[j];
+      acc[1][ly][lx * N + j] = ab[j];
+    }
+  }
+  __syncthreads();
+  const int which = threadIdx.x / (8 * N), k = threadIdx.x % (8 * N);
+  const int col = group * 8 * N + k;
+  if (which < 2 && col < C) {
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) s += acc[which][r][k];
+    (which ? dbeta : dgamma)[col] = col < n ? s : 0.f;
+  }
+}
+
+// dx, and dgamma / dbeta: this block's share of them, part[block][2][C],
+// or (FEW rows) all of them from the blocks behind the first `blocks`,
+// which go by columns.
+template <typename T, int TPR, int NV, bool FEW>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
     const T* __restrict__ dy, const T* __restrict__ x,
     const float* __restrict__ gamma, const float* __restrict__ mean,
     const float* __restrict__ rstd, T* __restrict__ dx,
-    float* __restrict__ part, long rows, int C, int n, long ldx,
-    long lddy) {
+    float* __restrict__ part, float* dgamma, float* dbeta, int blocks,
+    long rows, int C, int n, long ldx, long lddy) {
+  if (FEW && (int)blockIdx.x >= blocks) {
+    ln_cols(dy, x, mean, rstd, dgamma, dbeta, (int)blockIdx.x - blocks, 0,
+            rows, C, n, ldx, lddy);
+    return;
+  }
   constexpr int N = Vec<T>::N;
   constexpr int BLOCK = TPR > 256 ? TPR : 256;
   constexpr int RPB = BLOCK / TPR;
@@ -241,7 +294,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
   int turn = 0;
   const int lane = threadIdx.x % TPR;
   const float inv_n = 1.f / (float)n;
-  const long step = (long)gridDim.x * RPB;
+  const long step = (long)blocks * RPB;
   long r = (long)blockIdx.x * RPB + threadIdx.x / TPR;
   // the next row, as loaded: what is computed from it is computed twice
   // rather than kept over the sums
@@ -286,8 +339,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
         // behind the row's end dy and gamma are 0, and so is what a row
         // that is not there adds; x is 0 there, and xh is finite
         const float xh = (vx[i][j] - m) * rs, d = vy[i][j];
-        ag[i][j] += d * xh;
-        ab[i][j] += d;
+        if (!FEW) {
+          ag[i][j] += d * xh;
+          ab[i][j] += d;
+        }
         s[0] += d * ga[i][j];
         s[1] += d * ga[i][j] * xh;
       }
@@ -306,51 +361,52 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
       }
     }
   }
-  if (!part) return;
-  float* pg = part + (long)blockIdx.x * 2 * C;
-  float* pb = pg + C;
-  // channels behind n have no gradient, whatever a row's NaN makes of 0
-  if constexpr (TPR >= 256) {
+  if constexpr (!FEW) {
+    float* pg = part + (long)blockIdx.x * 2 * C;
+    float* pb = pg + C;
+    // channels behind n have no gradient, whatever a row's NaN makes of 0
+    if constexpr (TPR >= 256) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int c = (lane + i * TPR) * N + j;
-        if (c < C) {
-          pg[c] = c < n ? ag[i][j] : 0.f;
-          pb[c] = c < n ? ab[i][j] : 0.f;
+        for (int j = 0; j < N; ++j) {
+          const int c = (lane + i * TPR) * N + j;
+          if (c < C) {
+            pg[c] = c < n ? ag[i][j] : 0.f;
+            pb[c] = c < n ? ab[i][j] : 0.f;
+          }
         }
-      }
-  } else {
-    // the block's row groups are added up in a fixed order: within a
-    // wave by exchange, between waves (or pairs of them) in LDS
-    constexpr int SLOTS = TPR <= 64 ? WAVES : RPB;
-    __shared__ float acc[2][SLOTS][TPR * NV * N];
-    const int slot = TPR <= 64 ? threadIdx.x >> 6 : threadIdx.x / TPR;
+    } else {
+      // the block's row groups are added up in a fixed order: within a
+      // wave by exchange, between waves (or pairs of them) in LDS
+      constexpr int SLOTS = TPR <= 64 ? WAVES : RPB;
+      __shared__ float acc[2][SLOTS][TPR * NV * N];
+      const int slot = TPR <= 64 ? threadIdx.x >> 6 : threadIdx.x / TPR;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
+        for (int j = 0; j < N; ++j) {
 #pragma unroll
-        for (int off = 32; off >= TPR; off >>= 1) {
-          ag[i][j] += __shfl_xor(ag[i][j], off, 64);
-          ab[i][j] += __shfl_xor(ab[i][j], off, 64);
+          for (int off = 32; off >= TPR; off >>= 1) {
+            ag[i][j] += __shfl_xor(ag[i][j], off, 64);
+            ab[i][j] += __shfl_xor(ab[i][j], off, 64);
+          }
+          if (TPR >= 64 || (threadIdx.x & 63) < TPR) {
+            acc[0][slot][(lane + i * TPR) * N + j] = ag[i][j];
+            acc[1][slot][(lane + i * TPR) * N + j] = ab[i][j];
+          }
         }
-        if (TPR >= 64 || (threadIdx.x & 63) < TPR) {
-          acc[0][slot][(lane + i * TPR) * N + j] = ag[i][j];
-          acc[1][slot][(lane + i * TPR) * N + j] = ab[i][j];
-        }
-      }
-    __syncthreads();
-    for (int c = threadIdx.x; c < C; c += BLOCK) {
-      float sg = 0.f, sb = 0.f;
+      __syncthreads();
+      for (int c = threadIdx.x; c < C; c += BLOCK) {
+        float sg = 0.f, sb = 0.f;
 #pragma unroll
-      for (int w = 0; w < SLOTS; ++w) {
-        sg += acc[0][w][c];
-        sb += acc[1][w][c];
+        for (int w = 0; w < SLOTS; ++w) {
+          sg += acc[0][w][c];
+          sb += acc[1][w][c];
+        }
+        pg[c] = c < n ? sg : 0.f;
+        pb[c] = c < n ? sb : 0.f;
       }
-      pg[c] = c < n ? sg : 0.f;
-      pb[c] = c < n ? sb : 0.f;
     }
   }
 }
@@ -397,56 +453,16 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide_k(
   }
 }
 
-// dgamma / dbeta of a group of channels straight from x and dy: for few
-// rows and for rows too wide for ln_bwd_k.  8 lanes x 16 bytes across,
-// 32 rows down, then a fixed-order sum in LDS.  With `part`, of one of
-// gridDim.y ranges of rows, to be joined.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_cols_k(
     const T* __restrict__ dy, const T* __restrict__ x,
     const float* __restrict__ mean, const float* __restrict__ rstd,
-    float* __restrict__ dgamma, float* __restrict__ dbeta,
     float* __restrict__ part, long rows, int C, int n, long ldx,
     long lddy) {
-  constexpr int N = Vec<T>::N;
-  __shared__ float acc[2][32][8 * N + 1];
-  const long r0 = rows * blockIdx.y / gridDim.y;
-  const long r1 = rows * (blockIdx.y + 1) / gridDim.y;
-  if (part) {
-    dgamma = part + (long)blockIdx.y * 2 * C;
-    dbeta = dgamma + C;
-  }
-  const int lx = threadIdx.x & 7, ly = threadIdx.x >> 3;
-  const int c = (blockIdx.x * 8 + lx) * N;
-  float ag[N], ab[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) ag[j] = ab[j] = 0.f;
-#pragma unroll 4
-  for (long r = r0 + ly; r < r1; r += 32) {
-    const float m = mean[r], rs = rstd[r];
-    Vec<T> g, v;
-    g.load(dy + r * lddy, c, n);
-    v.load(x + r * ldx, c, n);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      ag[j] += g[j] * ((v[j] - m) * rs);
-      ab[j] += g[j];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    acc[0][ly][lx * N + j] = ag[j];
-    acc[1][ly][lx * N + j] = ab[j];
-  }
-  __syncthreads();
-  const int which = threadIdx.x / (8 * N), k = threadIdx.x % (8 * N);
-  const int col = blockIdx.x * 8 * N + k;
-  if (which < 2 && col < C) {
-    float s = 0.f;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) s += acc[which][r][k];
-    (which ? dbeta : dgamma)[col] = col < n ? s : 0.f;
-  }
+  float* dgamma = part + (long)blockIdx.y * 2 * C;
+  ln_cols(dy, x, mean, rstd, dgamma, dgamma + C, blockIdx.x,
+          rows * blockIdx.y / gridDim.y, rows * (blockIdx.y + 1) / gridDim.y,
+          C, n, ldx, lddy);
 }
 
 // the blocks' shares, added up in a fixed order: 16 channels across, 64
@@ -527,38 +543,42 @@ template <typename T>
 hipError_t bwd(const void* dy, const void* x, const float* gamma,
                const float* mean, const float* rstd, void* dx,
                float* dgamma, float* dbeta, float* part, long blocks,
-               long shares, int by_column, long rows, int C, int n,
+               long shares, long rows, int C, int n,
                long ldx, long lddy, hipStream_t stream) {
   const long v = (C + Vec<T>::N - 1) / Vec<T>::N;
+  constexpr int per = 8 * Vec<T>::N;
+  const unsigned across = (unsigned)((C + per - 1) / per);
   if (v > WIDEST_BWD) {
     hipLaunchKernelGGL(ln_bwd_wide_k<T>,
                        dim3((unsigned)(rows < 4096 ? rows : 4096)),
                        dim3(1024), 0, stream, (const T*)dy, (const T*)x,
                        gamma, mean, rstd, (T*)dx, rows, C, n, ldx, lddy);
+    HIP_KERNEL_ASSERT_OK(hipGetLastError());
+    hipLaunchKernelGGL(ln_cols_k<T>, dim3(across, (unsigned)shares),
+                       dim3(256), 0, stream, (const T*)dy, (const T*)x,
+                       mean, rstd, part, rows, C, n, ldx, lddy);
   } else {
+    const unsigned all = (unsigned)blocks + (shares ? 0 : across);
 #define LN_BWD(TPR, NV)                                                 \
   do {                                                                  \
     constexpr int block = TPR > 256 ? TPR : 256;                        \
-    hipLaunchKernelGGL((ln_bwd_k<T, TPR, NV>), dim3((unsigned)blocks),  \
-                       dim3(block), 0, stream, (const T*)dy,            \
-                       (const T*)x, gamma, mean, rstd, (T*)dx,          \
-                       by_column ? nullptr : part,                      \
-                       rows, C, n, ldx, lddy);                          \
+    if (shares)                                                         \
+      hipLaunchKernelGGL((ln_bwd_k<T, TPR, NV, false>), dim3(all),      \
+                         dim3(block), 0, stream, (const T*)dy,          \
+                         (const T*)x, gamma, mean, rstd, (T*)dx, part,  \
+                         dgamma, dbeta, (int)blocks, rows, C, n, ldx,   \
+                         lddy);                                         \
+    else                                                                \
+      hipLaunchKernelGGL((ln_bwd_k<T, TPR, NV, true>), dim3(all),       \
+                         dim3(block), 0, stream, (const T*)dy,          \
+                         (const T*)x, gamma, mean, rstd, (T*)dx, part,  \
+                         dgamma, dbeta, (int)blocks, rows, C, n, ldx,   \
+                         lddy);                                         \
   } while (0)
     LN_PICK(v, LN_BWD);
 #undef LN_BWD
   }
   HIP_KERNEL_ASSERT_OK(hipGetLastError());
-  if (by_column) {
-    constexpr int per = 8 * Vec<T>::N;
-    hipLaunchKernelGGL(ln_cols_k<T>,
-                       dim3((unsigned)((C + per - 1) / per),
-                            (unsigned)(shares ? shares : 1)),
-                       dim3(256), 0, stream, (const T*)dy, (const T*)x,
-                       mean, rstd, dgamma, dbeta, shares ? part : nullptr,
-                       rows, C, n, ldx, lddy);
-    HIP_KERNEL_ASSERT_OK(hipGetLastError());
-  }
   if (shares)
     hipLaunchKernelGGL(ln_join_k, dim3((unsigned)((2 * C + 15) / 16)),
                        dim3(1024), 0, stream, part, dgamma, dbeta,
@@ -585,13 +605,20 @@ hipError_t launch_ln_fwd(const void* x, const float* gamma,
                      stream);
 }
 
-// How the backward is launched: *blocks row blocks; dgamma and dbeta from
-// these, or (*by_column) from the column kernel; *shares parts of them to
-// be joined, [shares][2C] floats (0: there is nothing to join).
-void ln_bwd_plan(long rows, int C, int kind, long* blocks, long* shares,
-                 int* by_column) {
+// How the backward is launched: *blocks row blocks, and *shares parts of
+// dgamma and dbeta to be joined, [shares][2C] floats (0: few rows, whose
+// columns are summed in one go).
+void ln_bwd_plan(long rows, int C, int kind, long* blocks, long* shares) {
   const int N = kind == 0 ? 4 : 8;
   const long v = (C + N - 1) / N;
+  if (v > WIDEST_BWD) {
+    const long across = (C + 8 * N - 1) / (8 * N);
+    const long most = (1024 + across - 1) / across;
+    const long down = (rows + 127) / 128;
+    *blocks = 0;
+    *shares = down < most ? down : most;
+    return;
+  }
   int tpr = 1024;
 #define LN_TPR(TPR, NV) tpr = TPR
   LN_PICK(v, LN_TPR);
@@ -603,33 +630,25 @@ void ln_bwd_plan(long rows, int C, int kind, long* blocks, long* shares,
   const long most = 256L * (kind == 0 && v <= 64 ? 2048 : 1024) / block;
   const long grid = (rows + rpb - 1) / rpb;
   *blocks = grid < most ? grid : most;
-  *by_column = v > WIDEST_BWD || rows <= 512;
-  *shares = *blocks;
-  if (*by_column) {
-    const long across = (C + 8 * N - 1) / (8 * N);
-    long down = (rows + 127) / 128;
-    if (down > (1024 + across - 1) / across)
-      down = (1024 + across - 1) / across;
-    *shares = rows <= 512 ? 0 : down;
-  }
+  *shares = rows <= 512 ? 0 : *blocks;
 }
 
 hipError_t launch_ln_bwd(const void* dy, const void* x,
                          const float* gamma, const float* mean,
                          const float* rstd, void* dx, float* dgamma,
                          float* dbeta, float* part, long blocks,
-                         long shares, int by_column, long rows, int C,
-                         int n, long ldx, long lddy, int kind,
+                         long shares, long rows, int C, int n,
+                         long ldx, long lddy, int kind,
                          hipStream_t stream) {
   if (kind == 0)
     return bwd<float>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part,
-                      blocks, shares, by_column, rows, C, n, ldx, lddy, stream);
+                      blocks, shares, rows, C, n, ldx, lddy, stream);
   if (kind == 1)
     return bwd<_Float16>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta,
-                         part, blocks, shares, by_column, rows, C, n, ldx,
+                         part, blocks, shares, rows, C, n, ldx,
                          lddy, stream);
   return bwd<__bf16>(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, part,
-                     blocks, shares, by_column, rows, C, n, ldx, lddy,
+                     blocks, shares, rows, C, n, ldx, lddy,
                      stream);
 }
 

@@ -479,6 +479,23 @@ def test_label_logprobs_gpu_agrees_with_the_fused_loss():
         float((idx[:, 0] != labels).float().mean()))
 
 
+@gpu
+def test_label_logprobs_gpu_most_classes():
+    for dtype, most in ((torch.float32, 2 ** 21), (torch.bfloat16, 2 ** 22)):
+        x = torch.zeros(1, most + 1, dtype=dtype, device=dev())
+        x[0, most - 1] = 20.0
+        labels = torch.full((1,), most - 1, device=dev())
+        logp, _, _, idx = OF.label_logprobs(x, labels, n_classes=most,
+                                            top=3)
+        want = -math.log1p((most - 1) * math.exp(-20.0))
+        # sums of 2^22 equal terms: DEPTH roundings of the sum, on its
+        # logarithm, and of the logit
+        assert abs(float(logp) - want) < DEPTH * U + 40 * U
+        assert idx[0].tolist() == [most - 1, 0, 1]
+        with pytest.raises(RuntimeError):
+            OF.label_logprobs(x, labels)
+
+
 def test_label_logprobs_refusals():
     x, labels = lp_inputs(4, 9, torch.float32, "cpu")
     with pytest.raises(TypeError):
@@ -675,7 +692,8 @@ def muon_check(shapes, device, phase=0, copies=True):
     wds = [0.1 * (i % 3) for i in range(many)]
     scales = [1.0 + i for i in range(many)]
     old = [[t.double().cpu() for t in part] for part in (ws, gs, vs)]
-    OF.muon_update(ws, gs, vs, outs, lrs, wds, 0.9, scales, phase)
+    given = gs if phase != 2 else [None] * many        # not read
+    OF.muon_update(ws, given, vs, outs, lrs, wds, 0.9, scales, phase)
     for i in range(many):
         w, g, v = (part[i] for part in old)
         if phase != 2:
@@ -771,8 +789,10 @@ def muon_refusals(device):
     assert isinstance(call(outs=lambda v: [v[0], v[1].float()]), TypeError)
     assert isinstance(call(outs=lambda v: [v[0], v[1][:1]]), ValueError)
     same = lambda v: [v[0], v[0].view(4, 6)]          # noqa: E731
-    assert isinstance(call(ws=same, gs=same, vs=same, outs=same),
-                      ValueError)
+    for k in ("ws", "vs", "outs"):
+        every = {j: (same if j == k else lambda v: [
+            v[0], v[0].clone()]) for j in ("ws", "gs", "vs", "outs")}
+        assert isinstance(call(**every), ValueError), k
     assert isinstance(call(phase=3), ValueError)
     for steps in (0, 65, 2.0):
         assert isinstance(call(steps=steps), ValueError)
@@ -869,6 +889,36 @@ def test_layernorm_layer_cpu():
                                                      (10,))) < 16 * U
     names = [n for n, _, _ in ln.logical_params()]
     assert names == ["gamma", "beta"]
+
+
+@gpu
+def test_muon_trains_a_model_gpu():
+    """A convolutional network's step: padded weight entries stay 0, the
+    working copies follow the masters, and every weight moves by about
+    lr * rms (between half and 1.3 times: the singular values end between
+    0.68 and 1.21, and merged or padded matrices have some at 0)."""
+    from theanompi_amd.lib.opt import Muon
+    from theanompi_amd.models.cifar10 import Cifar10_model
+    for sync in ("cdd", "avg", "grad"):
+        m = Cifar10_model({"device": "cuda:0", "n_iters": 2,
+                           "batch_size": 16, "verbose": False,
+                           "optimizer": "muon"})
+        m.compile_iter_fns(sync)
+        assert type(m.opt) is Muon
+        before = [r.master.data.clone() for r in m.recs]
+        m.train_iter(0)
+        m.apply_update()
+        for r, b in zip(m.recs, before):
+            w = r.master.data
+            assert torch.isfinite(w).all()
+            if r.matrix is None:
+                continue
+            assert not w[b == 0].any()
+            assert torch.equal(r.bf16_out, w.to(torch.bfloat16))
+            lr, wd = m.opt.lr, m.opt.weight_decay
+            step = (w - (1 - lr * wd) * b)[b != 0]
+            rms = float(step.square().mean().sqrt()) / (lr * m.opt.rms)
+            assert 0.3 < rms < 1.3, (sync, r.name, rms)
 
 
 class _Head(torch.nn.Module):

@@ -565,8 +565,9 @@ def label_logprobs(logits, labels, n_classes=None, top=0):
     classes: probability 0, and no gradient unless the label or an
     alternative names them.  A row of masked classes alone has logp
     -inf, entropy 0 and gradient 0.  A NaN or +inf gives
-    NaN in its row.  Differentiable once in the logits, through logp,
-    entropy and top_logp."""
+    NaN in its row.  On the GPU a row may have 2^21 classes in float32,
+    2^22 in the 16-bit types.  Differentiable once in the logits, through
+    logp, entropy and top_logp."""
     _check_float(logits, "logits")
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [rows, classes], not "
@@ -629,7 +630,7 @@ def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
     rows, cols] (each matrix of a batch on its own); ``outs``: bf16
     working copies of w, or None in the place of one that is not kept.
     ``phase``: 0 the whole update, 1 the momentum only, 2 the weights
-    only (g is not read), as in the SGD step.  On the GPU every matrix
+    only (gs are not read and may be None), as in the SGD step.  On the GPU every matrix
     of the list goes through each product in one launch."""
     many = len(ws)
     for name, part in (("gs", gs), ("vs", vs), ("outs", outs),
@@ -669,11 +670,12 @@ def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
                 raise ValueError(f"out {i} must be contiguous, of its "
                                  "weight's size and on its device")
         if w.numel():
-            for t in (w, vs[i]):
-                if t.data_ptr() in seen:
-                    raise ValueError("a weight or momentum is in the "
-                                     "list twice")
-                seen.add(t.data_ptr())
+            for t in (w, vs[i], outs[i]):
+                if t is not None and t.data_ptr() in seen:
+                    raise ValueError("a weight, momentum or working copy "
+                                     "is in the list twice")
+                if t is not None:
+                    seen.add(t.data_ptr())
     keeps = [1.0 - lr * wd for lr, wd in zip(lrs, wds)]
     rates = [lr * scale for lr, scale in zip(lrs, scales)]
     with torch.no_grad():
@@ -681,7 +683,8 @@ def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
             none = torch.empty(0, dtype=torch.bfloat16,
                                device=ws[0].device)
             _ops.ext().muon_update(
-                [w.detach() for w in ws], list(gs), list(vs),
+                [w.detach() for w in ws],
+                [none if phase == 2 else g for g in gs], list(vs),
                 [none if o is None else o for o in outs], keeps, rates,
                 float(momentum), phase, steps)
             return

@@ -28,6 +28,8 @@
 // kernel needs to know of them travels in its arguments, so a captured
 // graph holds it.
 
+#include <atomic>
+
 #include "common.hpp"
 #include "newton_schulz.hpp"
 
@@ -906,6 +908,19 @@ __global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
   }
 }
 
+// A kernel's dynamic LDS beyond the usual limit, once a device.
+hipError_t allow_lds(const void* kernel, int bytes,
+                     std::atomic<unsigned long>& allowed) {
+  int device;
+  HIP_KERNEL_ASSERT_OK(hipGetDevice(&device));
+  const unsigned long bit = 1ul << (device & 63);
+  if (allowed.load() & bit) return hipSuccess;
+  HIP_KERNEL_ASSERT_OK(hipFuncSetAttribute(
+      kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  allowed.fetch_or(bit);
+  return hipSuccess;
+}
+
 }  // namespace
 
 extern "C" {
@@ -990,10 +1005,10 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
 #define NS_GEMM(MODE, BT, WM, WN, S, DEEP)                               \
   do {                                                                   \
     constexpr int bytes = S * DEEP * BT * 256;                           \
-    static const hipError_t ok = hipFuncSetAttribute(                    \
-        (const void*)ns_gemm_k<MODE, BT, WM, WN, S, DEEP>,               \
-        hipFuncAttributeMaxDynamicSharedMemorySize, bytes);              \
-    HIP_KERNEL_ASSERT_OK(ok);                                            \
+    static std::atomic<unsigned long> allowed;                           \
+    HIP_KERNEL_ASSERT_OK(allow_lds(                                      \
+        (const void*)ns_gemm_k<MODE, BT, WM, WN, S, DEEP>, bytes,        \
+        allowed));                                                       \
     hipLaunchKernelGGL((ns_gemm_k<MODE, BT, WM, WN, S, DEEP>),           \
                        dim3(blocks), dim3(64 * WM * WN), bytes, stream,  \
                        *a);                                              \

@@ -211,24 +211,52 @@ DEV void store_split(_Float16* m, int ld, int R, int c, const float* f) {
   }
 }
 
-// the same into the result: N values of row R as stored, of `cols`
+// N neighbours as T, 16 bytes a store, wherever they lie
+template <typename T, int N>
+DEV void store_some(T* d, const float* f) {
+  constexpr int PER = 16 / sizeof(T);
+  if constexpr (N % PER == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += PER) {
+      union { u32x4 u; T t[PER]; } v;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) v.t[j] = (T)f[k + j];
+      ((any16*)(d + k))->v = v.u;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) d[j] = (T)f[j];
+  }
+}
+
+// N values into the result, from column c of `cols` on
 template <int N>
 DEV void store_result(const NsProb& p, long at, int c, int cols,
                       const float* f) {
+  if (N > 1 && c + N > cols) {
+    for (int j = 0; j < N && c + j < cols; ++j) {
+      float one = 0.f;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    if (c + j >= cols) break;
-    if (p.w) {
-      const float w = p.keep * p.w[at + j] + p.rate * f[j];
-      p.w[at + j] = w;
-      if (p.copy) ((__bf16*)p.copy)[at + j] = (__bf16)w;
-    } else if (p.kind == 0) {
-      ((float*)p.out)[at + j] = f[j];
-    } else if (p.kind == 1) {
-      ((_Float16*)p.out)[at + j] = (_Float16)f[j];
-    } else {
-      ((__bf16*)p.out)[at + j] = (__bf16)f[j];
+      for (int k = 0; k < N; ++k) one = j == k ? f[k] : one;
+      store_result<1>(p, at + j, c + j, cols, &one);
     }
+    return;
+  }
+  if (c >= cols) return;
+  if (p.w) {
+    float w[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = p.w[at + j];
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = p.keep * w[j] + p.rate * f[j];
+    store_some<float, N>(p.w + at, w);
+    if (p.copy) store_some<__bf16, N>((__bf16*)p.copy + at, w);
+  } else if (p.kind == 0) {
+    store_some<float, N>((float*)p.out + at, f);
+  } else if (p.kind == 1) {
+    store_some<_Float16, N>((_Float16*)p.out + at, f);
+  } else {
+    store_some<__bf16, N>((__bf16*)p.out + at, f);
   }
 }
 
@@ -295,8 +323,19 @@ DEV half8 frag_cols(const _Float16* lds, int c, int part) {
   return f;
 }
 
+// Blocks go to the 8 XCDs in turn, and each of these has its own L2: the
+// work's order is dealt out so that an XCD has neighbours, which share
+// rows and columns.  In turn every XCD read nearly all of both operands:
+// (us) 8 x 512 x 512 239 -> 188, 1536 x 1536 458 -> 439, 4096 x 9216
+// 5738 -> 5494.
+DEV int xcd_order(int block, int blocks) {
+  const int x = block & 7, each = blocks >> 3, more = blocks & 7;
+  return x * each + (x < more ? x : more) + (block >> 3);
+}
+
 // Where a tile of a product lies.  Of symmetric matrices (GRAM, SQUARE) the
-// tiles on and below the diagonal, row by row.
+// tiles on and below the diagonal, row by row; of X, eight rows at a time,
+// column by column, so that neighbours make a patch.
 template <int MODE, int BT>
 struct Tile {
   long mat;
@@ -305,14 +344,23 @@ struct Tile {
   DEV Tile(const NsProb& p, int b) {
     if (MODE == APPLY) {
       const int tn = p.np / BT, tiles = p.mp / BT * tn;
-      mat = b / tiles;
-      b %= tiles;
-      ti = b / tn;
-      tj = b % tn;
+      mat = 0;
+      if (p.batch > 1) {            // a division costs 0.1 us of start
+        mat = b / tiles;
+        b -= (int)mat * tiles;
+      }
+      const int band = b / (8 * tn), rows = p.mp / BT - band * 8;
+      b -= band * 8 * tn;
+      const int high = rows < 8 ? rows : 8;
+      tj = b / high;
+      ti = band * 8 + b - tj * high;
     } else {
       const int t = p.mp / BT, tiles = t * (t + 1) / 2;
-      mat = b / tiles;
-      b %= tiles;
+      mat = 0;
+      if (p.batch > 1) {
+        mat = b / tiles;
+        b -= (int)mat * tiles;
+      }
       ti = (int)((sqrtf(8.f * b + 1.f) - 1.f) * 0.5f);
       if (ti * (ti + 1) / 2 > b) --ti;
       if ((ti + 1) * (ti + 2) / 2 <= b) ++ti;
@@ -416,30 +464,42 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wr = wave / WN * (BT / WM), wc = wave % WN * (BT / WN);
-  const bool single = (int)blockIdx.x < a.whole;
-  const int run = (int)blockIdx.x - a.whole;
+  const int b = blockIdx.x;         // whole tiles and runs: each their share
+  const int order = b < a.whole ? xcd_order(b, a.whole)
+                    : a.whole + xcd_order(b - a.whole, gridDim.x - a.whole);
+  const bool single = order < a.whole;
+  const int run = order - a.whole;
   int i = 0, tile, first = 0, steps;
   if (single) {
-    while (i + 1 < a.count && (int)blockIdx.x >= a.tile0[i + 1]) ++i;
+    while (i + 1 < a.count && order >= a.tile0[i + 1]) ++i;
   } else {
     while (i + 1 < a.count && run >= a.start[i + 1]) ++i;
   }
   const NsProb& p = a.p[i];
   const int slices = (MODE == GRAM ? p.np : p.mp) / (32 * DEEP);
   if (single) {
-    tile = (int)blockIdx.x - a.tile0[i];
+    tile = order - a.tile0[i];
     steps = slices;
   } else {
     const int parts = a.parts[i];
-    tile = a.skip[i] + (run - a.start[i]) / parts;
-    const int part = (run - a.start[i]) % parts;
-    first = (int)((long)slices * part / parts);
-    steps = (int)((long)slices * (part + 1) / parts) - first;
+    tile = run - a.start[i];
+    steps = slices;
+    if (parts > 1) {
+      const int part = tile % parts;
+      tile /= parts;
+      first = slices * part / parts;
+      steps = slices * (part + 1) / parts - first;
+    }
+    tile += a.skip[i];
   }
   const Tile<MODE, BT> at(p, tile);
   const long mat = at.mat;
   const int r0 = at.ti * BT, c0 = at.tj * BT;
-  const float shift = p.shift[mat];
+  // asked for now, in a register of each lane, and not waited for before
+  // the end (a scalar load holds up all others)
+  int lazy = 0;
+  asm volatile("" : "+v"(lazy));
+  const float shift = MODE == SQUARE ? 1.f : p.shift[mat + lazy];
   const _Float16* X = (const _Float16*)p.X[a.step & 1]
                       + mat * 2 * p.mp * (long)p.np;
   const long sq = mat * 2 * p.mp * (long)p.mp;
@@ -1027,6 +1087,7 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
   } while (0)
   if (bt == 256) NS_MODES(256, 2, 4, 2, 1);
   else if (bt == 128) NS_MODES(128, 2, 2, 2, 1);
+  else if (blocks <= 256) NS_MODES(64, 2, 2, 4, 2);
   else NS_MODES(64, 2, 2, 2, 2);
 #undef NS_MODES
 #undef NS_GEMM

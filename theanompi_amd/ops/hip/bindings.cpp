@@ -1379,7 +1379,11 @@ static std::vector<torch::Tensor> label_logprobs(
 
 // Which kernels a matrix takes: 0, those for few rows; else the tile of
 // the general ones, larger where there is work enough for all compute
-// units.
+// units.  Measured (us, 5 steps), few rows against tiles of 64: 64 x 576
+// 44, 102; 64 x 16384 132, 141; 100 x 64 x 64 39, 88.  Tiles of 64, 128 and
+// 256: 1536 x 1536 440, 491, 523; 1536 x 4096 739, 674, 729; 32 x 512 x 512
+// 516, 512, 549; 3000 x 3000 2116, 1900, 1945; 4096 x 4096 5290, 3562,
+// 3461; 4096 x 9216 10644, 5717, 5547.
 static int ns_tile(const NsProb& p) {
   if (p.m <= 64) return 0;
   const long size = (long)p.batch * p.m * p.n;
@@ -1468,11 +1472,22 @@ static void ns_run(NsArgs& a, long steps,
     return;
   }
   // Two steps at a time cost a Gram matrix and an X product less and
-  // three products of m x m more: at m = 4096 406 + 750 us against 650,
-  // at n = 9216.  They pay from about n = 2m on, where the device is full.
-  bool pairs = a.tile >= 128;
-  for (int i = 0; i < a.count; ++i)
-    pairs = pairs && a.p[i].n >= 2L * a.p[i].m;
+  // three products of m x m more.  On a full device that pays from about
+  // n = 2m on (us: 2048 x 4096 1022 -> 981, 4096 x 9216 6535 -> 5545, but
+  // 2048 x 3000 874 -> 888); a smaller matrix waits for each launch, and
+  // has to be longer and large enough (1000 x 3000 381 -> 367, 512 x 4608
+  // 241 -> 222, the weights of a wide residual network 222 -> 205, but
+  // 1000 x 2000 288 -> 312, 512 x 2048 177 -> 184).
+  double size = 0.0, wide = 0.0, square = 0.0;
+  for (int i = 0; i < a.count; ++i) {
+    const NsProb& p = a.p[i];
+    const double one = (double)p.batch * p.m * p.n;
+    size += one;
+    wide += one * p.m;
+    square += (double)p.batch * p.m * p.m * p.m;
+  }
+  const bool pairs = a.tile >= 128 ? wide >= 2.0 * square
+                     : wide >= 2.9 * square && size >= (1L << 21);
   auto product = [&](int mode, int s1, int s2, int to, int poly) {
     a.s1 = s1;
     a.s2 = s2;

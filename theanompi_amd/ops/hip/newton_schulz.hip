@@ -20,13 +20,21 @@
 // Layout: a "split" matrix of R rows and K columns (both padded to the
 // tile with zeros, which every step keeps) is [R][K/32][2][32] halves,
 // 32 hi then 32 lo: a 32-deep slice of a row is one 128-byte line.
-// A, M and their products are symmetric: only tiles on and below the diagonal are
-// computed, each written twice.
+// A, M and their products are symmetric: only tiles on and below the
+// diagonal are computed, each written twice.
 //
 // Where n is large against m, two steps use X once (see ns_run): what X
-// X^T is after a step is A' = M A M, and X <- (M' M) X.  All matrices of a call go through each step in one launch; what a
-// kernel needs to know of them travels in its arguments, so a captured
-// graph holds it.
+// X^T is after a step is A' = M A M, and X <- (M' M) X.  All matrices of a
+// call go through each step in one launch; what a kernel needs to know of
+// them travels in its arguments, so a captured graph holds it.
+//
+// What bounds it, 5 steps: large matrices, the matrix units: 4096 x 9216
+// takes 5.5 ms, of which 775 us a product with X (1197 TFLOP/s in fp16,
+// where the library's largest fp16 products reach 1340 to 1390), 427 a
+// Gram matrix (1090), 199 one of A and M (1035).  Matrices up to some 2^20
+// elements: the 15 to 20 launches, which need one another's results.  One
+// takes 7 to 8 us: 1.3 of launch, 1.1 until a block knows its tile, 1.1
+// for the first slice, 0.43 a further one of 64, 0.9 to store the sums.
 
 #include <atomic>
 
@@ -528,7 +536,8 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
   if constexpr (PING) {
     // Two groups of four waves, one of each on every SIMD, half a beat
     // apart: while one reads its fragments (and asks for the next
-    // slice), the other multiplies.  Beats of a group: fragments of B
+    // slice), the other multiplies.  (X of 4096 x 9216: 775 us; with tiles
+    // of 128 and two blocks a unit 830.)  Beats of a group: fragments of B
     // and of the upper half of A; their products; the lower half of A;
     // their products.
     const bool late = wave >= 4;
@@ -713,8 +722,10 @@ __global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
 // `groups` blocks a matrix have a range of X's columns each.  Every block
 // adds up A from all blocks' shares and does the m x m work itself, which
 // costs less than a launch; then it multiplies its columns and leaves its
-// share of the next A.  At 64 x 576 five launches of 97 us become six
-// kernels: see the table of measurements.
+// share of the next A.  64 x 576, 5 steps: 44 us in 6 kernels (102 in 17 of
+// the general ones); they wait, in turn, for a launch, the shares, six
+// products that need one another, the columns: 7 to 10 us each, two thirds
+// of it in that chain.
 
 constexpr int FEW = 64;
 constexpr int SLICE = FEW * 64;               // halves of 32 columns
@@ -1027,25 +1038,30 @@ hipError_t launch_ns_few(NsArgs* a, hipStream_t stream) {
 // One product, for every matrix: mode 0 S[to] = X X^T, 1 S[to] = S[s1]
 // S[s2] (with poly: aI + b S[s1] + c S[s1] S[s1]), 2 X <- S[s1] X.
 hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
+  // A and M fill the device with tiles of 128 alone
   const int bt = a->tile == 256 && mode != APPLY ? 128 : a->tile;
-  const int deep = bt == 64 ? 64 : 32;
   const int slots = bt == 256 ? 256 : NS_SLOTS;   // blocks that run at once
-  const int least = 384 / deep;        // shortest run of k worth a join
   long tiles = 0, rest = 0, runs = 0, joins = 0;
   long n[NS_MAXP], s[NS_MAXP];
   for (int i = 0; i < a->count; ++i) {
     const NsProb& p = a->p[i];
     const long t = p.mp / bt;
     n[i] = p.batch * (mode == APPLY ? t * (p.np / bt) : t * (t + 1) / 2);
-    s[i] = (mode == GRAM ? p.np : p.mp) / deep;
     a->tile0[i] = (int)tiles;
     tiles += n[i];
   }
   if (tiles >= (1L << 30)) return hipErrorInvalidValue;
   a->tile0[a->count] = (int)tiles;
+  const int deep = bt == 64 && tiles <= NS_SLOTS ? 64 : 32;
+  const int least = 384 / deep;        // shortest run
+  for (int i = 0; i < a->count; ++i)
+    s[i] = (mode == GRAM ? a->p[i].np : a->p[i].mp) / deep;
   a->whole = (int)(tiles / slots * slots);
-  // the rest: cut k so that it, too, gives every slot a run, in runs of
-  // `least` slices or more
+  // The rest: cut k so that it, too, gives every slot a run of 384 or
+  // more, unless the longest run is then less than 768 shorter: a join is
+  // a launch of 6 us (us, with the cut and without: 768 x 768 217, 191;
+  // 1000 x 1000 270, 223; but 256 x 2304, 1700 shorter, 153, 206; shortest
+  // run of 192: 128 x 65536 427, of 384 330).
   rest = tiles - a->whole;
   for (int i = 0; i < a->count; ++i) {
     long skip = a->whole - a->tile0[i];
@@ -1053,7 +1069,7 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
     a->skip[i] = (int)skip;
     long parts = rest ? slots / rest : 1;
     if (parts > s[i] / least) parts = s[i] / least;
-    if (parts < 2) parts = 1;
+    if (parts < 2 || s[i] * (parts - 1) / parts * deep < 768) parts = 1;
     a->parts[i] = (int)parts;
     a->start[i] = (int)runs;
     runs += (n[i] - skip) * parts;
@@ -1085,8 +1101,16 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
     else if (mode == SQUARE) NS_GEMM(SQUARE, __VA_ARGS__); \
     else NS_GEMM(APPLY, __VA_ARGS__);                  \
   } while (0)
-  if (bt == 256) NS_MODES(256, 2, 4, 2, 1);
+  // Tiles of 64 wait for memory more than they multiply.  One block a
+  // compute unit, or none: four slices of 64 in LDS (us, instead of two:
+  // 256 x 256 124 -> 118, 512 x 512 168 -> 155; with more blocks the units
+  // would hold one where they could hold two: 1000 x 1000 268 -> 319).
+  // Two a unit: two of 64.  More: three of 32, so that three share a unit
+  // (512 x 4608 226 -> 209, a wide residual network's weights 206 -> 193,
+  // though 1000 x 4096 370 -> 382).
+  if (bt == 256) NS_GEMM(APPLY, 256, 2, 4, 2, 1);
   else if (bt == 128) NS_MODES(128, 2, 2, 2, 1);
+  else if (deep == 32) NS_MODES(64, 2, 2, 3, 1);
   else if (blocks <= 256) NS_MODES(64, 2, 2, 4, 2);
   else NS_MODES(64, 2, 2, 2, 2);
 #undef NS_MODES

@@ -496,6 +496,22 @@ def test_label_logprobs_gpu_most_classes():
             OF.label_logprobs(x, labels)
 
 
+@gpu
+def test_label_logprobs_gpu_more_rows_than_a_launch():
+    rows, tail = 2 ** 23 + 9, 100
+    x = torch.randn(rows, 10, device=dev()).bfloat16()
+    labels = torch.arange(rows, device=dev()) % 10
+    whole = x.requires_grad_(True)
+    part = x.detach()[-tail:].clone().requires_grad_(True)
+    got = OF.label_logprobs(whole, labels, top=2)
+    want = OF.label_logprobs(part, labels[-tail:], top=2)
+    for a, b in zip(got, want):
+        assert torch.equal(a[-tail:], b)
+    (dx,) = torch.autograd.grad(got[0].sum() + got[2].sum(), whole)
+    (dw,) = torch.autograd.grad(want[0].sum() + want[2].sum(), part)
+    assert torch.equal(dx[-tail:], dw)
+
+
 def test_label_logprobs_refusals():
     x, labels = lp_inputs(4, 9, torch.float32, "cpu")
     with pytest.raises(TypeError):

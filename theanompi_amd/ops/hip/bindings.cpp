@@ -1287,7 +1287,6 @@ static std::vector<torch::Tensor> lp_fwd(torch::Tensor x,
     int lanes, nv;
     const long segs = lp_plan(rows, n, kind, &lanes, &nv);
     TORCH_CHECK(segs > 0, "n_classes ", n, " is over what a row may have");
-    TORCH_CHECK(rows * segs < (1L << 31), "too many rows");
     torch::Tensor parts;           // keys, then sums, of every segment
     if (segs > 1)
       parts = torch::empty({rows * segs * (k + 2)}, i64);
@@ -1297,7 +1296,8 @@ static std::vector<torch::Tensor> lp_fwd(torch::Tensor x,
         x.data_ptr(), labels.data_ptr<long>(), logp.data_ptr<float>(),
         entropy.data_ptr<float>(), top_logp.data_ptr<float>(),
         top_idx.data_ptr<long>(), stat.data_ptr<float>(),
-        psum, pkey, rows, (int)n, ld, (int)segs, lanes, nv, (int)k, kind, cur_stream()));
+        psum, pkey, rows, (int)n, ld, (int)segs, lanes, nv, (int)k, kind,
+        cur_stream()));
   }
   return {logp, entropy, top_logp, top_idx, stat};
 }

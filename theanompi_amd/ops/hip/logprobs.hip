@@ -25,7 +25,6 @@ namespace {
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
 
-constexpr int KMAX = 32;       // alternatives
 constexpr int MAXSEG = 256;    // segments a row
 
 constexpr int CAP = 256;       // candidates a block may collect
@@ -574,25 +573,30 @@ hipError_t fwd(const FwdArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+struct BwdArgs {
+  const void* x;
+  const long *labels, *top_idx;
+  const float *stat, *dlogp, *dentropy, *dtop;
+  void* dx;
+  long rows;
+  int n, C;
+  long ldx;
+  int segs, k, nv;
+};
+
+template <typename T, int NV>
+void bwd_one(const BwdArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((lp_bwd_k<T, NV>), dim3((unsigned)(a.rows * a.segs)),
+                     dim3(256), 0, stream, (const T*)a.x, a.labels,
+                     a.top_idx, (const RowStat*)a.stat, a.dlogp, a.dentropy,
+                     a.dtop, (T*)a.dx, a.n, a.C, a.ldx, a.segs, a.k);
+}
+
 template <typename T>
-hipError_t bwd(const void* x, const long* labels, const long* top_idx,
-               const float* stat, const float* dlogp,
-               const float* dentropy, const float* dtop, void* dx,
-               long rows, int n, int C, long ldx, int k,
-               hipStream_t stream) {
-  constexpr int N = 16 / sizeof(T);
-#define LP_BWD(NV)                                                        \
-  do {                                                                    \
-    const int per = 256 * NV * N, segs = (C + per - 1) / per;             \
-    hipLaunchKernelGGL((lp_bwd_k<T, NV>), dim3((unsigned)(rows * segs)),  \
-                       dim3(256), 0, stream, (const T*)x, labels,         \
-                       top_idx, (const RowStat*)stat, dlogp, dentropy,    \
-                       dtop, (T*)dx, n, C, ldx, segs, k);                 \
-  } while (0)
-  if (C <= 256 * N) LP_BWD(1);
-  else if (C <= 512 * N) LP_BWD(2);
-  else LP_BWD(4);
-#undef LP_BWD
+hipError_t bwd(const BwdArgs& a, hipStream_t stream) {
+  if (a.nv == 1) bwd_one<T, 1>(a, stream);
+  else if (a.nv == 2) bwd_one<T, 2>(a, stream);
+  else bwd_one<T, 4>(a, stream);
   return hipGetLastError();
 }
 
@@ -621,6 +625,10 @@ int lp_plan(long rows, long n, int kind, int* lanes, int* nv) {
   return segs <= MAXSEG ? (int)segs : 0;
 }
 
+// A launch's threads are counted in 32 bits: 2^24 blocks of 256 are too
+// many, and rows go in launches of fewer.
+static const long BLOCKS = 1L << 23;
+
 // kind: 0 f32, 1 f16, 2 bf16
 hipError_t launch_lp_fwd(const void* x, const long* labels, float* logp,
                          float* entropy, float* top_logp, long* top_idx,
@@ -628,11 +636,24 @@ hipError_t launch_lp_fwd(const void* x, const long* labels, float* logp,
                          unsigned long long* pkey, long rows, int n,
                          long ldx, int segs, int lanes, int nv, int k,
                          int kind, hipStream_t stream) {
-  const FwdArgs a = {x, labels, logp, entropy, top_logp, top_idx, stat,
-                     psum, pkey, rows, n, ldx, segs, k, lanes, nv};
-  if (kind == 0) return fwd<float>(a, stream);
-  if (kind == 1) return fwd<_Float16>(a, stream);
-  return fwd<__bf16>(a, stream);
+  const long most = BLOCKS / segs;
+  for (long r = 0; r < rows; r += most) {
+    const FwdArgs a = {(const char*)x + r * ldx * (kind ? 2 : 4),
+                       labels + r,
+                       logp + r,
+                       entropy + r,
+                       top_logp + r * k,
+                       top_idx + r * k,
+                       stat + r * 3,
+                       psum ? psum + r * segs * 3 : nullptr,
+                       pkey ? pkey + r * segs * k : nullptr,
+                       rows - r < most ? rows - r : most,
+                       n, ldx, segs, k, lanes, nv};
+    HIP_KERNEL_ASSERT_OK(kind == 0   ? fwd<float>(a, stream)
+                         : kind == 1 ? fwd<_Float16>(a, stream)
+                                     : fwd<__bf16>(a, stream));
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_lp_bwd(const void* x, const long* labels,
@@ -641,14 +662,26 @@ hipError_t launch_lp_bwd(const void* x, const long* labels,
                          const float* dtop, void* dx, long rows, int n,
                          int C, long ldx, int k, int kind,
                          hipStream_t stream) {
-  if (kind == 0)
-    return bwd<float>(x, labels, top_idx, stat, dlogp, dentropy, dtop, dx,
-                      rows, n, C, ldx, k, stream);
-  if (kind == 1)
-    return bwd<_Float16>(x, labels, top_idx, stat, dlogp, dentropy, dtop,
-                         dx, rows, n, C, ldx, k, stream);
-  return bwd<__bf16>(x, labels, top_idx, stat, dlogp, dentropy, dtop, dx,
-                     rows, n, C, ldx, k, stream);
+  const long size = kind ? 2 : 4, vectors = (C * size + 15) / 16;
+  const int nv = vectors <= 256 ? 1 : vectors <= 512 ? 2 : 4;
+  const int segs = (int)((vectors + 256 * nv - 1) / (256 * nv));
+  const long most = BLOCKS / segs;
+  for (long r = 0; r < rows; r += most) {
+    const BwdArgs a = {(const char*)x + r * ldx * size,
+                       labels + r,
+                       top_idx + r * k,
+                       stat + r * 3,
+                       dlogp ? dlogp + r : nullptr,
+                       dentropy ? dentropy + r : nullptr,
+                       dtop ? dtop + r * k : nullptr,
+                       (char*)dx + r * C * size,
+                       rows - r < most ? rows - r : most,
+                       n, C, ldx, segs, k, nv};
+    HIP_KERNEL_ASSERT_OK(kind == 0   ? bwd<float>(a, stream)
+                         : kind == 1 ? bwd<_Float16>(a, stream)
+                                     : bwd<__bf16>(a, stream));
+  }
+  return hipSuccess;
 }
 
 }  // extern "C"

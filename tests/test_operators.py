@@ -352,7 +352,8 @@ LP_SHAPES = [(1, 1, None, 1), (3, 2, None, 2), (9, 10, None, 5),
              (128, 1008, 1000, 5), (5, 511, None, 32), (6, 513, 512, 7),
              (4, 1025, None, 3), (3, 2049, 2040, 20), (2, 9001, None, 8),
              (70, 20000, 19999, 4), (1, 131073, None, 32),
-             (2, 300007, 300001, 9), (3, 8192, None, 0)]
+             (2, 300007, 300001, 9), (3, 8192, None, 0),
+             (600, 17003, 16999, 4)]
 
 
 @gpu

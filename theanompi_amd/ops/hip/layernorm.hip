@@ -15,6 +15,12 @@
 // against the spread.  Only the first n of C channels count: what is
 // behind them (the physical channel padding) is left out of the
 // statistics, and its outputs are zeros.
+//
+// Measured: 802816 x 256 bf16 forward 142 us, 5.8 TB/s, backward 233 + 5
+// us, 5.3 TB/s (a copy of 411 MB here 5.3).  4099 x 1000 f32 forward 11,
+// backward 17 + 5 us; 128 x 4096 bf16 4 + 4.5, 32 x 1024 f16 3.1: a launch,
+// one trip to memory and the sums over a row.  A training call of few rows
+// takes the host 70 us, 46 of them any operator's trip through autograd.
 
 #include "common.hpp"
 

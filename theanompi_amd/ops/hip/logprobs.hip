@@ -11,7 +11,13 @@
 // them and writes their gradient.  A block holds its part of a row (a
 // segment) in registers, takes maximum and sums from there and writes
 // one partial result; rows of more than one segment are joined by a
-// second kernel, in a fixed order.
+// second kernel, in a fixed order.  2048 x 131072 bf16, top 8: forward
+// 114 + 6 us (4.7 TB/s; the vector units are at work for half of it, most
+// of that in one exp2 an element at a quarter of the rate), backward 166
+// (6.5 TB/s; a copy reaches 4.9 to 6.1 here).  Few rows wait for a chain
+// instead: 128 x 1000 5 + 5 us and 1 x 131072 fp32 6 + 4, of which a launch
+// is 1.3 each, and a training call's time is the host's: 70 us, 46 of them
+// any operator's trip through autograd.
 //
 // A class at -inf is masked: probability 0, nothing to the entropy, and
 // p_j = 0 in its gradient.  A row of nothing else has logp -inf, entropy 0
@@ -595,8 +601,7 @@ void bwd_one(const BwdArgs& a, hipStream_t stream) {
 template <typename T>
 hipError_t bwd(const BwdArgs& a, hipStream_t stream) {
   if (a.nv == 1) bwd_one<T, 1>(a, stream);
-  else if (a.nv == 2) bwd_one<T, 2>(a, stream);
-  else bwd_one<T, 4>(a, stream);
+  else bwd_one<T, 2>(a, stream);
   return hipGetLastError();
 }
 
@@ -606,6 +611,11 @@ extern "C" {
 
 // How a row of n classes is cut: lanes a block, vectors a lane, segments
 // a row.  Returns segments, or 0 where n is over what they can hold.
+// Measured (us, forward): a wave a row instead of a block 16384 x 1000 bf16
+// 20, 35; vectors a lane from 1, 2, 4 to 8: 2048 x 131072 bf16 246, 161,
+// 119, 114; 64 x 131072 fp32 28, 19, 15, 14; 512 x 10000 fp32 21, 15, 14,
+// 14; few blocks, where more run at once: 8 x 200000 bf16 17, 14, 14, 25;
+// a last segment nearly empty at 8: 4096 x 50000 bf16 185, 126, 103, 115.
 int lp_plan(long rows, long n, int kind, int* lanes, int* nv) {
   const long N = kind == 0 ? 4 : 8;
   const long v = (n + N - 1) / N;          // vectors a row
@@ -616,12 +626,17 @@ int lp_plan(long rows, long n, int kind, int* lanes, int* nv) {
   }
   *lanes = 256;
   *nv = 1;
-  while (*nv < 8 && v > 256L * *nv) {
-    const long segs = (v + 256L * *nv - 1) / (256L * *nv);
-    if (rows * segs <= 1024 && segs <= 64) break;
+  auto cut = [&] { return (v + 256L * *nv - 1) / (256L * *nv); };
+  while (*nv < 8 && v > 256L * *nv && (rows * cut() > 1024 || cut() > 64))
     *nv *= 2;
+  // a last segment that is mostly empty costs as much as a full one
+  if (*nv == 8) {
+    const long eight = cut() * 8;
+    *nv = 4;
+    const long four = cut() * 4;
+    if (eight * 10 <= four * 11 || cut() > MAXSEG) *nv = 8;
   }
-  const long segs = (v + 256L * *nv - 1) / (256L * *nv);
+  const long segs = cut();
   return segs <= MAXSEG ? (int)segs : 0;
 }
 
@@ -663,7 +678,9 @@ hipError_t launch_lp_bwd(const void* x, const long* labels,
                          int C, long ldx, int k, int kind,
                          hipStream_t stream) {
   const long size = kind ? 2 : 4, vectors = (C * size + 15) / 16;
-  const int nv = vectors <= 256 ? 1 : vectors <= 512 ? 2 : 4;
+  // more vectors a lane than two find no more to overlap (2048 x 131072
+  // bf16, the whole backward: 207 us with one, 176 with two, 191 with four)
+  const int nv = vectors <= 256 ? 1 : 2;
   const int segs = (int)((vectors + 256 * nv - 1) / (256 * nv));
   const long most = BLOCKS / segs;
   for (long r = 0; r < rows; r += most) {

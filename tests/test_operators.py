@@ -622,13 +622,15 @@ def ns_recurrence(x, steps=5):
     return x
 
 
-# One shape for each way through the general kernels: k cut into runs and
-# not, tiles of 64, 128 and 256, two steps at a time (n >= 2m) and one,
-# and the padding of m and n within a tile.
+# One shape for each way through the kernels: k cut into runs and not,
+# tiles of 64 with one, two and more blocks a compute unit, of 128 and 256,
+# two steps at a time and one, the padding of m and n within a tile; few
+# rows in many groups of columns.
 @gpu
 @pytest.mark.parametrize("shape,steps", [
     ((70, 5000), 5), ((700, 1100), 5), ((1300, 4650), 5), ((1300, 4650), 4),
-    ((2500, 2500), 5), ((2050, 8200), 5), ((4097, 4100), 3)], ids=str)
+    ((2500, 2500), 5), ((2050, 8200), 5), ((4097, 4100), 3),
+    ((33, 40003), 5), ((600, 4700), 5), ((1030, 1100), 5)], ids=str)
 def test_orthogonalize_gpu_large(shape, steps):
     x = ns_inputs(shape, torch.float32, dev())
     want = ns_recurrence(x, steps)

@@ -9,7 +9,9 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
@@ -1380,7 +1382,8 @@ static std::vector<torch::Tensor> label_logprobs(
 // Which kernels a matrix takes: 0, those for few rows; else the tile of
 // the general ones, larger where there is work enough for all compute
 // units.  Measured (us, 5 steps), few rows against tiles of 64: 64 x 576
-// 44, 102; 64 x 16384 132, 141; 100 x 64 x 64 39, 88.  Tiles of 64, 128 and
+// 36, 98; 64 x 16384 84, 135; 16 x 1000000 723, 736; 100 x 64 x 64 33, 82;
+// 20 x 48 x 20000 307, 293.  Tiles of 64, 128 and
 // 256: 1536 x 1536 440, 491, 523; 1536 x 4096 739, 674, 729; 32 x 512 x 512
 // 516, 512, 549; 3000 x 3000 2116, 1900, 1945; 4096 x 4096 5290, 3562,
 // 3461; 4096 x 9216 10644, 5717, 5547.
@@ -1420,11 +1423,16 @@ static torch::Tensor ns_workspace(NsArgs& a,
       for (int k = 0; k < 3; ++k)
         at.push_back(take(4L * p.batch * p.mp * p.mp));
     } else {
-      // about as many blocks as compute units, and no more than 16 a
-      // matrix, whose shares each of them adds up
+      // Blocks a matrix: as many as compute units in all, but each adds up
+      // the shares of all of its matrix (0.09 us one), and those of a long
+      // one do better with fewer, which have more columns each (1.3 us).
+      // Measured (us) with 8, 16, 32, 64 and 128: 64 x 1536 51, 48, 44, 44,
+      // 44; 64 x 8192 123, 83, 68, 71, 90; 64 x 16384 212, 128, 92, 84, 99;
+      // 64 x 100000 1271, 665, 367, 229, 179.
       const long cols = p.np / 64;
-      long groups = blocks <= 256 ? cols : (cols * 256 + blocks - 1) / blocks;
-      p.groups = (int)(groups < 16 ? groups : 16);
+      const long groups = blocks <= 256 ? cols : (cols * 256 + blocks - 1) / blocks;
+      const long most = std::max(24L, (long)(4.0 * std::sqrt((double)cols)));
+      p.groups = (int)std::min(groups, most);
       for (int k = 0; k < 3; ++k)
         at.push_back(take(k < 2 ? 4L * p.batch * p.groups * 64 * 64 : 0));
     }
@@ -1459,10 +1467,13 @@ static void ns_run(NsArgs& a, long steps,
   a.steps = (int)steps;
   CHECK_HIP(launch_ns_sum(&a, stream));
   if (a.phase == 1) return;
+  a.shared = !a.tile;
+  for (int i = 0; i < a.count; ++i)
+    a.shared = a.shared && a.p[i].groups == a.p[i].np / 64;
   CHECK_HIP(launch_ns_load(&a, stream));
   if (!a.tile) {
     a.pair = -1;
-    CHECK_HIP(launch_ns_few(&a, stream));
+    if (!a.shared) CHECK_HIP(launch_ns_few(&a, stream));
     for (int left = (int)steps; left > 0; ++a.step) {
       a.pair = left >= 2;
       left -= 1 + a.pair;

@@ -161,68 +161,6 @@ __global__ __launch_bounds__(256) void ns_sum_k(const NsArgs a) {
   if (threadIdx.x == 0) p.part[mat * p.parts + part] = s;
 }
 
-// X / (|X| + 1e-7) as a split matrix, a 64 x 64 tile a block, turned if
-// the matrix is tall
-__global__ __launch_bounds__(256) void ns_load_k(const NsArgs a) {
-  __shared__ float tile[64][65];
-  __shared__ double red[4];
-  const int i = find(a, blockIdx.x);
-  const NsProb& p = a.p[i];
-  const int tiles = (p.mp / 64) * (p.np / 64);
-  int b = blockIdx.x - a.start[i];
-  const long mat = b / tiles;
-  b %= tiles;
-  const int r0 = b / (p.np / 64) * 64, c0 = b % (p.np / 64) * 64;
-  // rows and columns as stored
-  const int sr0 = p.tall ? c0 : r0, sc0 = p.tall ? r0 : c0;
-  const int rows = p.tall ? p.n : p.m, cols = p.tall ? p.m : p.n;
-  const long base = mat * rows * (long)cols;
-  float f[16];
-  typed(p, [&](const auto* x) {
-    const int r = sr0 + (threadIdx.x >> 6), c = sc0 + (threadIdx.x & 63);
-    x += base + (long)r * cols + c;
-#pragma unroll
-    for (int t = 0; t < 16; ++t)
-      f[t] = r + t * 4 < rows && c < cols ? (float)x[t * 4L * cols] : 0.f;
-  });
-  double sum = 0.0;
-  for (int k = threadIdx.x; k < p.parts; k += 256)
-    sum += p.part[mat * p.parts + k];
-  sum = block_sum(sum, red);
-  // A norm far below 1e-7 leaves X far below 1, and fp16 would lose it:
-  // it is kept 2^e times as large, e so that `steps` growths by QA end
-  // below 1 all the same.
-  const double norm = sqrt(sum), inv0 = 1.0 / (norm + 1e-7);
-  int e = 0;
-  if (norm * inv0 < 0.5 && norm > 0.0)
-    e = -ilogb(norm * inv0) - 1 - (int)(1.785 * a.steps + 1.0);
-  if (e < 0) e = 0;
-  const double inv = ldexp((double)SCALE * inv0, e);
-  if (b == 0 && threadIdx.x == 0) p.shift[mat] = (float)ldexp(1.0, -e);
-#pragma unroll
-  for (int t = 0; t < 16; ++t)
-    tile[t * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] =
-        (float)(f[t] * inv);
-  __syncthreads();
-  _Float16* X = (_Float16*)p.X[0] + mat * 2 * p.mp * (long)p.np;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    // 8 columns a thread: 16 bytes of hi, 16 of lo
-    const int r = t * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
-    half8 hi, lo;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      _Float16 h, l;
-      split(p.tall ? tile[c + j][r] : tile[r][c + j], h, l);
-      hi[j] = h;
-      lo[j] = l;
-    }
-    _Float16* d = X + ((long)(r0 + r) * p.np + c0) * 2 + c / 32 * 64 + c % 32;
-    *(half8*)d = hi;
-    *(half8*)(d + 32) = lo;
-  }
-}
-
 enum { GRAM, SQUARE, APPLY };
 
 template <int V> struct Int { static constexpr int value = V; };
@@ -737,10 +675,12 @@ __global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
 // `groups` blocks a matrix have a range of X's columns each.  Every block
 // adds up A from all blocks' shares and does the m x m work itself, which
 // costs less than a launch; then it multiplies its columns and leaves its
-// share of the next A.  64 x 576, 5 steps: 44 us in 6 kernels (102 in 17 of
-// the general ones); they wait, in turn, for a launch, the shares, six
-// products that need one another, the columns: 7 to 10 us each, two thirds
-// of it in that chain.
+// share of the next A.  64 x 576, 5 steps: 36 us in 5 kernels (98 in 17 of
+// the general ones), 4 for the squares, 6 to load and for the first
+// shares, 10 for two steps, 6.6 for one.  They wait, in turn, for a launch,
+// the shares, up to six products that need one another, the columns.
+// (Asking for the columns before the products gained nothing here, and
+// lost where a block has many: 64 x 16384 128 -> 139 us.)
 
 constexpr int FEW = 64;
 constexpr int SLICE = FEW * 64;               // halves of 32 columns
@@ -994,6 +934,89 @@ __global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
   }
 }
 
+// X / (|X| + 1e-7) as a split matrix, a 64 x 64 tile a block, turned if
+// the matrix is tall.  SHARE: few rows in as many groups as tiles, whose
+// shares of X X^T are taken at once (64 x 576: 39.3 -> 36.5 us in all).
+template <bool SHARE>
+__global__ __launch_bounds__(256) void ns_load_k(const NsArgs a) {
+  __shared__ float tile[64][65];
+  __shared__ double red[4];
+  __shared__ __align__(16) _Float16 T[SHARE ? 2 * SLICE : 8];
+  const int i = find(a, blockIdx.x);
+  const NsProb& p = a.p[i];
+  const int tiles = (p.mp / 64) * (p.np / 64);
+  int b = blockIdx.x - a.start[i];
+  const long mat = b / tiles;
+  b %= tiles;
+  const int r0 = b / (p.np / 64) * 64, c0 = b % (p.np / 64) * 64;
+  // rows and columns as stored
+  const int sr0 = p.tall ? c0 : r0, sc0 = p.tall ? r0 : c0;
+  const int rows = p.tall ? p.n : p.m, cols = p.tall ? p.m : p.n;
+  const long base = mat * rows * (long)cols;
+  float f[16];
+  typed(p, [&](const auto* x) {
+    const int r = sr0 + (threadIdx.x >> 6), c = sc0 + (threadIdx.x & 63);
+    x += base + (long)r * cols + c;
+#pragma unroll
+    for (int t = 0; t < 16; ++t)
+      f[t] = r + t * 4 < rows && c < cols ? (float)x[t * 4L * cols] : 0.f;
+  });
+  double sum = 0.0;
+  for (int k = threadIdx.x; k < p.parts; k += 256)
+    sum += p.part[mat * p.parts + k];
+  sum = block_sum(sum, red);
+  // A norm far below 1e-7 leaves X far below 1, and fp16 would lose it:
+  // it is kept 2^e times as large, e so that `steps` growths by QA end
+  // below 1 all the same.
+  const double norm = sqrt(sum), inv0 = 1.0 / (norm + 1e-7);
+  int e = 0;
+  if (norm * inv0 < 0.5 && norm > 0.0)
+    e = -ilogb(norm * inv0) - 1 - (int)(1.785 * a.steps + 1.0);
+  if (e < 0) e = 0;
+  const double inv = ldexp((double)SCALE * inv0, e);
+  if (b == 0 && threadIdx.x == 0) p.shift[mat] = (float)ldexp(1.0, -e);
+#pragma unroll
+  for (int t = 0; t < 16; ++t)
+    tile[t * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] =
+        (float)(f[t] * inv);
+  __syncthreads();
+  _Float16* X = (_Float16*)p.X[0] + mat * 2 * p.mp * (long)p.np;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    // 8 columns a thread: 16 bytes of hi, 16 of lo
+    const int r = t * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
+    half8 hi, lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      _Float16 h, l;
+      split(p.tall ? tile[c + j][r] : tile[r][c + j], h, l);
+      hi[j] = h;
+      lo[j] = l;
+    }
+    _Float16* d = X + ((long)(r0 + r) * p.np + c0) * 2 + c / 32 * 64 + c % 32;
+    *(half8*)d = hi;
+    *(half8*)(d + 32) = lo;
+    if constexpr (SHARE) {
+      _Float16* at = T + c / 32 * SLICE + r * 64;
+      const int q = c % 32 / 8;
+      *(half8*)(at + (q ^ (r & 7)) * 8) = hi;
+      *(half8*)(at + ((q + 4) ^ (r & 7)) * 8) = lo;
+    }
+  }
+  if constexpr (SHARE) {
+    __syncthreads();
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    f32x4 acc[2][2];
+    few_product(T, T, (wave >> 1) * 32, (wave & 1) * 32, acc);
+    f32x4* to = (f32x4*)p.share[0] + (mat * p.groups + b) * (FEW * FEW / 4)
+                + wave * 256 + lane;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) to[(u * 2 + v) * 64] = acc[u][v];
+  }
+}
+
 // A kernel's dynamic LDS beyond the usual limit, once a device.
 hipError_t allow_lds(const void* kernel, int bytes,
                      std::atomic<unsigned long>& allowed) {
@@ -1030,7 +1053,10 @@ hipError_t launch_ns_load(NsArgs* a, hipStream_t stream) {
     at += a->p[i].batch * (a->p[i].mp / 64) * (a->p[i].np / 64);
   }
   a->start[a->count] = at;
-  hipLaunchKernelGGL(ns_load_k, dim3(at), dim3(256), 0, stream, *a);
+  if (a->shared)
+    hipLaunchKernelGGL(ns_load_k<true>, dim3(at), dim3(256), 0, stream, *a);
+  else
+    hipLaunchKernelGGL(ns_load_k<false>, dim3(at), dim3(256), 0, stream, *a);
   return hipGetLastError();
 }
 

@@ -35,6 +35,7 @@ struct NsArgs {
   // edge of an output tile, to which m and n are padded; 0: few rows
   int tile;
   int pair;                // few rows: two steps (1), one (0), first (-1)
+  int shared;              // few rows: loading them takes the first shares
   int s1, s2, to, poly;    // a product: which S, and whether aI + bS is added
   int count, steps, step, last, phase, whole;
   float mu;

@@ -13,8 +13,8 @@
 // one partial result; rows of more than one segment are joined by a
 // second kernel, in a fixed order.  2048 x 131072 bf16, top 8: forward
 // 114 + 6 us (4.7 TB/s; the vector units are at work for half of it, most
-// of that in one exp2 an element at a quarter of the rate), backward 166
-// (6.5 TB/s; a copy reaches 4.9 to 6.1 here).  Few rows wait for a chain
+// of that in one exp2 an element at a quarter of the rate), backward 170
+// (6.3 TB/s; a copy reaches 4.9 to 6.1 here).  Few rows wait for a chain
 // instead: 128 x 1000 5 + 5 us and 1 x 131072 fp32 6 + 4, of which a launch
 // is 1.3 each, and a training call's time is the host's: 70 us, 46 of them
 // any operator's trip through autograd.
@@ -679,7 +679,7 @@ hipError_t launch_lp_bwd(const void* x, const long* labels,
                          hipStream_t stream) {
   const long size = kind ? 2 : 4, vectors = (C * size + 15) / 16;
   // more vectors a lane than two find no more to overlap (2048 x 131072
-  // bf16, the whole backward: 207 us with one, 176 with two, 191 with four)
+  // bf16: 206 us with one, 175 with two, 188 with four)
   const int nv = vectors <= 256 ? 1 : 2;
   const int segs = (int)((vectors + 256 * nv - 1) / (256 * nv));
   const long most = BLOCKS / segs;

@@ -1092,3 +1092,138 @@ def test_operators_on_another_stream():
     side.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# offsets that 32 bits do not hold: the last rows against a call on these
+# ---------------------------------------------------------------------------
+
+@gpu
+def test_layernorm_gpu_long_offsets():
+    rows, c, tail = 270000, 8192, 40
+    x = torch.empty(rows, c, dtype=torch.bfloat16, device=dev()).normal_()
+    dy = torch.empty_like(x).normal_()
+    _, gamma, beta, _ = ln_inputs((1, c), torch.float32, dev())
+    leaf, end = x.requires_grad_(True), x.detach()[-tail:].clone()
+    y = OF.layernorm(leaf, gamma, beta)
+    (dx,) = torch.autograd.grad(y, leaf, dy)
+    end.requires_grad_(True)
+    ye = OF.layernorm(end, gamma, beta)
+    (de,) = torch.autograd.grad(ye, end, dy[-tail:])
+    assert torch.equal(y[-tail:], ye) and torch.equal(dx[-tail:], de)
+
+
+@gpu
+def test_label_logprobs_gpu_long_offsets():
+    rows, c, tail = 17000, 131072, 40
+    x = torch.empty(rows, c, dtype=torch.float16, device=dev()).normal_()
+    labels = torch.arange(rows, device=dev()) * 7
+    # the last rows again, among as many rows, which are cut alike
+    again = x.roll(tail, 0)
+    out = []
+    for leaf, lab in ((x, labels), (again, labels.roll(tail, 0))):
+        leaf.requires_grad_(True)
+        got = OF.label_logprobs(leaf, lab, top=3)
+        (dx,) = torch.autograd.grad(got[0].sum() + got[1].sum()
+                                    + got[2].sum(), leaf)
+        rows_of = slice(-tail, None) if leaf is x else slice(0, tail)
+        out.append([t[rows_of].clone() for t in (*got, dx)])
+        del got, dx
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(3000, 900, 800), (36000, 60, 1000)],
+                         ids=str)
+def test_orthogonalize_gpu_long_offsets_of_a_batch(shape):
+    x = torch.empty(shape, dtype=torch.bfloat16, device=dev()).normal_()
+    y = OF.orthogonalize(x)
+    for i in (0, shape[0] // 2, shape[0] - 1):
+        assert off(y[i], ns_formula(x[i])) < NS_TOL + half(x.dtype)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(11000000, 200), (200, 11000000),
+                                   (64, 16777215)], ids=str)
+def test_orthogonalize_gpu_long_offsets_of_a_matrix(shape):
+    x = torch.empty(shape, device=dev()).normal_()
+    y = OF.orthogonalize(x)
+    wide = x if shape[0] < shape[1] else x.t()
+    m, n = wide.shape
+    # X is a polynomial of its Gram matrix times itself: columns suffice
+    gram = torch.zeros(m, m, dtype=torch.float64, device=dev())
+    for part in wide.split(1 << 20, dim=1):
+        p = part.double()
+        gram += p @ p.t().contiguous()
+    norm = gram.trace().sqrt() + 1e-7
+    s, u = torch.linalg.eigh(gram.cpu() / norm.cpu() ** 2)
+    s = s.clamp_min(0).sqrt()
+    a, b, c = OF.NS_QUINTIC
+    f = torch.ones_like(s)
+    for _ in range(5):
+        q = (s * f) ** 2
+        f = f * (a + b * q + c * q * q)
+    poly = (u * f) @ u.t()
+    got = y if shape[0] < shape[1] else y.t()
+    for c0 in (0, n // 2, n - 500):
+        want = poly @ (wide[:, c0:c0 + 500].double() / norm).cpu()
+        assert off(got[:, c0:c0 + 500], want) < NS_TOL
+
+
+@gpu
+def test_two_graphs_of_all_kinds_replay_in_turn():
+    """Every way through the kernels, in two captured graphs that live and
+    replay beside each other and beside eager calls."""
+    mats = [ns_inputs(s, torch.float32, dev()) for s in
+            ((64, 576), (40, 4000), (5, 70, 90), (600, 4700), (1300, 4650),
+             (2500, 2500), (2050, 8200))]
+    logits = [lp_inputs(r, c, torch.bfloat16, dev())
+              for r, c in ((3, 300007), (700, 1000))]
+    norms = [ln_inputs(s, torch.bfloat16, dev())
+             for s in ((40, 8192), (3000, 512), (600, 12000))]
+
+    def first():
+        out = [OF.orthogonalize(m) for m in mats[::2]]
+        for x, lab in logits:
+            leaf = x.detach().requires_grad_(True)
+            got = OF.label_logprobs(leaf, lab, top=9)
+            out += [*got, *torch.autograd.grad(got[:3], leaf, [
+                torch.ones_like(t) for t in got[:3]])]
+        return [t.detach() for t in out]
+
+    def second():
+        out = [OF.orthogonalize(m) for m in mats[1::2]]
+        for x, gamma, beta, dy in norms:
+            leaves = [t.detach().requires_grad_(True)
+                      for t in (x, gamma, beta)]
+            y = OF.layernorm(*leaves)
+            out += [y, *torch.autograd.grad(y, leaves, dy)]
+        return [t.detach() for t in out]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first(), second()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for work in (first, second):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, work()))
+    for turn in range(3):
+        for t in mats:
+            t.mul_(0.5).add_(torch.randn_like(t), alpha=1e-3)
+        for x, _ in logits:
+            x.copy_(torch.randn_like(x))
+        for x, _, _, dy in norms:
+            x.copy_(torch.randn_like(x))
+            dy.copy_(torch.randn_like(x))
+        want = [[t.clone() for t in work()] for work in (first, second)]
+        for graph, _ in graphs[::1 - 2 * (turn % 2)]:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, held), ref in zip(graphs, want):
+            for i, (a, b) in enumerate(zip(held, ref)):
+                assert torch.equal(a, b), (turn, i)

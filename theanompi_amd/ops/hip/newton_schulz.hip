@@ -53,9 +53,15 @@ typedef __attribute__((address_space(3))) fp16x4 lds_fp16x4;
 constexpr float SCALE = 4096.f;   // of every split matrix
 constexpr float QA = 3.4445f, QB = -4.775f, QC = 2.0315f;
 
-DEV int find(const NsArgs& a, int at) {
+// Whose block it is: start[i] <= at < start[i + 1].  All entries are asked
+// for at once (one after the other, a list of 17 took a join 6.7 instead of
+// 5.7 us; the products, with much else to ask for, 9.6 instead of 10.8).
+DEV int find(const int* start, int count, int at) {
   int i = 0;
-  while (i + 1 < a.count && at >= a.start[i + 1]) ++i;
+  if (count > 1) {
+#pragma unroll
+    for (int k = 1; k < NS_MAXP; ++k) i += k < count && at >= start[k];
+  }
   return i;
 }
 
@@ -120,7 +126,7 @@ DEV double block_sum(double s, double* red) {
 // that fp32 holds is too small or too large for it
 __global__ __launch_bounds__(256) void ns_sum_k(const NsArgs a) {
   __shared__ double red[4];
-  const int i = find(a, blockIdx.x);
+  const int i = find(a.start, a.count, blockIdx.x);
   const NsProb& p = a.p[i];
   const int b = blockIdx.x - a.start[i];
   const int part = b % p.parts;
@@ -634,16 +640,11 @@ __global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
   constexpr int STRIPS = WM * WN * FM;       // of a tile
   __shared__ __align__(16) float strips[4][16 * (FN * 16 + 4)];
   const int lane = threadIdx.x & 63;
-  int job = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
-  int i = 0;
-  for (; i < a.count; ++i) {
-    const int jobs = a.parts[i] > 1
-                         ? (a.start[i + 1] - a.start[i]) / a.parts[i]
-                               * STRIPS : 0;
-    if (job < jobs) break;
-    job -= jobs;
-  }
-  if (i == a.count) return;
+  int job = (int)blockIdx.x * 4
+            + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (job >= a.tile0[a.count]) return;       // tile0: the first strip of each
+  const int i = find(a.tile0, a.count, job);
+  job -= a.tile0[i];
   const NsProb& p = a.p[i];
   const int cut = job / STRIPS, wave = job % STRIPS / FM, u = job % FM;
   const Tile<MODE, BT> at(p, a.skip[i] + cut);
@@ -774,7 +775,7 @@ template <bool FIRST>
 __global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
   __shared__ __align__(16) _Float16 P[2 * SLICE], Q[2 * SLICE],
       T[2 * SLICE];
-  const int i = find(a, blockIdx.x);
+  const int i = find(a.start, a.count, blockIdx.x);
   const NsProb& p = a.p[i];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
@@ -942,7 +943,7 @@ __global__ __launch_bounds__(256) void ns_load_k(const NsArgs a) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
   __shared__ __align__(16) _Float16 T[SHARE ? 2 * SLICE : 8];
-  const int i = find(a, blockIdx.x);
+  const int i = find(a.start, a.count, blockIdx.x);
   const NsProb& p = a.p[i];
   const int tiles = (p.mp / 64) * (p.np / 64);
   int b = blockIdx.x - a.start[i];
@@ -1076,13 +1077,26 @@ hipError_t launch_ns_few(NsArgs* a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// tile0 for a join: each matrix's first strip, `per` a tile that was cut
+static int join_starts(NsArgs* a, int per) {
+  int strips = 0;
+  for (int i = 0; i < a->count; ++i) {
+    a->tile0[i] = strips;
+    if (a->parts[i] > 1)
+      strips += (a->start[i + 1] - a->start[i]) / a->parts[i] * per;
+  }
+  a->tile0[a->count] = strips;
+  return strips;
+}
+
 // One product, for every matrix: mode 0 S[to] = X X^T, 1 S[to] = S[s1]
 // S[s2] (with poly: aI + b S[s1] + c S[s1] S[s1]), 2 X <- S[s1] X.
 hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
   // A and M fill the device with tiles of 128 alone
   const int bt = a->tile == 256 && mode != APPLY ? 128 : a->tile;
   const int slots = bt == 256 ? 256 : NS_SLOTS;   // blocks that run at once
-  long tiles = 0, rest = 0, runs = 0, joins = 0;
+  long tiles = 0, rest = 0, runs = 0;
+  bool cut = false;
   long n[NS_MAXP], s[NS_MAXP];
   for (int i = 0; i < a->count; ++i) {
     const NsProb& p = a->p[i];
@@ -1114,7 +1128,7 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
     a->parts[i] = (int)parts;
     a->start[i] = (int)runs;
     runs += (n[i] - skip) * parts;
-    if (parts > 1) joins += (n[i] - skip);
+    cut = cut || (parts > 1 && n[i] > skip);
   }
   a->start[a->count] = (int)runs;
   if (runs > NS_SLOTS) return hipErrorInvalidValue;
@@ -1129,8 +1143,8 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
     hipLaunchKernelGGL((ns_gemm_k<MODE, BT, WM, WN, S, DEEP>),           \
                        dim3(blocks), dim3(64 * WM * WN), bytes, stream,  \
                        *a);                                              \
-    if (joins) {                                                         \
-      const long strips = joins * (BT / 16 * WN);                        \
+    if (cut) {                                                           \
+      const int strips = join_starts(a, BT / 16 * WN);                   \
       hipLaunchKernelGGL((ns_join_k<MODE, BT, WM, WN>),                  \
                          dim3((unsigned)((strips + 3) / 4)), dim3(256),  \
                          0, stream, *a);                                 \

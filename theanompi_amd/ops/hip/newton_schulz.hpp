@@ -29,8 +29,9 @@ struct NsArgs {
   NsProb p[NS_MAXP];
   // first block (in a product: first run) of each; the end's last
   int start[NS_MAXP + 1];
-  // a product: first output tile of each, its tiles that are one block's,
-  // and the runs that k of its others is cut into
+  // a product: first output tile of each (in its join: first strip), its
+  // tiles that are one block's, and the runs that k of its others is cut
+  // into
   int tile0[NS_MAXP + 1], skip[NS_MAXP], parts[NS_MAXP];
   // edge of an output tile, to which m and n are padded; 0: few rows
   int tile;

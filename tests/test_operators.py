@@ -630,7 +630,8 @@ def ns_recurrence(x, steps=5):
 @pytest.mark.parametrize("shape,steps", [
     ((70, 5000), 5), ((700, 1100), 5), ((1300, 4650), 5), ((1300, 4650), 4),
     ((2500, 2500), 5), ((2050, 8200), 5), ((4097, 4100), 3),
-    ((33, 40003), 5), ((600, 4700), 5), ((1030, 1100), 5)], ids=str)
+    ((33, 40003), 5), ((600, 4700), 5), ((1030, 1100), 5),
+    ((1000, 8000), 5)], ids=str)
 def test_orthogonalize_gpu_large(shape, steps):
     x = ns_inputs(shape, torch.float32, dev())
     want = ns_recurrence(x, steps)

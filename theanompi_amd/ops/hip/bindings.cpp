@@ -1393,9 +1393,40 @@ static int ns_tile(const NsProb& p) {
   return size >= (1L << 24) ? 256 : size >= 6000000 ? 128 : 64;
 }
 
+// Two steps at a time cost a Gram matrix and an X product less and
+// products of m x m more.  That pays from about n = 2m on (us: 256 x 512
+// 121 -> 119, 512 x 1024 174 -> 162, 1000 x 2000 269 -> 268, 1000 x 1500
+// 252 -> 256, 1000 x 3000 327 -> 302, 1536 x 3100 661 -> 610, 2048 x 4096
+// 1022 -> 981, 2048 x 3000 874 -> 888, 4096 x 9216 6535 -> 5545).
+static bool ns_pairs(const NsArgs& a) {
+  double wide = 0.0, square = 0.0;
+  for (int i = 0; i < a.count; ++i) {
+    const NsProb& p = a.p[i];
+    wide += (double)p.batch * p.m * p.m * p.n;
+    square += (double)p.batch * p.m * p.m * p.m;
+  }
+  return wide >= 2.0 * square;
+}
+
+// Of two steps the products of m x m are five that follow one another, or
+// six in four launches: what counts is how many follow one another, until
+// two at a time fill the device (us: 512 x 4608 211 -> 188, the weights
+// of a wide residual network 184 -> 170; tiles of 128: 1000 x 8000, 36 of
+// them, 643 -> 593; 1536 x 4096, 78, 669 -> 653; 2000 x 4000, 136, 966 ->
+// 1014; 4096 x 9216, 528, 5505 -> 5932).
+static bool ns_six(const NsArgs& a) {
+  if (a.tile == 64) return true;
+  long tiles = 0;
+  for (int i = 0; i < a.count; ++i) {
+    const long t = (a.p[i].m + 127) / 128;
+    tiles += a.p[i].batch * (t * (t + 1) / 2);
+  }
+  return tiles <= 128;
+}
+
 // Fills in shapes and workspace of `a` (count problems that have m, n,
 // batch and pointers to their data), and returns the workspace.
-static torch::Tensor ns_workspace(NsArgs& a,
+static torch::Tensor ns_workspace(NsArgs& a, bool pairs,
                                   const torch::TensorOptions& opts) {
   const long tile = a.tile ? a.tile : 64;
   long total = 0;
@@ -1420,8 +1451,9 @@ static torch::Tensor ns_workspace(NsArgs& a,
     at.push_back(take(8L * p.batch * p.parts));
     at.push_back(take(4L * p.batch));
     if (a.tile) {
-      for (int k = 0; k < 3; ++k)
-        at.push_back(take(4L * p.batch * p.mp * p.mp));
+      const long squares = pairs && ns_six(a) ? 6 : 3;
+      at.push_back(take(squares * 4 * p.batch * p.mp * p.mp));
+      at.push_back(0);
     } else {
       // Blocks a matrix: as many as compute units in all, but each adds up
       // the shares of all of its matrix (0.09 us one), and those of a long
@@ -1433,8 +1465,8 @@ static torch::Tensor ns_workspace(NsArgs& a,
       const long groups = blocks <= 256 ? cols : (cols * 256 + blocks - 1) / blocks;
       const long most = std::max(24L, (long)(4.0 * std::sqrt((double)cols)));
       p.groups = (int)std::min(groups, most);
-      for (int k = 0; k < 3; ++k)
-        at.push_back(take(k < 2 ? 4L * p.batch * p.groups * 64 * 64 : 0));
+      for (int k = 0; k < 2; ++k)
+        at.push_back(take(4L * p.batch * p.groups * 64 * 64));
     }
   }
   const long partial = take(a.tile ? NS_SLOTS * tile * tile * 4 : 0);
@@ -1443,13 +1475,13 @@ static torch::Tensor ns_workspace(NsArgs& a,
   a.partial = (float*)(base + partial);
   for (int i = 0; i < a.count; ++i) {
     NsProb& p = a.p[i];
-    const long* o = &at[i * 7];
+    const long* o = &at[i * 6];
     p.X[0] = base + o[0];
     p.X[1] = base + o[1];
     p.part = (double*)(base + o[2]);
     p.shift = (float*)(base + o[3]);
     if (a.tile) {
-      for (int k = 0; k < 3; ++k) p.S[k] = base + o[4 + k];
+      p.S = base + o[4];
     } else {
       p.share[0] = (float*)(base + o[4]);
       p.share[1] = (float*)(base + o[5]);
@@ -1462,7 +1494,8 @@ static torch::Tensor ns_workspace(NsArgs& a,
 // kernels.
 static void ns_run(NsArgs& a, long steps,
                    const torch::TensorOptions& opts) {
-  auto ws = ns_workspace(a, opts);
+  const bool pairs = a.tile && ns_pairs(a), six = ns_six(a);
+  auto ws = ns_workspace(a, pairs, opts);
   auto stream = cur_stream();
   a.steps = (int)steps;
   CHECK_HIP(launch_ns_sum(&a, stream));
@@ -1482,27 +1515,10 @@ static void ns_run(NsArgs& a, long steps,
     }
     return;
   }
-  // Two steps at a time cost a Gram matrix and an X product less and
-  // three products of m x m more.  On a full device that pays from about
-  // n = 2m on (us: 2048 x 4096 1022 -> 981, 4096 x 9216 6535 -> 5545, but
-  // 2048 x 3000 874 -> 888); a smaller matrix waits for each launch, and
-  // has to be longer and large enough (1000 x 3000 381 -> 367, 512 x 4608
-  // 241 -> 222, the weights of a wide residual network 222 -> 205, but
-  // 1000 x 2000 288 -> 312, 512 x 2048 177 -> 184).
-  double size = 0.0, wide = 0.0, square = 0.0;
-  for (int i = 0; i < a.count; ++i) {
-    const NsProb& p = a.p[i];
-    const double one = (double)p.batch * p.m * p.n;
-    size += one;
-    wide += one * p.m;
-    square += (double)p.batch * p.m * p.m * p.m;
-  }
-  const bool pairs = a.tile >= 128 ? wide >= 2.0 * square
-                     : wide >= 2.9 * square && size >= (1L << 21);
   auto product = [&](int mode, int s1, int s2, int to, int poly) {
-    a.s1 = s1;
-    a.s2 = s2;
-    a.to = to;
+    a.s1[0] = s1;
+    a.s2[0] = s2;
+    a.to[0] = to;
     a.poly = poly;
     CHECK_HIP(launch_ns_gemm(&a, mode, stream));
   };
@@ -1512,7 +1528,15 @@ static void ns_run(NsArgs& a, long steps,
     a.last = left == 0;
     product(0, 0, 0, 0, 0);              // S0 = A
     product(1, 0, 0, 1, 1);              // S1 = M
-    if (two) {
+    if (two && six) {
+      a.two = 1;
+      a.s1[1] = 1, a.s2[1] = 0, a.to[1] = 3;
+      product(1, 1, 1, 2, 0);            // S2 = M M, S3 = M A
+      a.s1[1] = 2, a.s2[1] = 3, a.to[1] = 5;
+      product(1, 2, 0, 4, 0);            // S4 = A' = M M A, S5 = A' M
+      a.two = 0;
+      product(1, 4, 5, 0, 2);            // S0 = M' M = aM + bA'M + cA'A'M
+    } else if (two) {
       product(1, 1, 0, 2, 0);            // S2 = M A
       product(1, 1, 2, 0, 0);            // S0 = A' = M A M
       product(1, 0, 0, 2, 1);            // S2 = M'

@@ -336,13 +336,19 @@ struct Tile {
   }
 };
 
+// matrix `mat` of S[k]
+DEV _Float16* square(const NsProb& p, int k, long mat) {
+  return (_Float16*)p.S
+         + ((long)k * p.batch + mat) * 2 * p.mp * (long)p.mp;
+}
+
 // What is done with finished sums: 16 rows of a wave's part of a tile,
 // from row0, FN fragments wide, from col0.  The wave turns them around in
 // its strip of LDS, so that a lane has N neighbours of one row (or, for
 // the other half of a symmetric matrix, of one column) to store.
 template <int MODE, int FN>
-DEV void finish(const NsArgs& a, const NsProb& p, long mat, bool mirror,
-                int row0, int col0, float shift, const f32x4 (&acc)[FN],
+DEV void finish(const NsArgs& a, const NsProb& p, long mat, int which,
+                bool mirror, int row0, int col0, float shift, const f32x4 (&acc)[FN],
                 float* strip) {
   constexpr int N = FN * 4, W = FN * 16 + 4;
   const int lane = threadIdx.x & 63;
@@ -381,11 +387,11 @@ DEV void finish(const NsArgs& a, const NsProb& p, long mat, bool mirror,
                        + mat * 2 * p.mp * (long)p.np,
                    p.np, R, c, f);
   } else {
-    const long at = mat * 2 * p.mp * (long)p.mp;
     const bool poly = MODE == SQUARE && a.poly;
     if (poly) {
-      const _Float16* q = (const _Float16*)p.S[a.s1] + at
-                          + ((long)R * p.mp + c / 32 * 32) * 2 + c % 32;
+      const long at = ((long)R * p.mp + c / 32 * 32) * 2 + c % 32;
+      const _Float16* q = square(p, a.poly == 1 ? a.s1[0] : a.s2[0], mat)
+                          + at;
 #pragma unroll
       for (int k = 0; k < N; k += 8) {
         const half8 hi = *(const half8*)(q + k);
@@ -393,11 +399,18 @@ DEV void finish(const NsArgs& a, const NsProb& p, long mat, bool mirror,
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           f[k + j] = QC * f[k + j] + QB * ((float)hi[j] + (float)lo[j]);
-          if (R == c + k + j) f[k + j] += QA * SCALE;
+          if (a.poly == 1 && R == c + k + j) f[k + j] += QA * SCALE;
+        }
+        if (a.poly == 2) {
+          const _Float16* m = square(p, 1, mat) + at + k;
+          const half8 mh = *(const half8*)m, ml = *(const half8*)(m + 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            f[k + j] += QA * ((float)mh[j] + (float)ml[j]);
         }
       }
     }
-    _Float16* d = (_Float16*)p.S[a.to] + at;
+    _Float16* d = square(p, a.to[which], mat);
     store_split<N>(d, p.mp, R, c, f);
     if (mirror) {
       if (poly) {
@@ -459,6 +472,8 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
     }
     tile += a.skip[i];
   }
+  const int which = MODE == SQUARE && a.two ? tile & 1 : 0;
+  if (MODE == SQUARE && a.two) tile >>= 1;
   const Tile<MODE, BT> at(p, tile);
   const long mat = at.mat;
   const int r0 = at.ti * BT, c0 = at.tj * BT;
@@ -469,9 +484,8 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
   const float shift = MODE == SQUARE ? 1.f : p.shift[mat + lazy];
   const _Float16* X = (const _Float16*)p.X[a.step & 1]
                       + mat * 2 * p.mp * (long)p.np;
-  const long sq = mat * 2 * p.mp * (long)p.mp;
-  const _Float16* Ag = MODE == GRAM ? X : (const _Float16*)p.S[a.s1] + sq;
-  const _Float16* Bg = MODE == SQUARE ? (const _Float16*)p.S[a.s2] + sq : X;
+  const _Float16* Ag = MODE == GRAM ? X : square(p, a.s1[which], mat);
+  const _Float16* Bg = MODE == SQUARE ? square(p, a.s2[which], mat) : X;
   const int K = MODE == GRAM ? p.np : p.mp;
 
   auto stage = [&](int t, int buf) {
@@ -628,7 +642,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
   float* strip = (float*)lds + wave * 16 * (FN * 16 + 4);
 #pragma unroll
   for (int u = 0; u < FM; ++u)
-    finish<MODE, FN>(a, p, mat, at.ti != at.tj, r0 + wr + u * 16, c0 + wc,
+    finish<MODE, FN>(a, p, mat, which, at.ti != at.tj, r0 + wr + u * 16, c0 + wc,
                      shift, acc[u], strip);
 }
 
@@ -647,7 +661,10 @@ __global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
   job -= a.tile0[i];
   const NsProb& p = a.p[i];
   const int cut = job / STRIPS, wave = job % STRIPS / FM, u = job % FM;
-  const Tile<MODE, BT> at(p, a.skip[i] + cut);
+  int tile = a.skip[i] + cut;
+  const int which = MODE == SQUARE && a.two ? tile & 1 : 0;
+  if (MODE == SQUARE && a.two) tile >>= 1;
+  const Tile<MODE, BT> at(p, tile);
   const f32x4* from = (const f32x4*)a.partial
                       + (long)(a.start[i] + cut * a.parts[i]) * BT * BT / 4
                       + (wave * FM + u) * FN * 64 + lane;
@@ -659,7 +676,7 @@ __global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
 #pragma unroll
     for (int v = 0; v < FN; ++v)
       acc[v] += from[(long)j * (BT * BT / 4) + v * 64];
-  finish<MODE, FN>(a, p, at.mat, at.ti != at.tj,
+  finish<MODE, FN>(a, p, at.mat, which, at.ti != at.tj,
                    at.ti * BT + wave / WN * (BT / WM) + u * 16,
                    at.tj * BT + wave % WN * (BT / WN), p.shift[at.mat], acc,
                    strips[threadIdx.x >> 6]);
@@ -1089,8 +1106,8 @@ static int join_starts(NsArgs* a, int per) {
   return strips;
 }
 
-// One product, for every matrix: mode 0 S[to] = X X^T, 1 S[to] = S[s1]
-// S[s2] (with poly: aI + b S[s1] + c S[s1] S[s1]), 2 X <- S[s1] X.
+// One product (of mode 1 maybe two), for every matrix: mode 0 S[to] = X
+// X^T, 1 S[to] = S[s1] S[s2], 2 X <- S[s1] X.
 hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
   // A and M fill the device with tiles of 128 alone
   const int bt = a->tile == 256 && mode != APPLY ? 128 : a->tile;
@@ -1102,6 +1119,7 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
     const NsProb& p = a->p[i];
     const long t = p.mp / bt;
     n[i] = p.batch * (mode == APPLY ? t * (p.np / bt) : t * (t + 1) / 2);
+    if (mode == SQUARE && a->two) n[i] *= 2;
     a->tile0[i] = (int)tiles;
     tiles += n[i];
   }

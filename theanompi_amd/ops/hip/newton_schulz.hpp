@@ -13,7 +13,7 @@ struct NsProb {
   float* v;
   void* copy;
   void* X[2];          // split [mp][np], this step's and the next's
-  void* S[3];          // split [mp][mp]
+  void* S;             // split [.][batch][mp][mp], three or six of them
   double* part;        // [batch][parts] sums of squares
   float* shift;        // [batch] X is kept 1/shift times as large
   float* share[2];     // few rows: [batch][groups][64][64], of X X^T
@@ -37,7 +37,9 @@ struct NsArgs {
   int tile;
   int pair;                // few rows: two steps (1), one (0), first (-1)
   int shared;              // few rows: loading them takes the first shares
-  int s1, s2, to, poly;    // a product: which S, and whether aI + bS is added
+  // a square product S[to] = S[s1] S[s2], or two; poly 1: c times it + aI
+  // + b S[s1], 2: c times it + a S[1] + b S[s2]
+  int s1[2], s2[2], to[2], two, poly;
   int count, steps, step, last, phase, whole;
   float mu;
   float* partial;          // [NS_SLOTS][tile]

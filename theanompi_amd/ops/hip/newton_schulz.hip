@@ -23,7 +23,7 @@
 // A, M and their products are symmetric: only tiles on and below the
 // diagonal are computed, each written twice.
 //
-// Where n is large against m, two steps use X once (see ns_run): what X
+// Where n is large against m, two steps use X once (ns_pairs): what X
 // X^T is after a step is A' = M A M, and X <- (M' M) X.  All matrices of a
 // call go through each step in one launch; what a kernel needs to know of
 // them travels in its arguments, so a captured graph holds it.
@@ -32,7 +32,8 @@
 // takes 5.5 ms, of which 775 us a product with X (1197 TFLOP/s in fp16,
 // where the library's largest fp16 products reach 1340 to 1390), 427 a
 // Gram matrix (1090), 199 one of A and M (1035).  Matrices up to some 2^20
-// elements: the 15 to 20 launches, which need one another's results.  One
+// elements: the 15 to 20 launches, which need one another's results (12 x
+// 333 x 201 128 us, the 17 weights of a wide residual network 168).  One
 // takes 7 to 8 us: 1.3 of launch, 1.1 until a block knows its tile, 1.1
 // for the first slice, 0.43 a further one of 64, 0.9 to store the sums.
 

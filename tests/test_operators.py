@@ -641,6 +641,19 @@ def test_orthogonalize_gpu_large(shape, steps):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(5, 100, 300), (3, 1000, 2100),
+                                   (7, 130, 65), (2, 2100, 1000)], ids=str)
+def test_orthogonalize_gpu_batches(shape):
+    x = ns_inputs(shape, torch.float32, dev())
+    y = OF.orthogonalize(x)
+    for i in range(shape[0]):
+        m = x[i] if shape[1] <= shape[2] else x[i].t()
+        want = ns_recurrence(m, 5)
+        assert off(y[i], want if shape[1] <= shape[2]
+                   else want.t()) < NS_TOL
+
+
+@gpu
 def test_orthogonalize_gpu_same_bits_again():
     for shape in ((64, 576), (300, 2000), (1300, 4650)):
         x = ns_inputs(shape, torch.float32, dev())

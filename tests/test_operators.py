@@ -631,7 +631,7 @@ def ns_recurrence(x, steps=5):
     ((70, 5000), 5), ((700, 1100), 5), ((1300, 4650), 5), ((1300, 4650), 4),
     ((2500, 2500), 5), ((2050, 8200), 5), ((4097, 4100), 3),
     ((33, 40003), 5), ((600, 4700), 5), ((1030, 1100), 5),
-    ((1000, 8000), 5)], ids=str)
+    ((1000, 8000), 5), ((1800, 4500), 5), ((2050, 12000), 5)], ids=str)
 def test_orthogonalize_gpu_large(shape, steps):
     x = ns_inputs(shape, torch.float32, dev())
     want = ns_recurrence(x, steps)
@@ -642,7 +642,9 @@ def test_orthogonalize_gpu_large(shape, steps):
 
 @gpu
 @pytest.mark.parametrize("shape", [(5, 100, 300), (3, 1000, 2100),
-                                   (7, 130, 65), (2, 2100, 1000)], ids=str)
+                                   (7, 130, 65), (2, 2100, 1000),
+                                   (2, 1200, 4700), (5, 1100, 2400)],
+                         ids=str)
 def test_orthogonalize_gpu_batches(shape):
     x = ns_inputs(shape, torch.float32, dev())
     y = OF.orthogonalize(x)
@@ -762,7 +764,9 @@ def test_muon_update_gpu(phase):
 @gpu
 @pytest.mark.parametrize("shapes", [
     [(16, 27), (64, 576), (10, 256), (2, 3, 50)],      # few rows alone
-    [(16, 27), (128, 700), (1300, 4700), (64, 64)]], ids=["few", "mixed"])
+    [(16, 27), (128, 700), (1300, 4700), (64, 64)],
+    [(16, 27), (128, 700), (1800, 4500), (64, 64)]],
+                         ids=["few", "mixed", "large"])
 def test_muon_update_gpu_kinds(shapes):
     """Lists whose matrices take the same kernels and several kinds."""
     muon_check([s for s in shapes if s[0] < 1000], dev())
@@ -1191,7 +1195,7 @@ def test_two_graphs_of_all_kinds_replay_in_turn():
     replay beside each other and beside eager calls."""
     mats = [ns_inputs(s, torch.float32, dev()) for s in
             ((64, 576), (40, 4000), (5, 70, 90), (600, 4700), (1300, 4650),
-             (2500, 2500), (2050, 8200))]
+             (2500, 2500), (2050, 8200), (2050, 12000))]
     logits = [lp_inputs(r, c, torch.bfloat16, dev())
               for r, c in ((3, 300007), (700, 1000))]
     norms = [ln_inputs(s, torch.bfloat16, dev())

@@ -1380,17 +1380,22 @@ static std::vector<torch::Tensor> label_logprobs(
 // ---- Newton-Schulz / orthogonalised momentum --------------------------------
 
 // Which kernels a matrix takes: 0, those for few rows; else the tile of
-// the general ones, larger where there is work enough for all compute
-// units.  Measured (us, 5 steps), few rows against tiles of 64: 64 x 576
-// 36, 98; 64 x 16384 84, 135; 16 x 1000000 723, 736; 100 x 64 x 64 33, 82;
-// 20 x 48 x 20000 307, 293.  Tiles of 64, 128 and
-// 256: 1536 x 1536 440, 491, 523; 1536 x 4096 739, 674, 729; 32 x 512 x 512
-// 516, 512, 549; 3000 x 3000 2116, 1900, 1945; 4096 x 4096 5290, 3562,
-// 3461; 4096 x 9216 10644, 5717, 5547.
+// the general ones, larger where the products are long enough to fill all
+// compute units with it, 256 not where it pads many more rows than 128.
+// Measured (us, 5 steps), few rows against tiles of 64: 64 x 576 37, 88;
+// 64 x 16384 85, 110; 100 x 64 x 64 32, 78; 16 x 1000000 727, 723; 20 x 48
+// x 20000 307, 281.  Tiles of 64, 128 and 256, by batch m m n in 10^9: 0.3
+// (65 x 65536) 220, 293, 435; 8 (1000 x 8000) 466, 563, 625; 12 (1000 x
+// 12000) 605, 699, 683; 12 (2000 x 3000) 866, 824, 896; 14 (2400 x 2400)
+// 1109, 998, 1147; 16 (2000 x 4000) 1073, 914, 963; 18 (300 x 200000) 1347,
+// 1457, 2083; 27 (3000 x 3000) 2144, 1826, 1910; 43 (3500 x 3500) 3415, 2527,
+// 2451; 155 (4096 x 9216) 9532, 5516, 5356.
 static int ns_tile(const NsProb& p) {
   if (p.m <= 64) return 0;
-  const long size = (long)p.batch * p.m * p.n;
-  return size >= (1L << 24) ? 256 : size >= 6000000 ? 128 : 64;
+  const double work = (double)p.batch * p.m * p.m * p.n;
+  const long small = (p.m + 127) / 128 * 128, large = (p.m + 255) / 256 * 256;
+  if (work >= 4e10 && large * 10 <= small * 11) return 256;
+  return work >= 1.25e10 ? 128 : 64;
 }
 
 // Two steps at a time cost a Gram matrix and an X product less and

@@ -123,7 +123,8 @@ LN_SHAPES = [(1, 1), (1, 3), (7, 8), (33, 64), (5, 65), (2, 3, 127),
              (260, 128), (31, 256), (70, 257), (600, 300), (513, 512),
              (129, 1000), (40, 1001), (19, 2048), (11, 2049), (6, 4096),
              (5, 8191), (4, 16384), (3, 16385), (2, 33000), (2, 2, 5, 48),
-             (5000, 16), (700, 9001), (530, 20000)]
+             (5000, 16), (700, 9001), (530, 20000), (520, 768), (6, 1500),
+             (5, 2500), (600, 5000), (3, 12000)]
 
 
 @gpu

@@ -27,23 +27,56 @@
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
-// 16 bytes at any element boundary: global memory takes unaligned wide
-// accesses, so rows of an odd length need no path of their own
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+// 16 bytes (8, 4) at any element boundary: global memory takes unaligned
+// wide accesses, so rows of an odd length need no path of their own
 struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
+struct __attribute__((packed, aligned(2))) any8 { u32x2 v; };
+struct __attribute__((packed, aligned(2))) any4 { unsigned v; };
 
 template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
   union { u32x4 u; T t[N]; };
 
-  // elements [start, start+N) of a row of n that counts; zeros behind it
-  DEV void load(const T* row, int start, int n) {
-    if (start + N <= n) {
-      u = ((const any16*)(row + start))->v;
+  // elements [start, start+N) of a row of n that counts, zeros behind it:
+  // ask, and settle once they are there.  What the row's end cuts is asked
+  // for as the row's last N, by the same instruction as the rest (a path
+  // of its own would wait for its load, and for all before it), and moved.
+  // `load` is for loops with little more than whole vectors.
+  DEV void ask(const T* row, int start, int n) {
+    if (n >= N) {
+      u = ((const any16*)(row + (start + N <= n ? start : n - N)))->v;
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
         t[j] = start + j < n ? row[start + j] : (T)0.f;
+    }
+  }
+  DEV void settle(int start, int n) {
+    if (start >= n) {
+      u = u32x4{0, 0, 0, 0};
+    } else if (start + N > n && n >= N) {
+      u32x4 w = u;
+      const int off = (start + N - n) * (int)sizeof(T);        // bytes
+      if (off & 8) w = u32x4{w[2], w[3], 0, 0};
+      if (off & 4) w = u32x4{w[1], w[2], w[3], 0};
+      if (sizeof(T) == 2 && (off & 2)) {
+        const unsigned long a = (unsigned long)w[1] << 32 | w[0],
+                            b = (unsigned long)w[2] << 32 | w[1],
+                            c = (unsigned long)w[3] << 32 | w[2];
+        w = u32x4{(unsigned)(a >> 16), (unsigned)(b >> 16),
+                  (unsigned)(c >> 16), w[3] >> 16};
+      }
+      u = w;
+    }
+  }
+  DEV void load(const T* row, int start, int n) {
+    if (start + N <= n) {
+      u = ((const any16*)(row + start))->v;
+    } else {
+      ask(row, start, n);
+      settle(start, n);
     }
   }
   DEV float operator[](int j) const { return (float)t[j]; }
@@ -75,10 +108,28 @@ DEV void store_row(T* row, int start, int n, int C, const float* f) {
 #pragma unroll
     for (int j = 0; j < N; ++j) v.t[j] = (T)f[j];
     ((any16*)(row + start))->v = v.u;
-  } else {
+  } else if (start < C) {
+    // 8, 4 and 2 bytes as they come
+    Vec<T> v;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (start + j < C) row[start + j] = start + j < n ? (T)f[j] : (T)0.f;
+    for (int j = 0; j < N; ++j) v.t[j] = start + j < n ? (T)f[j] : (T)0.f;
+    int left = (C - start < N ? C - start : N) * (int)sizeof(T);
+    char* to = (char*)(row + start);
+    if (left >= 16) {
+      ((any16*)to)->v = v.u;
+      left = 0;
+    }
+    if (left & 8) {
+      ((any8*)to)->v = u32x2{v.u[0], v.u[1]};
+      to += 8;
+      v.u = u32x4{v.u[2], v.u[3], 0, 0};
+    }
+    if (left & 4) {
+      ((any4*)to)->v = v.u[0];
+      to += 4;
+      v.u[0] = v.u[1];
+    }
+    if (left & 2) *(unsigned short*)to = (unsigned short)v.u[0];
   }
 }
 
@@ -128,8 +179,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_k(
   auto fetch = [&](long row) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      next[i].load(x + (row < rows ? row : 0) * ldx, (lane + i * TPR) * N,
-                   row < rows ? n : 0);
+      next[i].ask(x + (row < rows ? row : 0) * ldx, (lane + i * TPR) * N, n);
   };
   fetch(r);
   float ga[NV][N], be[NV][N];
@@ -146,6 +196,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_k(
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       v[i] = next[i];
+      v[i].settle((lane + i * TPR) * N, n);
 #pragma unroll
       for (int j = 0; j < N; ++j) s[0] += v[i][j];
     }
@@ -252,8 +303,10 @@ DEV void ln_cols(const T* __restrict__ dy, const T* __restrict__ x,
     for (long r = r0 + ly; r < r1; r += 32) {
       const float m = mean[r], rs = rstd[r];
       Vec<T> g, v;
-      g.load(dy + r * lddy, c, n);
-      v.load(x + r * ldx, c, n);
+      g.ask(dy + r * lddy, c, n);
+      v.ask(x + r * ldx, c, n);
+      g.settle(c, n);
+      v.settle(c, n);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         ag[j] += g[j] * ((v[j] - m) * rs);
@@ -279,7 +332,7 @@ DEV void ln_cols(const T* __restrict__ dy, const T* __restrict__ x,
 
 // dx, and dgamma / dbeta: this block's share of them, part[block][2][C],
 // or (FEW rows) all of them from the blocks behind the first `blocks`,
-// which go by columns.
+// which go by columns.  Only dx where there are no such blocks.
 template <typename T, int TPR, int NV, bool FEW>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
     const T* __restrict__ dy, const T* __restrict__ x,
@@ -307,15 +360,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
   Vec<T> nx[NV], ny[NV];
   float nm, nr;
   auto fetch = [&](long row) {
-    const bool there = row < rows;
-    const long rr = there ? row : 0;
+    const long rr = row < rows ? row : 0;
     nm = mean[rr];
     nr = rstd[rr];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (lane + i * TPR) * N;
-      ny[i].load(dy + rr * lddy, c, there ? n : 0);
-      nx[i].load(x + rr * ldx, c, there ? n : 0);
+      ny[i].ask(dy + rr * lddy, c, n);
+      nx[i].ask(x + rr * ldx, c, n);
     }
   };
   fetch(r);
@@ -333,8 +385,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
     const float m = nm, rs = nr;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const int c = (lane + i * TPR) * N;
       vx[i] = nx[i];
       vy[i] = ny[i];
+      vx[i].settle(c, live ? n : 0);
+      vy[i].settle(c, live ? n : 0);
     }
     if (base + step < rows) fetch(r + step);
     float s[2] = {0.f, 0.f};
@@ -496,9 +551,7 @@ __global__ __launch_bounds__(1024) void ln_join_k(
   }
 }
 
-// Lanes a row and vectors a lane: one 16-byte vector a lane as long as a
-// block has lanes enough.  Two vectors on half the lanes, tried at 1024 to
-// 8192 bf16 channels, ran at 60 to 80 % of that.  v: vectors a row has.
+// Lanes a row of v vectors, with one vector a lane.
 #define LN_PICK(v, CALL)               \
   do {                                 \
     if ((v) <= 8) CALL(8, 1);          \
@@ -508,44 +561,58 @@ __global__ __launch_bounds__(1024) void ln_join_k(
     else if ((v) <= 128) CALL(128, 1); \
     else if ((v) <= 256) CALL(256, 1); \
     else if ((v) <= 512) CALL(512, 1); \
-    else if ((v) <= 1024) CALL(1024, 1); \
-    else CALL(1024, 2);                \
+    else CALL(1024, 1);                \
   } while (0)
 
-// Vectors a row may have for registers.  The backward's sums for two
-// vectors do not fit the 128 that 1024 threads have each (spilled it took
-// 120 us at 2048 x 16384 bf16): rows over 1024 vectors take the wide
-// kernel and the column kernel, which read x and dy twice, in 71 us.
-constexpr long WIDEST_FWD = 2048, WIDEST_BWD = 1024;
+// Vectors a row may have for registers.  The backward's sums of dgamma and
+// dbeta for two vectors do not fit the 128 registers that 1024 threads have
+// each, but without them it does: rows over 1024 vectors leave them to the
+// column kernel, which reads x and dy again (16384 bf16: 3.15 TB/s of the
+// three arrays; with both passes from the wide kernel 2.64).
+constexpr long WIDEST = 2048, WIDEST_SUMS = 1024;
+
+// Threads a compute unit: rows are fetched ahead, and 16 waves do better
+// than 32 (TB/s forward: 256 bf16 5.76, 4.61; 1000 bf16 5.54, 4.40; 512
+// fp32 5.95, 5.25).
+constexpr long THREADS = 1024;
 
 template <typename T>
 hipError_t fwd(const void* x, const float* gamma, const float* beta,
                void* y, float* mean, float* rstd, long rows, int C, int n,
                long ldx, float eps, hipStream_t stream) {
   const long v = (C + Vec<T>::N - 1) / Vec<T>::N;
-  if (v > WIDEST_FWD) {
+  if (v > WIDEST) {
     hipLaunchKernelGGL(ln_fwd_wide_k<T>,
                        dim3((unsigned)(rows < 4096 ? rows : 4096)),
                        dim3(1024), 0, stream, (const T*)x, gamma, beta,
                        (T*)y, mean, rstd, rows, C, n, ldx, eps);
     return hipGetLastError();
   }
-  // Threads a compute unit: rows are fetched ahead, and 16 waves do better
-  // than 32 where a wave has whole rows of a 16-bit type (802816 x 256
-  // bf16: 140 against 173 us); elsewhere they do worse (300000 x 100 f32:
-  // 70 against 50 us, 8192 x 8192 bf16: 74 against 52 us).
-  const long threads = sizeof(T) == 2 && v <= 64 ? 1024 : 2048;
 #define LN_FWD(TPR, NV)                                                  \
   do {                                                                   \
     constexpr int block = TPR > 256 ? TPR : 256;                         \
     long grid = (rows + block / TPR - 1) / (block / TPR);                \
-    const long most = 256L * threads / block;                            \
+    const long most = 256 * THREADS / block;                             \
     if (grid > most) grid = most;                                        \
     hipLaunchKernelGGL((ln_fwd_k<T, TPR, NV>), dim3((unsigned)grid),     \
                        dim3(block), 0, stream, (const T*)x, gamma, beta, \
                        (T*)y, mean, rstd, rows, C, n, ldx, eps);         \
   } while (0)
-  LN_PICK(v, LN_FWD);
+  // Three vectors on lanes that they fill, where one would leave a quarter
+  // to a half of the lanes idle (TB/s with three and one: 300 bf16 4.83,
+  // 3.18; 768 bf16 5.25, 4.72; 1500 bf16 5.15, 3.75; 2500 bf16 4.99, 2.95;
+  // 2500 fp32 5.47, 4.78; 9000 bf16 5.38, two 4.36); past 512 vectors 16-bit
+  // types do better with two (5000 bf16: 4.28 with three, 5.23 with two,
+  // 4.46 with one).
+  if (v > 32 && v <= 48) LN_FWD(16, 3);
+  else if (v > 64 && v <= 96) LN_FWD(32, 3);
+  else if (v > 128 && v <= 192) LN_FWD(64, 3);
+  else if (v > 256 && v <= 384) LN_FWD(128, 3);
+  else if (sizeof(T) == 2 && v > 512 && v <= 1024) LN_FWD(512, 2);
+  else if (sizeof(T) == 4 && v > 512 && v <= 768) LN_FWD(256, 3);
+  else if (v > 1024 && v <= 1536) LN_FWD(512, 3);
+  else if (v > 1536) LN_FWD(1024, 2);
+  else LN_PICK(v, LN_FWD);
 #undef LN_FWD
   return hipGetLastError();
 }
@@ -559,11 +626,19 @@ hipError_t bwd(const void* dy, const void* x, const float* gamma,
   const long v = (C + Vec<T>::N - 1) / Vec<T>::N;
   constexpr int per = 8 * Vec<T>::N;
   const unsigned across = (unsigned)((C + per - 1) / per);
-  if (v > WIDEST_BWD) {
-    hipLaunchKernelGGL(ln_bwd_wide_k<T>,
-                       dim3((unsigned)(rows < 4096 ? rows : 4096)),
-                       dim3(1024), 0, stream, (const T*)dy, (const T*)x,
-                       gamma, mean, rstd, (T*)dx, rows, C, n, ldx, lddy);
+  if (v > WIDEST_SUMS) {
+    if (v <= WIDEST) {
+      const int grid = (int)(rows < 512 ? rows : 512);
+      hipLaunchKernelGGL((ln_bwd_k<T, 1024, 2, true>), dim3(grid),
+                         dim3(1024), 0, stream, (const T*)dy, (const T*)x,
+                         gamma, mean, rstd, (T*)dx, part, dgamma, dbeta,
+                         grid, rows, C, n, ldx, lddy);
+    } else {
+      hipLaunchKernelGGL(ln_bwd_wide_k<T>,
+                         dim3((unsigned)(rows < 4096 ? rows : 4096)),
+                         dim3(1024), 0, stream, (const T*)dy, (const T*)x,
+                         gamma, mean, rstd, (T*)dx, rows, C, n, ldx, lddy);
+    }
     HIP_KERNEL_ASSERT_OK(hipGetLastError());
     hipLaunchKernelGGL(ln_cols_k<T>, dim3(across, (unsigned)shares),
                        dim3(256), 0, stream, (const T*)dy, (const T*)x,
@@ -622,7 +697,7 @@ hipError_t launch_ln_fwd(const void* x, const float* gamma,
 void ln_bwd_plan(long rows, int C, int kind, long* blocks, long* shares) {
   const int N = kind == 0 ? 4 : 8;
   const long v = (C + N - 1) / N;
-  if (v > WIDEST_BWD) {
+  if (v > WIDEST_SUMS) {
     const long across = (C + 8 * N - 1) / (8 * N);
     const long most = (1024 + across - 1) / across;
     const long down = (rows + 127) / 128;
@@ -635,10 +710,7 @@ void ln_bwd_plan(long rows, int C, int kind, long* blocks, long* shares) {
   LN_PICK(v, LN_TPR);
 #undef LN_TPR
   const int block = tpr > 256 ? tpr : 256, rpb = block / tpr;
-  // 16 waves a compute unit; 32 for narrow rows in f32, whose vectors are
-  // half as many values (300000 x 100: 62 against 100 us; but 4099 x 1000
-  // f32 19 against 14, 802816 x 256 bf16 252 against 228)
-  const long most = 256L * (kind == 0 && v <= 64 ? 2048 : 1024) / block;
+  const long most = 256 * THREADS / block;
   const long grid = (rows + rpb - 1) / rpb;
   *blocks = grid < most ? grid : most;
   *shares = rows <= 512 ? 0 : *blocks;

@@ -354,7 +354,8 @@ LP_SHAPES = [(1, 1, None, 1), (3, 2, None, 2), (9, 10, None, 5),
              (4, 1025, None, 3), (3, 2049, 2040, 20), (2, 9001, None, 8),
              (70, 20000, 19999, 4), (1, 131073, None, 32),
              (2, 300007, 300001, 9), (3, 8192, None, 0),
-             (600, 17003, 16999, 4)]
+             (600, 17003, 16999, 4), (9, 1500, None, 6), (5, 2500, 2499, 6),
+             (1100, 5001, None, 3)]
 
 
 @gpu

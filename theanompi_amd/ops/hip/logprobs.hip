@@ -119,31 +119,47 @@ struct Part {
     }
   }
 
-  // All loads are issued before the first is waited for: vectors that
-  // the row does not fill load its start instead, and are overwritten.
+  // All loads are issued before the first is waited for: a vector that
+  // the row's end cuts is loaded as the row's last N, and moved; one
+  // behind it loads the row's start.
   DEV void load(const T* row, int seg0, int n_) {
     first = seg0 + (int)threadIdx.x * N;
     n = n_;
+    const T inf = (T)-__builtin_inff();
     if (n >= N) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        c[i].u = ((const any16*)(row + (has(i, N - 1) ? col(i, 0) : 0)))->v;
+        c[i].u = ((const any16*)(row + (has(i, N - 1) ? col(i, 0)
+                                        : has(i, 0) ? n - N : 0)))->v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          c[i].t[j] = has(i, j) ? row[col(i, j)] : inf;
+      return;
     }
     if (seg0 + LANES * NV * N <= n) return;
+    union { T t[2]; unsigned u; } pad;
+    pad.t[0] = pad.t[1] = inf;
+    const unsigned f = sizeof(T) == 4 ? __float_as_uint(-__builtin_inff())
+                                      : pad.u;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (!has(i, N - 1)) {
+    for (int i = 0; i < NV; ++i) {
+      if (!has(i, 0)) {
+        c[i].u = u32x4{f, f, f, f};
+      } else if (!has(i, N - 1)) {
+        u32x4 w = c[i].u;
+        const int off = (col(i, N) - n) * (int)sizeof(T);      // bytes
+        if (off & 8) w = u32x4{w[2], w[3], f, f};
+        if (off & 4) w = u32x4{w[1], w[2], w[3], f};
+        if (sizeof(T) == 2 && (off & 2))
 #pragma unroll
-        for (int j = 0; j < N; ++j) c[i].t[j] = (T)-__builtin_inff();
+          for (int j = 0; j < 4; ++j)
+            w[j] = w[j] >> 16 | (j < 3 ? w[j + 1] : f) << 16;
+        c[i].u = w;
       }
-    if (n % N == 0) return;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (has(i, 0) && !has(i, N - 1)) {
-#pragma unroll
-        for (int j = 0; j < N - 1; ++j)
-          if (has(i, j)) c[i].t[j] = row[col(i, j)];
-      }
+    }
   }
 };
 
@@ -173,6 +189,16 @@ DEV void write_row(RowStat* stat, float* logp, float* entropy, long r,
   logp[r] = lab < 0 ? 0.f : lab < n ? logp_of(st, xlab)
                                     : __builtin_nanf("");
   entropy[r] = st.H;
+}
+
+// A thread's row of its block's.  The compiler has to see that a wave's
+// are one: what is read of a row then goes through scalar loads (2048 x
+// 131072 with 8 alternatives, backward: 245 us without, 172 with).
+template <int LANES>
+DEV int group() {
+  if (LANES >= 256) return 0;
+  if (LANES >= 64) return __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+  return threadIdx.x / LANES;
 }
 
 // One segment of one row.  Where a row has one segment only (segs == 1)
@@ -465,20 +491,23 @@ __global__ __launch_bounds__(64) void lp_join_k(
   }
 }
 
-// dx of BLOCK*NV vectors of a row: every class as if it were not given,
-// then the few that are.
-template <typename T, int NV>
+// dx of LANES*NV vectors of a row (of several rows, where these are all):
+// every class as if it were not given, then the few that are.
+template <typename T, int LANES, int NV>
 __global__ __launch_bounds__(256) void lp_bwd_k(
     const T* __restrict__ x, const long* __restrict__ labels,
     const long* __restrict__ top_idx, const RowStat* __restrict__ stat,
     const float* __restrict__ dlogp, const float* __restrict__ dentropy,
-    const float* __restrict__ dtop, T* __restrict__ dx, int n, int C,
-    long ldx, int segs, int k) {
+    const float* __restrict__ dtop, T* __restrict__ dx, long rows, int n,
+    int C, long ldx, int segs, int k) {
   constexpr int N = 16 / sizeof(T);
-  const long r = blockIdx.x / segs;
+  const int tid = threadIdx.x % LANES;
+  const long mine = blockIdx.x / segs * (256L / LANES) + group<LANES>();
+  const bool live = mine < rows;
+  const long r = live ? mine : 0;
   const int seg = (int)(blockIdx.x % segs);
-  const int seg0 = seg * 256 * NV * N;
-  const int seg1 = seg0 + 256 * NV * N;
+  const int seg0 = seg * LANES * NV * N;
+  const int seg1 = seg0 + LANES * NV * N;
   const T* row = x + r * ldx;
   T* out = dx + r * C;
   const RowStat st = stat[r];
@@ -488,8 +517,16 @@ __global__ __launch_bounds__(256) void lp_bwd_k(
                    : lab < n ? dlogp[r] : __builtin_nanf("");
   const float dh = dentropy ? dentropy[r] : 0.f;
   float all = dl;
-  if (dtop)
-    for (int a = 0; a < k; ++a) all += dtop[r * k + a];
+  if (dtop) {
+    float sum = 0.f;
+    if (LANES >= 64) {
+      for (int a = 0; a < k; ++a) sum += dtop[r * k + a];
+    } else {
+      for (int a = tid; a < k; a += LANES) sum += dtop[r * k + a];
+      sum = lane_sum<LANES>(sum);
+    }
+    all += sum;
+  }
   const float c0 = -all - dh * st.H;
 
   auto plain = [&](float v) -> float {
@@ -500,8 +537,8 @@ __global__ __launch_bounds__(256) void lp_bwd_k(
            * (c0 - dh * fmaxf(lp, -200.f));
   };
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = seg0 + (i * 256 + (int)threadIdx.x) * N;
+  for (int i = 0; i < NV && live; ++i) {
+    const int c = seg0 + (i * LANES + tid) * N;
     union { u32x4 u; T t[N]; } v;
     if (c + N <= n) {
       v.u = ((const any16*)(row + c))->v;
@@ -515,14 +552,14 @@ __global__ __launch_bounds__(256) void lp_bwd_k(
           out[c + j] = c + j < n ? (T)plain((float)row[c + j]) : (T)0.f;
     }
   }
-  if (empty) return;
   __syncthreads();                 // the block's own stores come first
-  const int a = (int)threadIdx.x;  // 0: the label; from 1: alternatives
-  if (a <= k) {
+  if (empty || !live) return;
+  // 0: the label; from 1: alternatives
+  for (int a = tid; a <= k; a += LANES) {
     const bool isl = a == 0;
     long j = isl ? lab : top_idx[r * k + a - 1];
     if ((isl && (!dlogp || lab < 0 || lab >= n)) || j < seg0 || j >= seg1)
-      return;
+      continue;
     // the label among the alternatives is the label's to write
     float add = isl ? dl : dtop ? dtop[r * k + a - 1] : 0.f;
     if (isl) {
@@ -530,7 +567,7 @@ __global__ __launch_bounds__(256) void lp_bwd_k(
         for (int b = 0; b < k; ++b)
           if (top_idx[r * k + b] == j) add += dtop[r * k + b];
     } else if (!dtop || (dlogp && j == lab)) {
-      return;
+      continue;
     }
     out[j] = (T)(plain((float)row[j]) + add);
   }
@@ -561,15 +598,18 @@ void fwd_one(const FwdArgs& a, hipStream_t stream) {
 
 template <typename T>
 hipError_t fwd(const FwdArgs& a, hipStream_t stream) {
-  if (a.lanes == 64) {
-    if (a.nv == 1) fwd_one<T, 64, 1>(a, stream);
-    else fwd_one<T, 64, 2>(a, stream);
-  } else {
-    if (a.nv == 1) fwd_one<T, 256, 1>(a, stream);
-    else if (a.nv == 2) fwd_one<T, 256, 2>(a, stream);
-    else if (a.nv == 4) fwd_one<T, 256, 4>(a, stream);
-    else fwd_one<T, 256, 8>(a, stream);
-  }
+#define LP_FWD(LANES)                                     \
+  do {                                                    \
+    if (a.nv == 1) fwd_one<T, LANES, 1>(a, stream);       \
+    else if (a.nv == 2) fwd_one<T, LANES, 2>(a, stream);  \
+    else if (a.nv == 3) fwd_one<T, LANES, 3>(a, stream);  \
+    else if (a.nv == 4) fwd_one<T, LANES, 4>(a, stream);  \
+    else if (a.nv == 6) fwd_one<T, LANES, 6>(a, stream);  \
+    else fwd_one<T, LANES, 8>(a, stream);                 \
+  } while (0)
+  if (a.lanes == 64) LP_FWD(64);
+  else LP_FWD(256);
+#undef LP_FWD
   HIP_KERNEL_ASSERT_OK(hipGetLastError());
   if (a.segs > 1)
     hipLaunchKernelGGL(lp_join_k<T>, dim3((unsigned)a.rows), dim3(64), 0,
@@ -587,21 +627,27 @@ struct BwdArgs {
   long rows;
   int n, C;
   long ldx;
-  int segs, k, nv;
+  int segs, k, lanes, nv;
 };
 
-template <typename T, int NV>
+template <typename T, int LANES, int NV>
 void bwd_one(const BwdArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((lp_bwd_k<T, NV>), dim3((unsigned)(a.rows * a.segs)),
+  constexpr long ROWS = 256 / LANES;
+  const long blocks = (a.rows + ROWS - 1) / ROWS * a.segs;
+  hipLaunchKernelGGL((lp_bwd_k<T, LANES, NV>), dim3((unsigned)blocks),
                      dim3(256), 0, stream, (const T*)a.x, a.labels,
                      a.top_idx, (const RowStat*)a.stat, a.dlogp, a.dentropy,
-                     a.dtop, (T*)a.dx, a.n, a.C, a.ldx, a.segs, a.k);
+                     a.dtop, (T*)a.dx, a.rows, a.n, a.C, a.ldx, a.segs,
+                     a.k);
 }
 
 template <typename T>
 hipError_t bwd(const BwdArgs& a, hipStream_t stream) {
-  if (a.nv == 1) bwd_one<T, 1>(a, stream);
-  else bwd_one<T, 2>(a, stream);
+  if (a.lanes == 16) bwd_one<T, 16, 1>(a, stream);
+  else if (a.lanes == 64 && a.nv == 1) bwd_one<T, 64, 1>(a, stream);
+  else if (a.lanes == 64) bwd_one<T, 64, 2>(a, stream);
+  else if (a.nv == 1) bwd_one<T, 256, 1>(a, stream);
+  else bwd_one<T, 256, 2>(a, stream);
   return hipGetLastError();
 }
 
@@ -611,17 +657,23 @@ extern "C" {
 
 // How a row of n classes is cut: lanes a block, vectors a lane, segments
 // a row.  Returns segments, or 0 where n is over what they can hold.
-// Measured (us, forward): a wave a row instead of a block 16384 x 1000 bf16
-// 20, 35; vectors a lane from 1, 2, 4 to 8: 2048 x 131072 bf16 246, 161,
-// 119, 114; 64 x 131072 fp32 28, 19, 15, 14; 512 x 10000 fp32 21, 15, 14,
-// 14; few blocks, where more run at once: 8 x 200000 bf16 17, 14, 14, 25;
-// a last segment nearly empty at 8: 4096 x 50000 bf16 185, 126, 103, 115.
+// Measured (us, forward): a wave a row instead of a block, up to eight
+// vectors a lane: 200000 x 1000 bf16 130, 220; 97656 x 2048 bf16 72, 124;
+// 100000 x 1000 fp32 72, 123; 64 x 2048 fp32 10, 13.  Three vectors or six
+// where they hold a row: 133333 x 1500 bf16 106, four 126; 80000 x 2500
+// bf16 110, eight 129.  Longer rows, vectors a lane from 1, 2, 4 to 8: 2048 x
+// 131072 bf16 246, 161, 119, 114; 64 x 131072 fp32 28, 19, 15, 14; 512 x
+// 10000 fp32 21, 15, 14, 14; few blocks, where more run at once: 8 x 200000
+// bf16 17, 14, 14, 25; a last segment nearly empty at 8: 4096 x 50000 bf16
+// 185, 126, 103, 115.
 int lp_plan(long rows, long n, int kind, int* lanes, int* nv) {
   const long N = kind == 0 ? 4 : 8;
   const long v = (n + N - 1) / N;          // vectors a row
-  if (v <= 128) {
+  if (v <= 512) {
     *lanes = 64;
-    *nv = v <= 64 ? 1 : 2;
+    *nv = 1;
+    while (v > 64 * *nv) *nv *= 2;
+    if (*nv >= 4 && v <= 48 * *nv) *nv = *nv / 4 * 3;
     return 1;
   }
   *lanes = 256;
@@ -637,6 +689,10 @@ int lp_plan(long rows, long n, int kind, int* lanes, int* nv) {
     if (eight * 10 <= four * 11 || cut() > MAXSEG) *nv = 8;
   }
   const long segs = cut();
+  if (*nv >= 4) {                          // as many segments of less
+    const int less = *nv / 4 * 3;
+    if (256L * less * segs >= v) *nv = less;
+  }
   return segs <= MAXSEG ? (int)segs : 0;
 }
 
@@ -678,10 +734,13 @@ hipError_t launch_lp_bwd(const void* x, const long* labels,
                          int C, long ldx, int k, int kind,
                          hipStream_t stream) {
   const long size = kind ? 2 : 4, vectors = (C * size + 15) / 16;
-  // more vectors a lane than two find no more to overlap (2048 x 131072
-  // bf16: 206 us with one, 175 with two, 188 with four)
-  const int nv = vectors <= 256 ? 1 : 2;
-  const int segs = (int)((vectors + 256 * nv - 1) / (256 * nv));
+  // Short rows share a block (1048576 x 10 bf16: 1210 -> 115 us, 200000 x
+  // 1000 309 -> 165).  Longer ones: more vectors a lane than two
+  // find no more to overlap (2048 x 131072 bf16: 206 us with one, 175 with
+  // two, 188 with four).
+  const int lanes = vectors <= 16 ? 16 : vectors <= 128 ? 64 : 256;
+  const int nv = vectors <= lanes ? 1 : 2;
+  const int segs = (int)((vectors + lanes * nv - 1) / (lanes * nv));
   const long most = BLOCKS / segs;
   for (long r = 0; r < rows; r += most) {
     const BwdArgs a = {(const char*)x + r * ldx * size,
@@ -693,7 +752,7 @@ hipError_t launch_lp_bwd(const void* x, const long* labels,
                        dtop ? dtop + r * k : nullptr,
                        (char*)dx + r * C * size,
                        rows - r < most ? rows - r : most,
-                       n, C, ldx, segs, k, nv};
+                       n, C, ldx, segs, k, lanes, nv};
     HIP_KERNEL_ASSERT_OK(kind == 0   ? bwd<float>(a, stream)
                          : kind == 1 ? bwd<_Float16>(a, stream)
                                      : bwd<__bf16>(a, stream));

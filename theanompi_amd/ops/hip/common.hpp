@@ -129,6 +129,46 @@ DEV void glds16(const void* gsrc, void* lds_base) {
                                    16, 0, 0);
 }
 
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+// 16 bytes (8, 4) at any element boundary: global memory takes unaligned
+// wide accesses, so rows of an odd length need no path of their own
+struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
+struct __attribute__((packed, aligned(2))) any8 { u32x2 v; };
+struct __attribute__((packed, aligned(2))) any4 { unsigned v; };
+
+// w from byte `off` (even, below 16) on, `fill` behind its end: what a
+// row's end cuts is loaded as the row's last 16 bytes, like the rest, and
+// moved into place.
+DEV u32x4 move_down(u32x4 w, int off, unsigned fill) {
+  if (off & 8) w = u32x4{w[2], w[3], fill, fill};
+  if (off & 4) w = u32x4{w[1], w[2], w[3], fill};
+  if (off & 2)
+    w = u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16,
+              w[2] >> 16 | w[3] << 16, w[3] >> 16 | fill << 16};
+  return w;
+}
+
+// the first `left` bytes (even) of 16: 8, 4 and 2 as they come
+DEV void store_first(void* at, u32x4 u, int left) {
+  char* to = (char*)at;
+  if (left >= 16) {
+    ((any16*)to)->v = u;
+    return;
+  }
+  if (left & 8) {
+    ((any8*)to)->v = u32x2{u[0], u[1]};
+    to += 8;
+    u = u32x4{u[2], u[3], 0, 0};
+  }
+  if (left & 4) {
+    ((any4*)to)->v = u[0];
+    to += 4;
+    u[0] = u[1];
+  }
+  if (left & 2) *(unsigned short*)to = (unsigned short)u[0];
+}
+
 // Sums and maxima over aligned groups of W lanes (2 to 64), on every lane
 // of the group, without LDS: data-parallel moves within 16 lanes (pairs,
 // quads, then mirrors of 8 and of 16, which exchange the halves once

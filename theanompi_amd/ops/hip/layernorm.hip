@@ -26,14 +26,6 @@
 
 namespace {
 
-typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
-typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
-// 16 bytes (8, 4) at any element boundary: global memory takes unaligned
-// wide accesses, so rows of an odd length need no path of their own
-struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
-struct __attribute__((packed, aligned(2))) any8 { u32x2 v; };
-struct __attribute__((packed, aligned(2))) any4 { unsigned v; };
-
 template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
@@ -57,18 +49,7 @@ struct Vec {
     if (start >= n) {
       u = u32x4{0, 0, 0, 0};
     } else if (start + N > n && n >= N) {
-      u32x4 w = u;
-      const int off = (start + N - n) * (int)sizeof(T);        // bytes
-      if (off & 8) w = u32x4{w[2], w[3], 0, 0};
-      if (off & 4) w = u32x4{w[1], w[2], w[3], 0};
-      if (sizeof(T) == 2 && (off & 2)) {
-        const unsigned long a = (unsigned long)w[1] << 32 | w[0],
-                            b = (unsigned long)w[2] << 32 | w[1],
-                            c = (unsigned long)w[3] << 32 | w[2];
-        w = u32x4{(unsigned)(a >> 16), (unsigned)(b >> 16),
-                  (unsigned)(c >> 16), w[3] >> 16};
-      }
-      u = w;
+      u = move_down(u, (start + N - n) * (int)sizeof(T), 0);
     }
   }
   DEV void load(const T* row, int start, int n) {
@@ -109,27 +90,11 @@ DEV void store_row(T* row, int start, int n, int C, const float* f) {
     for (int j = 0; j < N; ++j) v.t[j] = (T)f[j];
     ((any16*)(row + start))->v = v.u;
   } else if (start < C) {
-    // 8, 4 and 2 bytes as they come
     Vec<T> v;
 #pragma unroll
     for (int j = 0; j < N; ++j) v.t[j] = start + j < n ? (T)f[j] : (T)0.f;
-    int left = (C - start < N ? C - start : N) * (int)sizeof(T);
-    char* to = (char*)(row + start);
-    if (left >= 16) {
-      ((any16*)to)->v = v.u;
-      left = 0;
-    }
-    if (left & 8) {
-      ((any8*)to)->v = u32x2{v.u[0], v.u[1]};
-      to += 8;
-      v.u = u32x4{v.u[2], v.u[3], 0, 0};
-    }
-    if (left & 4) {
-      ((any4*)to)->v = v.u[0];
-      to += 4;
-      v.u[0] = v.u[1];
-    }
-    if (left & 2) *(unsigned short*)to = (unsigned short)v.u[0];
+    store_first(row + start, v.u,
+                C - start < N ? (C - start) * (int)sizeof(T) : 16);
   }
 }
 

@@ -28,9 +28,6 @@
 
 namespace {
 
-typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
-struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
-
 constexpr int MAXSEG = 256;    // segments a row
 
 constexpr int CAP = 256;       // candidates a block may collect
@@ -149,15 +146,7 @@ struct Part {
       if (!has(i, 0)) {
         c[i].u = u32x4{f, f, f, f};
       } else if (!has(i, N - 1)) {
-        u32x4 w = c[i].u;
-        const int off = (col(i, N) - n) * (int)sizeof(T);      // bytes
-        if (off & 8) w = u32x4{w[2], w[3], f, f};
-        if (off & 4) w = u32x4{w[1], w[2], w[3], f};
-        if (sizeof(T) == 2 && (off & 2))
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[j] = w[j] >> 16 | (j < 3 ? w[j + 1] : f) << 16;
-        c[i].u = w;
+        c[i].u = move_down(c[i].u, (col(i, N) - n) * (int)sizeof(T), f);
       }
     }
   }
@@ -545,11 +534,20 @@ __global__ __launch_bounds__(256) void lp_bwd_k(
 #pragma unroll
       for (int j = 0; j < N; ++j) v.t[j] = (T)plain((float)v.t[j]);
       ((any16*)(out + c))->v = v.u;
-    } else {
+    } else if (c < C) {
+      v.u = u32x4{0, 0, 0, 0};
+      if (c < n && n >= N) {
+        v.u = move_down(((const any16*)(row + n - N))->v,
+                        (c + N - n) * (int)sizeof(T), 0);
+      } else if (c < n) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (c + j < n) v.t[j] = row[c + j];
+      }
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (c + j < C)
-          out[c + j] = c + j < n ? (T)plain((float)row[c + j]) : (T)0.f;
+        v.t[j] = c + j < n ? (T)plain((float)v.t[j]) : (T)0.f;
+      store_first(out + c, v.u, C - c < N ? (C - c) * (int)sizeof(T) : 16);
     }
   }
   __syncthreads();                 // the block's own stores come first

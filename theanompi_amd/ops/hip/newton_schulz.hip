@@ -44,8 +44,6 @@
 
 namespace {
 
-typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
-struct __attribute__((packed, aligned(2))) any16 { u32x4 v; };
 typedef __attribute__((ext_vector_type(4))) _Float16 half4;
 typedef __attribute__((ext_vector_type(8))) _Float16 half8;
 typedef __attribute__((ext_vector_type(4))) __fp16 fp16x4;

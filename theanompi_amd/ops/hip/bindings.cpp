@@ -1513,7 +1513,10 @@ static void ns_run(NsArgs& a, long steps,
     a.pair = -1;
     if (!a.shared) CHECK_HIP(launch_ns_few(&a, stream));
     for (int left = (int)steps; left > 0; ++a.step) {
-      a.pair = left >= 2;
+      // The first step alone: two at once lose more of it than of the later
+      // ones (54 x 33, five steps: 1.8e-6 as 2 2 1, 1.5e-6 as 1 2 2; 29 x
+      // 4885 3.8e-6, 1.5e-6).
+      a.pair = a.step > 0 && left >= 2;
       left -= 1 + a.pair;
       a.last = left == 0;
       CHECK_HIP(launch_ns_few(&a, stream));
@@ -1528,7 +1531,8 @@ static void ns_run(NsArgs& a, long steps,
     CHECK_HIP(launch_ns_gemm(&a, mode, stream));
   };
   for (int left = (int)steps; left > 0; ++a.step) {
-    const bool two = pairs && left >= 2;
+    // as with few rows, the first alone (65 x 130: 2.2e-6, 2.0e-6)
+    const bool two = pairs && a.step > 0 && left >= 2;
     left -= two ? 2 : 1;
     a.last = left == 0;
     product(0, 0, 0, 0, 0);              // S0 = A

@@ -516,11 +516,18 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
     }
   };
 
-  f32x4 acc[FM][FN];
+  // The small products of a tile of 64 have sums of their own (see
+  // few_terms); larger ones, whose matrices have longer sums, no registers
+  // for them.
+  constexpr bool APART = BT == 64;
+  f32x4 acc[FM][FN], small[APART ? FM : 1][FN];
 #pragma unroll
   for (int u = 0; u < FM; ++u)
 #pragma unroll
-    for (int v = 0; v < FN; ++v) acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int v = 0; v < FN; ++v) {
+      acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (APART) small[u][v] = acc[u][v];
+    }
   if constexpr (PING) {
     // Two groups of four waves, one of each on every SIMD, half a beat
     // apart: while one reads its fragments (and asks for the next
@@ -637,13 +644,20 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
 #pragma unroll
           for (int u = 0; u < FM; ++u)
 #pragma unroll
-            for (int v = 0; v < FN; ++v)
-              acc[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                  fa[d][term == 2][u], fb[d][term == 1][v], acc[u][v], 0,
-                  0, 0);
+            for (int v = 0; v < FN; ++v) {
+              f32x4& sum = APART && term ? small[APART ? u : 0][v]
+                                         : acc[u][v];
+              sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  fa[d][term == 2][u], fb[d][term == 1][v], sum, 0, 0, 0);
+            }
       buf = buf + 1 == S ? 0 : buf + 1;
     }
   }
+  if constexpr (APART)
+#pragma unroll
+    for (int u = 0; u < FM; ++u)
+#pragma unroll
+      for (int v = 0; v < FN; ++v) acc[u][v] += small[u][v];
   __syncthreads();                  // the ring is free again
   if (steps < slices) {
     f32x4* to = (f32x4*)(a.partial + (long)run * BT * BT);
@@ -709,9 +723,9 @@ __global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
 // `groups` blocks a matrix have a range of X's columns each.  Every block
 // adds up A from all blocks' shares and does the m x m work itself, which
 // costs less than a launch; then it multiplies its columns and leaves its
-// share of the next A.  64 x 576, 5 steps: 36 us in 5 kernels (98 in 17 of
+// share of the next A.  64 x 576, 5 steps: 37.5 us in 5 kernels (88 in 20 of
 // the general ones), 4 for the squares, 6 to load and for the first
-// shares, 10 for two steps, 6.6 for one.  They wait, in turn, for a launch,
+// shares, 10 for two steps, 7 for one.  They wait, in turn, for a launch,
 // the shares, up to six products that need one another, the columns.
 // (Asking for the columns before the products gained nothing here, and
 // lost where a block has many: 64 x 16384 128 -> 139 us.)
@@ -723,6 +737,24 @@ constexpr int SLICE = FEW * 64;               // halves of 32 columns
 // 32 part.  The lanes' columns are rows of P, so that a lane has four
 // neighbours of a row of the result (kept transposed instead, the errors
 // of the chain of products came out twice as large).
+// All four products, the small ones first: an addition in the matrix
+// units seems to cut the sum off, and six of them on the large sum made a
+// step 1.3e-7 off instead of 1.0e-7.  (The smallest, lo * lo, costs 1 us of
+// 36 here and takes a tenth off the errors.)
+DEV void few_terms(const half8 (&f)[2][2][2], const half8 (&g)[2][2][2],
+                   f32x4 (&acc)[2][2]) {
+#pragma unroll
+  for (int term = 3; term >= 0; --term)
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+          acc[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              f[d][term >> 1][u], g[d][term & 1][v], acc[u][v], 0, 0, 0);
+}
+
 DEV void few_product(const _Float16* P, const _Float16* Q, int wr, int wc,
                      f32x4 (&acc)[2][2]) {
   const int l = threadIdx.x & 15;
@@ -730,29 +762,23 @@ DEV void few_product(const _Float16* P, const _Float16* Q, int wr, int wc,
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int v = 0; v < 2; ++v) acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  half8 f[2][2][2], g[2][2][2];
 #pragma unroll
-  for (int d = 0; d < 2; ++d) {
-    half8 f[2][2], g[2][2];
+  for (int d = 0; d < 2; ++d)
 #pragma unroll
     for (int part = 0; part < 2; ++part)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        f[part][u] = frag_rows(Q + d * SLICE, wr + u * 16 + l, part);
-        g[part][u] = frag_rows(P + d * SLICE, wc + u * 16 + l, part);
+        f[d][part][u] = frag_rows(Q + d * SLICE, wr + u * 16 + l, part);
+        g[d][part][u] = frag_rows(P + d * SLICE, wc + u * 16 + l, part);
       }
-#pragma unroll
-    for (int term = 0; term < 3; ++term)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-          acc[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              f[term == 2][u], g[term == 1][v], acc[u][v], 0, 0, 0);
-  }
+  few_terms(f, g, acc);
 }
 
-// four neighbours of row r from column c on into a stage_rows slice pair
-DEV void few_put(_Float16* lds, int r, int c, const f32x4& val) {
+// four neighbours of row r from column c on into a stage_rows slice pair;
+// what is kept of them
+DEV f32x4 few_put(_Float16* lds, int r, int c, const f32x4& val) {
+  f32x4 kept;
   half4 hi, lo;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -760,22 +786,26 @@ DEV void few_put(_Float16* lds, int r, int c, const f32x4& val) {
     split(val[j], h, l);
     hi[j] = h;
     lo[j] = l;
+    kept[j] = (float)h + (float)l;
   }
   _Float16* at = lds + c / 32 * SLICE + r * 64 + c % 8;
   const int q = c % 32 / 8;
   *(half4*)(at + ((q ^ (r & 7)) * 8)) = hi;
   *(half4*)(at + (((q + 4) ^ (r & 7)) * 8)) = lo;
+  return kept;
 }
 
-// a wave's part of a product into LDS
-DEV void few_store(_Float16* lds, int wr, int wc, const f32x4 (&val)[2][2]) {
+// A wave's part of a product into LDS, and what is kept of it in its
+// place: aI + bA + cAA has to be of one A, or what its rounding does to the
+// terms no longer cancels.
+DEV void few_store(_Float16* lds, int wr, int wc, f32x4 (&val)[2][2]) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int v = 0; v < 2; ++v)
-      few_put(lds, wc + v * 16 + (lane & 15),
-              wr + u * 16 + 4 * (lane >> 4), val[u][v]);
+      val[u][v] = few_put(lds, wc + v * 16 + (lane & 15),
+                          wr + u * 16 + 4 * (lane >> 4), val[u][v]);
 }
 
 // aI + b A + c AA (all as kept, SCALE times) from A and the sums of AA
@@ -888,26 +918,18 @@ __global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int v = 0; v < 2; ++v) acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+      half8 f[2][2][2], m[2][2][2];
 #pragma unroll
-      for (int d = 0; d < 2; ++d) {
-        half8 f[2][2], m[2][2];
+      for (int d = 0; d < 2; ++d)
 #pragma unroll
         for (int part = 0; part < 2; ++part)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            f[part][u] = frag_cols<FEW>(T + d * SLICE, wr + u * 16, part);
-            m[part][u] = frag_rows(mul + d * SLICE,
-                                   wc + u * 16 + (lane & 15), part);
+            f[d][part][u] = frag_cols<FEW>(T + d * SLICE, wr + u * 16, part);
+            m[d][part][u] = frag_rows(mul + d * SLICE,
+                                      wc + u * 16 + (lane & 15), part);
           }
-#pragma unroll
-        for (int term = 0; term < 3; ++term)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
-              acc[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                  f[term == 2][u], m[term == 1][v], acc[u][v], 0, 0, 0);
-      }
+      few_terms(f, m, acc);
       few_scale(acc, a.last ? shift / (SCALE * SCALE) : 1.f / SCALE);
       __syncthreads();                         // T is read
 #pragma unroll

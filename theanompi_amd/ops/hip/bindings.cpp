@@ -1510,13 +1510,18 @@ static void ns_run(NsArgs& a, long steps,
     a.shared = a.shared && a.p[i].groups == a.p[i].np / 64;
   CHECK_HIP(launch_ns_load(&a, stream));
   if (!a.tile) {
+    bool elongated = true;
+    for (int i = 0; i < a.count; ++i)
+      elongated = elongated && a.p[i].n >= 4L * a.p[i].m;
     a.pair = -1;
     if (!a.shared) CHECK_HIP(launch_ns_few(&a, stream));
     for (int left = (int)steps; left > 0; ++a.step) {
       // The first step alone: two at once lose more of it than of the later
-      // ones (54 x 33, five steps: 1.8e-6 as 2 2 1, 1.5e-6 as 1 2 2; 29 x
-      // 4885 3.8e-6, 1.5e-6).
-      a.pair = a.step > 0 && left >= 2;
+      // ones (29 x 4885, five steps: 3.8e-6 as 2 2 1, 1.5e-6 as 1 2 2).  Of
+      // matrices that are not long, whose singular values lie far apart, only
+      // the last two go together (54 x 33: 1.5e-6 as 1 2 2, 1.0e-6 as 1 1 1
+      // 2, for 34 us instead of 30).
+      a.pair = left >= 2 && (elongated ? a.step > 0 : left == 2);
       left -= 1 + a.pair;
       a.last = left == 0;
       CHECK_HIP(launch_ns_few(&a, stream));

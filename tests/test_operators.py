@@ -680,6 +680,40 @@ def test_orthogonalize_gpu_weak_directions(shape):
     assert off(OF.orthogonalize(x), ns_formula(x)) < 2.0 ** -13
 
 
+def ns_gradient(shape, seed):
+    """Up to 16 strong directions of falling strength over noise."""
+    g = torch.Generator().manual_seed(seed)
+    rank = max(1, min(16, min(shape) // 4))
+    left = torch.randn(shape[0], rank, generator=g)
+    left *= torch.logspace(0, -1, rank)
+    strong = left @ torch.randn(rank, shape[1], generator=g)
+    return (1e-3 * (strong + 0.5 * torch.randn(*shape, generator=g))).to(
+        dev())
+
+
+def ns_error_check(mats, got):
+    """Distances from 64 bits, of the kernels and of plain fp32 products.
+    Operands of 22 bits are rounded at twice to four times fp32's step, which
+    shows where sums are short: twice plain fp32's error is allowed.  In
+    long sums the additions' roundings are most of it, and both have these:
+    from 128 rows on no more than plain fp32's is."""
+    want = [ns_recurrence(m) for m in mats]
+    plain = [OF.orthogonalize_ref(m) for m in mats]
+    ours = sum(off(a, b) for a, b in zip(got, want))
+    fp32 = sum(off(a, b) for a, b in zip(plain, want))
+    few = min(mats[0].shape) < 128
+    assert ours < (2.0 if few else 1.0) * fp32, (ours, fp32)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [
+    (800, 1600), (2000, 4000), (2500, 2500), (4096, 4096), (4096, 9216)],
+                         ids=str)
+def test_orthogonalize_gpu_errors_of_float32(shape):
+    mats = [ns_gradient(shape, s) for s in range(6 if shape[0] < 512 else 1)]
+    ns_error_check(mats, [OF.orthogonalize(m) for m in mats])
+
+
 @gpu
 @pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e15, 1e30])
 def test_orthogonalize_gpu_magnitudes(scale):

@@ -1381,20 +1381,16 @@ static std::vector<torch::Tensor> label_logprobs(
 
 // Which kernels a matrix takes: 0, those for few rows; else the tile of
 // the general ones, larger where the products are long enough to fill all
-// compute units with it, 256 not where it pads many more rows than 128.
-// Measured (us, 5 steps), few rows against tiles of 64: 64 x 576 37, 88;
-// 64 x 16384 85, 110; 100 x 64 x 64 32, 78; 16 x 1000000 727, 723; 20 x 48
-// x 20000 307, 281.  Tiles of 64, 128 and 256, by batch m m n in 10^9: 0.3
-// (65 x 65536) 220, 293, 435; 8 (1000 x 8000) 466, 563, 625; 12 (1000 x
-// 12000) 605, 699, 683; 12 (2000 x 3000) 866, 824, 896; 14 (2400 x 2400)
-// 1109, 998, 1147; 16 (2000 x 4000) 1073, 914, 963; 18 (300 x 200000) 1347,
-// 1457, 2083; 27 (3000 x 3000) 2144, 1826, 1910; 43 (3500 x 3500) 3415, 2527,
-// 2451; 155 (4096 x 9216) 9532, 5516, 5356.
+// compute units with it.  Measured (us, 5 steps), few rows against tiles of
+// 64: 64 x 576 40, 101; 64 x 16384 88, 134; 100 x 64 x 64 43, 81; 16 x
+// 1000000 743, 1126; 20 x 48 x 20000 317, 382.  Tiles of 64 and 128, by batch
+// m m n in 10^9: 0.3 (65 x 65536) 231, 300; 8 (1000 x 8000) 479, 596; 12
+// (1000 x 12000) 612, 720; 12 (2000 x 3000) 896, 878; 14 (2400 x 2400) 1147,
+// 1030; 16 (2000 x 4000) 1098, 954; 18 (300 x 200000) 1358, 1477; 27 (3000 x
+// 3000) 2187, 1861; 43 (3500 x 3500) 3415, 2675; 155 (4096 x 9216) 9570, 5783.
 static int ns_tile(const NsProb& p) {
   if (p.m <= 64) return 0;
   const double work = (double)p.batch * p.m * p.m * p.n;
-  const long small = (p.m + 127) / 128 * 128, large = (p.m + 255) / 256 * 256;
-  if (work >= 4e10 && large * 10 <= small * 11) return 256;
   return work >= 1.25e10 ? 128 : 64;
 }
 
@@ -1645,7 +1641,7 @@ static void muon_update(std::vector<torch::Tensor> ws,
              ws[i].dim() == 3 ? ws[i].size(0) : 1);
     general = general || ns_tile(p) == 64;
   }
-  for (int tile : {0, 64, 128, 256}) {
+  for (int tile : {0, 64, 128}) {
     size_t i = 0;
     while (i < n) {
       NsArgs a;

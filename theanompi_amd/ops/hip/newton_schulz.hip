@@ -168,8 +168,6 @@ __global__ __launch_bounds__(256) void ns_sum_k(const NsArgs a) {
 
 enum { GRAM, SQUARE, APPLY };
 
-template <int V> struct Int { static constexpr int value = V; };
-
 // what lanes of a wave hand each other through LDS stays in order
 DEV void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -435,10 +433,10 @@ DEV void finish(const NsArgs& a, const NsProb& p, long mat, int which,
 // others is cut into parts[i] runs, whose sums go to a.partial, one place
 // a run, for ns_join_k to add.
 template <int MODE, int BT, int WM, int WN, int S, int DEEP>
-__global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, BT == 128 ? 2 : 1)
+void ns_gemm_k(const NsArgs a) {
   constexpr int THREADS = 64 * WM * WN;
   constexpr int FM = BT / WM / 16, FN = BT / WN / 16;  // fragments a wave
-  constexpr bool PING = BT == 256;
   constexpr int HALVES = BT * 128;           // a 32-deep slice in LDS
   constexpr int LOADS = DEEP * BT * 16 / THREADS;          // a lane
   extern __shared__ __align__(16) _Float16 lds[];
@@ -516,148 +514,86 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_gemm_k(const NsArgs a) {
     }
   };
 
-  // The small products of a tile of 64 have sums of their own (see
-  // few_terms); larger ones, whose matrices have longer sums, no registers
-  // for them.
-  constexpr bool APART = BT == 64;
-  f32x4 acc[FM][FN], small[APART ? FM : 1][FN];
+  // The matrix units cut a sum off where they add to it, always towards 0
+  // and at the sum's own size, and over a long product that is more than all
+  // else is off by.  Tiles of 64 have sums of their own for the small
+  // products (see few_terms).  Those of 128 have longer products and more
+  // registers: the sums of 8 slices are taken by themselves, and added up
+  // with rounding (errors of five steps over those of plain fp32 products,
+  // 4096 x 9216 1.28 -> 0.44, 4096 x 4096 1.32 -> 0.45, 8192 x 8192 1.42 ->
+  // 0.34; 2 slices 0.38 and 16 0.55 at 4096 x 9216, in 6110 and 5750 us where
+  // 8 take 5780).
+  constexpr bool RUNS = BT == 128;
+  f32x4 acc[FM][FN], apart[FM][FN];
 #pragma unroll
   for (int u = 0; u < FM; ++u)
 #pragma unroll
-    for (int v = 0; v < FN; ++v) {
-      acc[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (APART) small[u][v] = acc[u][v];
-    }
-  if constexpr (PING) {
-    // Two groups of four waves, one of each on every SIMD, half a beat
-    // apart: while one reads its fragments (and asks for the next
-    // slice), the other multiplies.  (X of 4096 x 9216: 775 us; with tiles
-    // of 128 and two blocks a unit 830.)  Beats of a group: fragments of B
-    // and of the upper half of A; their products; the lower half of A;
-    // their products.
-    const bool late = wave >= 4;
-    half8 fa[2][FM / 2], fb[2][FN];
-    auto beat = [] {
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    auto read_a = [&](const _Float16* la, int h) {
-#pragma unroll
-      for (int part = 0; part < 2; ++part)
-#pragma unroll
-        for (int u = 0; u < FM / 2; ++u)
-          fa[part][u] = frag_rows(
-              la, wr + (h * (FM / 2) + u) * 16 + (lane & 15), part);
-    };
-    auto multiply = [&](auto h) {
-      constexpr int H = decltype(h)::value * (FM / 2);
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int term = 0; term < 3; ++term)
-#pragma unroll
-        for (int u = 0; u < FM / 2; ++u)
-#pragma unroll
-          for (int v = 0; v < FN; ++v)
-            acc[H + u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                fa[term == 2][u], fb[term == 1][v], acc[H + u][v], 0, 0,
-                0);
-      __builtin_amdgcn_s_setprio(0);
-    };
-    stage(first, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    beat();
-    if (late) beat();
-    for (int t = 0; t < steps; ++t) {
-      const _Float16* la = lds + (t & 1) * HALVES;
-      const _Float16* lb = la + BT * 64;
-#pragma unroll
-      for (int part = 0; part < 2; ++part)
-#pragma unroll
-        for (int v = 0; v < FN; ++v)
-          fb[part][v] =
-              MODE == APPLY
-                  ? frag_cols<BT>(lb, wc + v * 16, part)
-                  : frag_rows(lb, wc + v * 16 + (lane & 15), part);
-      read_a(la, 0);
-      // the other buffer's last readers, the late group in its third
-      // beat of the slice before, are past that beat's barrier
-      if (t + 1 < steps) stage(first + t + 1, (t + 1) & 1);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      beat();
-      multiply(Int<0>());
-      beat();
-      read_a(la, 1);
-      // the next slice is read first in the beat after next
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      beat();
-      multiply(Int<1>());
-      beat();
-    }
-    if (!late) beat();
-  } else {
-    for (int t = 0; t < S - 1 && t < steps; ++t) stage(first + t, t);
-    int buf = 0;
-    for (int t = 0; t < steps; ++t) {
-      // Slice t has landed when only the S - 2 after it are
-      // outstanding.  The barrier is the bare one: a full one would
-      // wait for them too.
-      if (t + S - 1 <= steps)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((S - 2)
-                                                           * LOADS)
-                     : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      // all fragments first: read one by one, each read's latency
-      // stood before its products
-      half8 fa[DEEP][2][FM], fb[DEEP][2][FN];
-#pragma unroll
-      for (int d = 0; d < DEEP; ++d) {
-        const _Float16* la = lds + (buf * DEEP + d) * HALVES;
-        const _Float16* lb = la + BT * 64;
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-#pragma unroll
-          for (int v = 0; v < FN; ++v)
-            fb[d][part][v] =
-                MODE == APPLY
-                    ? frag_cols<BT>(lb, wc + v * 16, part)
-                    : frag_rows(lb, wc + v * 16 + (lane & 15), part);
-#pragma unroll
-          for (int u = 0; u < FM; ++u)
-            fa[d][part][u] =
-                frag_rows(la, wr + u * 16 + (lane & 15), part);
-        }
-      }
-      // into the buffer that every wave was done with at that barrier
-      if (t + S - 1 < steps)
-        stage(first + t + S - 1, buf == 0 ? S - 1 : buf - 1);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int d = 0; d < DEEP; ++d)
-#pragma unroll
-        for (int term = 0; term < 3; ++term)
-#pragma unroll
-          for (int u = 0; u < FM; ++u)
-#pragma unroll
-            for (int v = 0; v < FN; ++v) {
-              f32x4& sum = APART && term ? small[APART ? u : 0][v]
-                                         : acc[u][v];
-              sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                  fa[d][term == 2][u], fb[d][term == 1][v], sum, 0, 0, 0);
-            }
-      buf = buf + 1 == S ? 0 : buf + 1;
-    }
-  }
-  if constexpr (APART)
+    for (int v = 0; v < FN; ++v)
+      acc[u][v] = apart[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto add_apart = [&] {
 #pragma unroll
     for (int u = 0; u < FM; ++u)
 #pragma unroll
-      for (int v = 0; v < FN; ++v) acc[u][v] += small[u][v];
+      for (int v = 0; v < FN; ++v) {
+        acc[u][v] += apart[u][v];
+        apart[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+  };
+  for (int t = 0; t < S - 1 && t < steps; ++t) stage(first + t, t);
+  int buf = 0;
+  for (int t = 0; t < steps; ++t) {
+    // Slice t has landed when only the S - 2 after it are
+    // outstanding.  The barrier is the bare one: a full one would
+    // wait for them too.
+    if (t + S - 1 <= steps)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((S - 2)
+                                                         * LOADS)
+                   : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // all fragments first: read one by one, each read's latency
+    // stood before its products
+    half8 fa[DEEP][2][FM], fb[DEEP][2][FN];
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      const _Float16* la = lds + (buf * DEEP + d) * HALVES;
+      const _Float16* lb = la + BT * 64;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+#pragma unroll
+        for (int v = 0; v < FN; ++v)
+          fb[d][part][v] =
+              MODE == APPLY
+                  ? frag_cols<BT>(lb, wc + v * 16, part)
+                  : frag_rows(lb, wc + v * 16 + (lane & 15), part);
+#pragma unroll
+        for (int u = 0; u < FM; ++u)
+          fa[d][part][u] =
+              frag_rows(la, wr + u * 16 + (lane & 15), part);
+      }
+    }
+    // into the buffer that every wave was done with at that barrier
+    if (t + S - 1 < steps)
+      stage(first + t + S - 1, buf == 0 ? S - 1 : buf - 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+      for (int term = 0; term < 3; ++term)
+#pragma unroll
+        for (int u = 0; u < FM; ++u)
+#pragma unroll
+          for (int v = 0; v < FN; ++v) {
+            f32x4& sum = RUNS || term ? apart[u][v] : acc[u][v];
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                fa[d][term == 2][u], fb[d][term == 1][v], sum, 0, 0, 0);
+          }
+    if (RUNS && (t & 7) == 7) add_apart();
+    buf = buf + 1 == S ? 0 : buf + 1;
+  }
+  add_apart();
   __syncthreads();                  // the ring is free again
   if (steps < slices) {
     f32x4* to = (f32x4*)(a.partial + (long)run * BT * BT);
@@ -1147,9 +1083,7 @@ static int join_starts(NsArgs* a, int per) {
 // One product (of mode 1 maybe two), for every matrix: mode 0 S[to] = X
 // X^T, 1 S[to] = S[s1] S[s2], 2 X <- S[s1] X.
 hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
-  // A and M fill the device with tiles of 128 alone
-  const int bt = a->tile == 256 && mode != APPLY ? 128 : a->tile;
-  const int slots = bt == 256 ? 256 : NS_SLOTS;   // blocks that run at once
+  const int bt = a->tile, slots = NS_SLOTS;   // blocks that run at once
   long tiles = 0, rest = 0, runs = 0;
   bool cut = false;
   long n[NS_MAXP], s[NS_MAXP];
@@ -1219,8 +1153,7 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
   // Two a unit: two of 64.  More: three of 32, so that three share a unit
   // (512 x 4608 226 -> 209, a wide residual network's weights 206 -> 193,
   // though 1000 x 4096 370 -> 382).
-  if (bt == 256) NS_GEMM(APPLY, 256, 2, 4, 2, 1);
-  else if (bt == 128) NS_MODES(128, 2, 2, 2, 1);
+  if (bt == 128) NS_MODES(128, 2, 2, 2, 1);
   else if (deep == 32) NS_MODES(64, 2, 2, 3, 1);
   else if (blocks <= 256) NS_MODES(64, 2, 2, 4, 2);
   else NS_MODES(64, 2, 2, 2, 2);

@@ -707,11 +707,31 @@ def ns_error_check(mats, got):
 
 @gpu
 @pytest.mark.parametrize("shape", [
-    (800, 1600), (2000, 4000), (2500, 2500), (4096, 4096), (4096, 9216)],
-                         ids=str)
+    (32, 2000), (48, 192), (64, 256), (65, 130), (65, 576), (128, 256),
+    (128, 1152), (256, 512), (350, 700), (512, 2000), (800, 1600),
+    (2000, 4000), (2500, 2500), (4096, 4096), (4096, 9216)], ids=str)
 def test_orthogonalize_gpu_errors_of_float32(shape):
     mats = [ns_gradient(shape, s) for s in range(6 if shape[0] < 512 else 1)]
     ns_error_check(mats, [OF.orthogonalize(m) for m in mats])
+
+
+@gpu
+def test_muon_update_gpu_errors_in_a_list():
+    """Short matrices among long ones: with nothing kept of the weight, the
+    momentum all new and a rate of 1 a weight is its orthogonalised gradient."""
+    shapes = [(16, 27), (128, 128), (64, 64), (128, 1152), (256, 2304),
+              (256, 256), (512, 4608), (65, 130)]
+    runs = []
+    for seed in range(4):
+        mats = [ns_gradient(s, seed * 10 + i) for i, s in enumerate(shapes)]
+        ws = [torch.zeros_like(m) for m in mats]
+        vs = [torch.zeros_like(m) for m in mats]
+        many = len(mats)
+        OF.muon_update(ws, [-m for m in mats], vs, [None] * many,
+                       [1.0] * many, [0.0] * many, 0.9, [1.0] * many)
+        runs.append((mats, ws))
+    for i in range(len(shapes)):
+        ns_error_check([m[i] for m, _ in runs], [w[i] for _, w in runs])
 
 
 @gpu

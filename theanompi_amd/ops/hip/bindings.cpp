@@ -1382,8 +1382,8 @@ static std::vector<torch::Tensor> label_logprobs(
 // Which kernels a matrix takes: 0, those for few rows; else the tile of
 // the general ones, larger where the products are long enough to fill all
 // compute units with it.  Measured (us, 5 steps), few rows against tiles of
-// 64: 64 x 576 40, 101; 64 x 16384 88, 134; 100 x 64 x 64 43, 81; 16 x
-// 1000000 743, 1126; 20 x 48 x 20000 317, 382.  Tiles of 64 and 128, by batch
+// 64: 64 x 576 46, 101; 64 x 16384 107, 134; 100 x 64 x 64 40, 81; 16 x
+// 1000000 949, 1126; 20 x 48 x 20000 394, 382.  Tiles of 64 and 128, by batch
 // m m n in 10^9: 0.3 (65 x 65536) 231, 300; 8 (1000 x 8000) 479, 596; 12
 // (1000 x 12000) 612, 720; 12 (2000 x 3000) 896, 878; 14 (2400 x 2400) 1147,
 // 1030; 16 (2000 x 4000) 1098, 954; 18 (300 x 200000) 1358, 1477; 27 (3000 x
@@ -1395,18 +1395,25 @@ static int ns_tile(const NsProb& p) {
 }
 
 // Two steps at a time cost a Gram matrix and an X product less and
-// products of m x m more.  That pays from about n = 2m on (us: 256 x 512
-// 121 -> 119, 512 x 1024 174 -> 162, 1000 x 2000 269 -> 268, 1000 x 1500
-// 252 -> 256, 1000 x 3000 327 -> 302, 1536 x 3100 661 -> 610, 2048 x 4096
-// 1022 -> 981, 2048 x 3000 874 -> 888, 4096 x 9216 6535 -> 5545).
-static bool ns_pairs(const NsArgs& a) {
-  double wide = 0.0, square = 0.0;
+// products of m x m more.  They also cost accuracy: what X X^T is after a
+// step is then M A M, and takes A's rounding up to |M|^2 = 11.9 times as
+// large.  That is less than a plain fp32 product of many rows is off by, but
+// not of few (errors over those of plain fp32 products, one strong direction
+// in 16 and noise: 65 x 130 2.8, 128 x 1152 1.9, 256 x 2304 1.1, 350 x 5000
+// 1.1, 512 x 2048 0.8, 1000 x 8000 0.7; one at a time 0.7, 0.6, 0.7, 0.6, 0.5,
+// 0.4; matrices of little more than two rows' length up to 1.0: 800 x 1600),
+// nor of the first three steps (512 x 2048 1.9; five 0.8).  Hence from 512
+// rows on, where there are four steps, and where it pays: with tiles of 64
+// from n = 3m (us: 512 x 1536 176 -> 164, 1000 x 3000 320 -> 302, 1000 x 8000
+// 613 -> 475), with tiles of 128, whose sums are more exact (0.4 to 0.6), from
+// 2m (2000 x 4000 1006 -> 954, 4096 x 9216 6957 -> 5767).  In a list only if
+// all of its matrices may.
+static bool ns_pairs(const NsArgs& a, long steps) {
   for (int i = 0; i < a.count; ++i) {
     const NsProb& p = a.p[i];
-    wide += (double)p.batch * p.m * p.m * p.n;
-    square += (double)p.batch * p.m * p.m * p.m;
+    if (p.m < 512 || p.n < (a.tile == 64 ? 3L : 2L) * p.m) return false;
   }
-  return wide >= 2.0 * square;
+  return steps >= 4;
 }
 
 // Of two steps the products of m x m are five that follow one another, or
@@ -1495,7 +1502,7 @@ static torch::Tensor ns_workspace(NsArgs& a, bool pairs,
 // kernels.
 static void ns_run(NsArgs& a, long steps,
                    const torch::TensorOptions& opts) {
-  const bool pairs = a.tile && ns_pairs(a), six = ns_six(a);
+  const bool pairs = a.tile && ns_pairs(a, steps), six = ns_six(a);
   auto ws = ns_workspace(a, pairs, opts);
   auto stream = cur_stream();
   a.steps = (int)steps;
@@ -1506,18 +1513,14 @@ static void ns_run(NsArgs& a, long steps,
     a.shared = a.shared && a.p[i].groups == a.p[i].np / 64;
   CHECK_HIP(launch_ns_load(&a, stream));
   if (!a.tile) {
-    bool elongated = true;
-    for (int i = 0; i < a.count; ++i)
-      elongated = elongated && a.p[i].n >= 4L * a.p[i].m;
     a.pair = -1;
     if (!a.shared) CHECK_HIP(launch_ns_few(&a, stream));
     for (int left = (int)steps; left > 0; ++a.step) {
-      // The first step alone: two at once lose more of it than of the later
-      // ones (29 x 4885, five steps: 3.8e-6 as 2 2 1, 1.5e-6 as 1 2 2).  Of
-      // matrices that are not long, whose singular values lie far apart, only
-      // the last two go together (54 x 33: 1.5e-6 as 1 2 2, 1.0e-6 as 1 1 1
-      // 2, for 34 us instead of 30).
-      a.pair = left >= 2 && (elongated ? a.step > 0 : left == 2);
+      // Only the last two of five or more go together, when the singular
+      // values have gathered (see ns_pairs; errors over those of plain fp32
+      // products, 32 x 2000 2.2 as 1 2 2, 0.8 as 1 1 1 2 and one by one;
+      // 64 x 576, us, 40, 46 and 51).
+      a.pair = left == 2 && a.step >= 3;
       left -= 1 + a.pair;
       a.last = left == 0;
       CHECK_HIP(launch_ns_few(&a, stream));
@@ -1532,7 +1535,7 @@ static void ns_run(NsArgs& a, long steps,
     CHECK_HIP(launch_ns_gemm(&a, mode, stream));
   };
   for (int left = (int)steps; left > 0; ++a.step) {
-    // as with few rows, the first alone (65 x 130: 2.2e-6, 2.0e-6)
+    // the first alone: the weak directions are weakest then
     const bool two = pairs && a.step > 0 && left >= 2;
     left -= two ? 2 : 1;
     a.last = left == 0;

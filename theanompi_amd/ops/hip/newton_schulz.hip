@@ -12,8 +12,11 @@
 // few strong ones.  So every matrix is kept as the sum of two fp16
 // numbers (22 bits of significand), scaled by 2^12 so that the second
 // one stays clear of fp16's smallest step, and a product is three matrix
-// products, hi*hi + hi*lo + lo*hi, in fp32 accumulators: the accuracy of
-// fp32 at a third of the fp16 rate, five times the fp32 matrix rate.
+// products, hi*hi + hi*lo + lo*hi, in fp32 accumulators, at a third of the
+// fp16 rate, five times the fp32 matrix rate.  Five steps are off by 0.6 to
+// 2.2e-6 (Frobenius norm, relative): 0.4 to 0.9 times what plain fp32 products
+// are from 65 rows on, and up to 1.7 times of some ten rows, whose sums are
+// so short that the two bits show.
 // The entries stay far below fp16's largest: singular values of X are at
 // most 1.21 over the whole iteration, those of M at most 3.45.
 //
@@ -26,7 +29,9 @@
 // Where n is large against m, two steps use X once (ns_pairs): what X
 // X^T is after a step is A' = M A M, and X <- (M' M) X.  All matrices of a
 // call go through each step in one launch; what a kernel needs to know of
-// them travels in its arguments, so a captured graph holds it.
+// them travels in its arguments, so a captured graph holds it.  How a matrix'
+// sums are cut, and whether two steps go together, depends on its neighbours
+// in a list: equal lists give equal bits, and a matrix alone others.
 //
 // What bounds it, 5 steps: large matrices, the matrix units: 4096 x 9216
 // takes 5.5 ms, of which 775 us a product with X (1197 TFLOP/s in fp16,

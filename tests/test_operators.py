@@ -955,6 +955,70 @@ def test_muon_optimizer_phases_and_rest_cpu():
     assert 0.5 * 0.1 * 0.2 < rms < 1.3 * 0.1 * 0.2
 
 
+def muon_recs_without_gradients(device):
+    """A trained matrix, a frozen one, one that got a single gradient, and
+    their optimizer under each way to step."""
+    from theanompi_amd.lib.opt import Muon, ParamRec
+    after = []
+    for way in ("step", "phases", "persistent"):
+        g = torch.Generator().manual_seed(0)
+        ps = [torch.nn.Parameter(torch.randn(4, 6, generator=g).to(device))
+              for _ in range(3)]
+        ps[1].requires_grad_(False)
+        recs = [ParamRec(p, matrix=(1, 4, 6)) for p in ps]
+        opt = Muon(recs, lr=0.1, momentum=0.9, weight_decay=0.01)
+        if way == "persistent":
+            opt.make_persistent()
+        start = [p.detach().clone() for p in ps]
+        once = None
+        for it in range(10):
+            opt.zero_grad()
+            grad = torch.randn(4, 6, generator=g).to(device)
+            if way == "persistent":
+                ps[0].grad.copy_(grad)
+            else:
+                ps[0].grad = grad
+                ps[2].grad = 1e-6 * grad if it == 0 else None
+            if way == "phases":
+                opt.phase1()
+                opt.phase2()
+            else:
+                opt.step()
+            if it == 0:
+                once = ps[2].detach().clone()
+        assert not torch.equal(ps[0], start[0])
+        assert torch.equal(ps[1], start[1]), way
+        if way != "persistent":
+            assert not torch.equal(once, start[2])
+            assert torch.equal(ps[2], once), way
+            after.append([p.detach().clone() for p in ps])
+    for a, b in zip(*after):
+        assert torch.equal(a, b)
+
+
+def test_muon_leaves_weights_without_a_gradient_cpu():
+    muon_recs_without_gradients("cpu")
+
+
+@gpu
+def test_muon_leaves_weights_without_a_gradient_gpu():
+    muon_recs_without_gradients(dev())
+
+
+def test_muon_phase2_by_itself_cpu():
+    """Without a first phase the gradients that are there decide."""
+    from theanompi_amd.lib.opt import Muon, ParamRec
+    ps = [torch.nn.Parameter(torch.ones(3, 4)) for _ in range(2)]
+    recs = [ParamRec(p, matrix=(1, 3, 4)) for p in ps]
+    for r in recs:
+        r.vel.copy_(torch.eye(3, 4))
+    opt = Muon(recs, lr=0.1)
+    ps[0].grad = torch.zeros(3, 4)
+    opt.phase2()
+    assert not torch.equal(ps[0], torch.ones(3, 4))
+    assert torch.equal(ps[1], torch.ones(3, 4))
+
+
 def test_optimizer_by_name():
     from theanompi_amd.lib import opt
     from theanompi_amd.models.cifar10 import Cifar10_model

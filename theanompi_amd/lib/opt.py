@@ -218,9 +218,12 @@ class Muon(SGDMomentum):
     NS are ``steps`` Newton-Schulz products (ops.functional.
     orthogonalize); its entries' root mean square is about
     1/sqrt(longer side), so an update's is about lr*rms whatever the
-    matrix's shape.  Between the phases the cdd exchange averages the
-    momenta, and every worker orthogonalises the average.  A merged
-    weight (several 1x1 convolutions over one input) is one matrix."""
+    matrix's shape.  A matrix without a gradient is left as it is, in
+    both phases: orthogonalising would make a full step of whatever
+    momentum it has left.  Between the phases the cdd exchange averages
+    the momenta, and every worker orthogonalises the average; so a matrix
+    has to have a gradient on all workers or on none.  A merged weight
+    (several 1x1 convolutions over one input) is one matrix."""
 
     def __init__(self, recs, lr=0.02, momentum=0.95, weight_decay=0.0,
                  grad_arena=None, steps=5, rms=0.2):
@@ -228,6 +231,7 @@ class Muon(SGDMomentum):
         self.steps = steps
         self.rms = rms
         self._mats = [r for r in self.recs if r.matrix is not None]
+        self._moved = None             # matrices of the last phase 1
         self._rest = SGDMomentum(
             [r for r in self.recs if r.matrix is None], lr, momentum,
             weight_decay)
@@ -242,8 +246,15 @@ class Muon(SGDMomentum):
         self._rest.invalidate()
 
     def _update(self, phase):
-        recs = self._mats if phase == 2 else [
-            r for r in self._mats if r.master.grad is not None]
+        if phase == 2 and self._moved is not None:
+            recs = self._moved
+        else:
+            # persistent gradients are there for frozen weights, too
+            recs = [r for r in self._mats if r.master.grad is not None
+                    and (r.master.requires_grad
+                         or not self.persistent_grads)]
+        if phase == 1:
+            self._moved = recs
         ws, gs, vs, outs, lrs, wds, scales = [], [], [], [], [], [], []
         for r in recs:
             ws.append(r.master.data.view(r.matrix))

@@ -440,6 +440,37 @@ def test_label_logprobs_nan_and_bad_labels_gpu():
     lp_nan_check(dev())
 
 
+def lp_nan_first_check(device, dtype):
+    """NaN in the first class, in all and in the first few of them: the
+    alternatives are those of a stable sort, whatever their number."""
+    nan = float("nan")
+    for c, k in ((1, 1), (10, 10), (32, 32), (40, 7), (3000, 5), (9001, 32),
+                 (70000, 8)):
+        x, labels = lp_inputs(5, c, dtype, device)
+        x[0, 0] = nan
+        x[1] = nan
+        x[2, :3] = nan
+        x[3, ::2] = nan
+        x[3, 1::2] = float("inf")
+        out = OF.label_logprobs(x, labels, top=k)
+        want = torch.sort(x.float().cpu(), dim=1, descending=True,
+                          stable=True).indices[:, :k]
+        assert torch.equal(out[3].cpu(), want), (c, k)
+        for t in out[:3]:
+            assert torch.isnan(t[:4]).all() and torch.isfinite(t[4]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_label_logprobs_nan_first_cpu(dtype):
+    lp_nan_first_check("cpu", dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_label_logprobs_nan_first_gpu(dtype):
+    lp_nan_first_check(dev(), dtype)
+
+
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_label_logprobs_gpu_strides(dtype):

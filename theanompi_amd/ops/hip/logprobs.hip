@@ -37,9 +37,11 @@ constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
 // classes.
 struct RowStat { float M, logs, H; };
 
-// floats in an order that unsigned integers have: NaN above all, -0 as 0
+// floats in an order that unsigned integers have: NaN above all, -0 as 0.
+// No float has all bits set, so that every key lies below ~0, where the
+// search for the best starts.
 DEV unsigned ordered(float f) {
-  if (f != f) return 0xffffffffu;
+  if (f != f) return 0xfffffffeu;
   const unsigned u = __float_as_uint(f + 0.f);
   return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }

@@ -773,6 +773,38 @@ def test_orthogonalize_gpu_magnitudes(scale):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(40, 100), (64, 9000), (70, 150),
+                                   (600, 2000), (1300, 8000)], ids=str)
+@pytest.mark.parametrize("scale,steps", [
+    (1e-12, 3), (1e-12, 10), (1e-16, 14), (1e-20, 12), (1e-20, 20),
+    (1e-20, 27), (1e-30, 1), (1e-30, 40), (1e-30, 44), (3e-38, 2),
+    (3e-38, 60)])
+def test_orthogonalize_gpu_small_norms_and_many_steps(scale, steps, shape):
+    """Norms far below 1e-7 leave X as far below 1, which takes a step for
+    each factor of 3.4445 to grow: on the way there and a few steps after
+    (singular values that have grown go to and fro between 0.7 and 1.2, and
+    tens of such steps would make any rounding large)."""
+    x = ns_inputs(shape, torch.float32, dev(), scale=scale)
+    want = ns_recurrence(x, steps)
+    assert 0 < float(want.norm()) < 1.3 * math.sqrt(shape[0])
+    assert off(OF.orthogonalize(x, steps), want) < NS_TOL * max(1, steps / 5)
+
+
+@gpu
+def test_orthogonalize_gpu_small_norms_in_a_batch():
+    scales = (1e-15, 1e-18, 1e-20, 0.0, 1e-30)
+    for shape in ((30, 50), (80, 90)):
+        x = torch.stack([ns_inputs(shape, torch.float32, dev(), scale=s,
+                                   seed=i) for i, s in enumerate(scales)])
+        y = OF.orthogonalize(x, 20)
+        for i, s in enumerate(scales):
+            if s:
+                assert off(y[i], ns_recurrence(x[i], 20)) < NS_TOL * 20 / 5
+            else:
+                assert not y[i].any()
+
+
+@gpu
 def test_orthogonalize_gpu_zero_nan_empty():
     x = torch.zeros(3, 40, 50, device=dev())
     x[1] = torch.randn(40, 50, device=dev())

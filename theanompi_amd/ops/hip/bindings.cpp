@@ -1487,7 +1487,7 @@ static torch::Tensor ns_workspace(NsArgs& a, bool pairs,
     p.X[0] = base + o[0];
     p.X[1] = base + o[1];
     p.part = (double*)(base + o[2]);
-    p.shift = (float*)(base + o[3]);
+    p.low = (int*)(base + o[3]);
     if (a.tile) {
       p.S = base + o[4];
     } else {
@@ -1505,7 +1505,12 @@ static void ns_run(NsArgs& a, long steps,
   const bool pairs = a.tile && ns_pairs(a, steps), six = ns_six(a);
   auto ws = ns_workspace(a, pairs, opts);
   auto stream = cur_stream();
-  a.steps = (int)steps;
+  // `left` steps to go, of which the next launch makes the `more` first
+  auto grow = [&](long left, int more) {
+    const double rate = std::log2(3.4445);
+    a.grown = (int)std::ceil(rate * (steps - left));
+    a.grows = (int)std::ceil(rate * (steps - left + more));
+  };
   CHECK_HIP(launch_ns_sum(&a, stream));
   if (a.phase == 1) return;
   a.shared = !a.tile;
@@ -1521,6 +1526,7 @@ static void ns_run(NsArgs& a, long steps,
       // products, 32 x 2000 2.2 as 1 2 2, 0.8 as 1 1 1 2 and one by one;
       // 64 x 576, us, 40, 46 and 51).
       a.pair = left == 2 && a.step >= 3;
+      grow(left, 1 + a.pair);
       left -= 1 + a.pair;
       a.last = left == 0;
       CHECK_HIP(launch_ns_few(&a, stream));
@@ -1537,6 +1543,7 @@ static void ns_run(NsArgs& a, long steps,
   for (int left = (int)steps; left > 0; ++a.step) {
     // the first alone: the weak directions are weakest then
     const bool two = pairs && a.step > 0 && left >= 2;
+    grow(left, two ? 2 : 1);
     left -= two ? 2 : 1;
     a.last = left == 0;
     product(0, 0, 0, 0, 0);              // S0 = A

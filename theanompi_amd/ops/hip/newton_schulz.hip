@@ -80,6 +80,15 @@ DEV void typed(const NsProb& p, F f) {
   else f((const __bf16*)p.in);
 }
 
+// A norm far below 1e-7 leaves X far below 1, and fp16 would lose it: X is
+// kept 2^kept() times as large.  |X| starts in [1, 2) 2^-low and grows by QA at
+// most in each step, and by just that while it is small; `grown` is log2 of
+// that, rounded up.  So what is kept stays between 1/4 and 1 until X itself is
+// that large.
+DEV int kept(int low, int grown) {
+  return low - 1 > grown ? low - 1 - grown : 0;
+}
+
 DEV void split(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
@@ -350,7 +359,7 @@ DEV _Float16* square(const NsProb& p, int k, long mat) {
 // the other half of a symmetric matrix, of one column) to store.
 template <int MODE, int FN>
 DEV void finish(const NsArgs& a, const NsProb& p, long mat, int which,
-                bool mirror, int row0, int col0, float shift,
+                bool mirror, int row0, int col0, int low,
                 const f32x4 (&acc)[FN], float* strip,
                 const half8* early = nullptr) {
   constexpr int N = FN * 4, W = FN * 16 + 4;
@@ -359,8 +368,12 @@ DEV void finish(const NsArgs& a, const NsProb& p, long mat, int which,
   const int xc = lane % (FN * 16), xr = lane / (FN * 16) * N;
   const bool result = MODE == APPLY && a.last;
   // what takes a sum to the scale of the split matrix or of the result
-  const float unit = MODE == GRAM ? shift * shift / SCALE
-                     : result ? shift / (SCALE * SCALE) : 1.f / SCALE;
+  const int now = MODE == SQUARE ? 0 : kept(low, a.grown);
+  const float unit =
+      MODE == GRAM     ? ldexpf(1.f / SCALE, -2 * now)
+      : MODE == SQUARE ? 1.f / SCALE
+      : result         ? ldexpf(1.f / (SCALE * SCALE), -now)
+                       : ldexpf(1.f / SCALE, kept(low, a.grows) - now);
   // lane: column lane&15 of a fragment, rows 4*(lane>>4) + r
 #pragma unroll
   for (int v = 0; v < FN; ++v)
@@ -484,7 +497,7 @@ void ns_gemm_k(const NsArgs a) {
   // the end (a scalar load holds up all others)
   int lazy = 0;
   asm volatile("" : "+v"(lazy));
-  const float shift = MODE == SQUARE ? 1.f : p.shift[mat + lazy];
+  const int low = MODE == SQUARE ? 0 : p.low[mat + lazy];
   const _Float16* X = (const _Float16*)p.X[a.step & 1]
                       + mat * 2 * p.mp * (long)p.np;
   const _Float16* Ag = MODE == GRAM ? X : square(p, a.s1[which], mat);
@@ -613,7 +626,7 @@ void ns_gemm_k(const NsArgs a) {
 #pragma unroll
   for (int u = 0; u < FM; ++u)
     finish<MODE, FN>(a, p, mat, which, at.ti != at.tj, r0 + wr + u * 16,
-                     c0 + wc, shift, acc[u], strip,
+                     c0 + wc, low, acc[u], strip,
                      EARLY ? early[u] : nullptr);
 }
 
@@ -649,7 +662,7 @@ __global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
       acc[v] += from[(long)j * (BT * BT / 4) + v * 64];
   finish<MODE, FN>(a, p, at.mat, which, at.ti != at.tj,
                    at.ti * BT + wave / WN * (BT / WM) + u * 16,
-                   at.tj * BT + wave % WN * (BT / WN), p.shift[at.mat], acc,
+                   at.tj * BT + wave % WN * (BT / WN), p.low[at.mat], acc,
                    strips[threadIdx.x >> 6]);
 }
 
@@ -785,7 +798,7 @@ __global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
   const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
   const int b = blockIdx.x - a.start[i], g = b % p.groups;
   const long mat = b / p.groups;
-  const float shift = p.shift[mat];
+  const int low = p.low[mat], now = kept(low, a.grown);
   const _Float16* X = (const _Float16*)p.X[a.step & 1]
                       + mat * 2 * FEW * (long)p.np;
   const int blocks = p.np / FEW;               // of 64 columns
@@ -810,7 +823,7 @@ __global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
 #pragma unroll
         for (int v = 0; v < 2; ++v)
           sum[u][v] += from[j * (FEW * FEW / 4) + (u * 2 + v) * 64];
-    few_scale(sum, shift * shift / SCALE);
+    few_scale(sum, ldexpf(1.f / SCALE, -2 * now));
     few_store(P, wr, wc, sum);                 // P = A
     __syncthreads();
     few_product(P, P, wr, wc, acc);
@@ -837,6 +850,8 @@ __global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
     }
   }
   const _Float16* mul = a.pair ? P : Q;
+  const float unit = a.last ? ldexpf(1.f / (SCALE * SCALE), -now)
+                            : ldexpf(1.f / SCALE, kept(low, a.grows) - now);
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -871,7 +886,7 @@ __global__ __launch_bounds__(256) void ns_few_k(const NsArgs a) {
                                       wc + u * 16 + (lane & 15), part);
           }
       few_terms(f, m, acc);
-      few_scale(acc, a.last ? shift / (SCALE * SCALE) : 1.f / SCALE);
+      few_scale(acc, unit);
       __syncthreads();                         // T is read
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -962,16 +977,10 @@ __global__ __launch_bounds__(256) void ns_load_k(const NsArgs a) {
   for (int k = threadIdx.x; k < p.parts; k += 256)
     sum += p.part[mat * p.parts + k];
   sum = block_sum(sum, red);
-  // A norm far below 1e-7 leaves X far below 1, and fp16 would lose it:
-  // it is kept 2^e times as large, e so that `steps` growths by QA end
-  // below 1 all the same.
   const double norm = sqrt(sum), inv0 = 1.0 / (norm + 1e-7);
-  int e = 0;
-  if (norm * inv0 < 0.5 && norm > 0.0)
-    e = -ilogb(norm * inv0) - 1 - (int)(1.785 * a.steps + 1.0);
-  if (e < 0) e = 0;
-  const double inv = ldexp((double)SCALE * inv0, e);
-  if (b == 0 && threadIdx.x == 0) p.shift[mat] = (float)ldexp(1.0, -e);
+  const int low = norm * inv0 < 0.5 && norm > 0.0 ? -ilogb(norm * inv0) : 1;
+  const double inv = ldexp((double)SCALE * inv0, kept(low, 0));
+  if (b == 0 && threadIdx.x == 0) p.low[mat] = low;
 #pragma unroll
   for (int t = 0; t < 16; ++t)
     tile[t * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] =

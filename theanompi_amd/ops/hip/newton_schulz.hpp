@@ -15,7 +15,7 @@ struct NsProb {
   void* X[2];          // split [mp][np], this step's and the next's
   void* S;             // split [.][batch][mp][mp], three or six of them
   double* part;        // [batch][parts] sums of squares
-  float* shift;        // [batch] X is kept 1/shift times as large
+  int* low;            // [batch] |X| starts in [1, 2) 2^-low
   float* share[2];     // few rows: [batch][groups][64][64], of X X^T
   int m, n, mp, np;    // m <= n; padded
   int groups;          // few rows: blocks a matrix
@@ -40,7 +40,8 @@ struct NsArgs {
   // a square product S[to] = S[s1] S[s2], or two; poly 1: c times it + aI
   // + b S[s1], 2: c times it + a S[1] + b S[s2]
   int s1[2], s2[2], to[2], two, poly;
-  int count, steps, step, last, phase, whole;
+  int grown, grows;        // log2 of what X has grown by at most; after it
+  int count, step, last, phase, whole;
   float mu;
   float* partial;          // [NS_SLOTS][tile]
 };

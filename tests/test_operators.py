@@ -181,6 +181,36 @@ def test_layernorm_gpu_constant_rows_and_no_rows():
 
 
 @gpu
+@pytest.mark.parametrize("dtype,value", [
+    (torch.float32, 1000.0), (torch.float32, 16000.0), (torch.float32, 1e5),
+    (torch.float32, -0.1), (torch.float16, 16000.0), (torch.float16, 1001.0),
+    (torch.bfloat16, 1.5e5)])
+def test_layernorm_gpu_rows_of_one_large_value(dtype, value):
+    """Outputs are beta, at any width.  The mean as first summed is off by
+    DEPTH U |x| at most; the mean of the deviations from it gives that to
+    within DEPTH U again, (DEPTH U)^2 |x| = 6e-11 |x|, which is below half
+    a step of x, so the mean is x.  The variance is off by 2 DEPTH U
+    (DEPTH U x)^2 at most, dx by half of that relative to eps, and rounded."""
+    for c in (3, 7, 48, 100, 300, 700, 1000, 1500, 2500, 5000, 9001, 12000,
+              20000, 40000):
+        for rows in (5, 600):
+            _, gamma, beta, dy = ln_inputs((rows, c), dtype, dev())
+            x = torch.full((rows, c), value, dtype=dtype, device=dev())
+            leaf = x.requires_grad_(True)
+            y = OF.layernorm(leaf, gamma, beta)
+            assert torch.equal(y, beta.to(dtype).expand_as(y)), (c, rows)
+            if abs(value) > 1001:
+                continue
+            (dx,) = torch.autograd.grad(y, leaf, dy)
+            g = dy.double() * gamma.double()
+            want = (g - g.mean(1, keepdim=True)) / math.sqrt(1e-5)
+            var = 2 * DEPTH * U * (DEPTH * U * value) ** 2 / 1e-5
+            close(dx, want, (var / 2 + DEPTH * U + half(dtype)) * want.abs()
+                  + DEPTH * U * g.abs().mean(1, keepdim=True)
+                  / math.sqrt(1e-5), (c, rows))
+
+
+@gpu
 @pytest.mark.parametrize("shape", [(700, 300), (100, 4000)], ids=str)
 def test_layernorm_gpu_same_bits_again(shape):
     args = ln_inputs(shape, torch.bfloat16, dev())

@@ -12,7 +12,8 @@
 // lanes (TPR of them, NV 16-byte vectors each), so every element is
 // read once; the variance is the mean of squared deviations from the
 // mean already known, which keeps its digits where the mean is large
-// against the spread.  Only the first n of C channels count: what is
+// against the spread, and the deviations' own mean takes the roundings of
+// the first sum out (see row_stats).  Only the first n of C channels count: what is
 // behind them (the physical channel padding) is left out of the
 // statistics, and its outputs are zeros.
 //
@@ -125,6 +126,25 @@ DEV void row_sum(float* v, float* red, int& turn) {
   }
 }
 
+// A row's mean as first summed, and rounded: left to itself the compiler fuses
+// the product into each deviation, and these are from a mean with more bits
+// than the one that is corrected by them.
+DEV float first_mean(float sum, float inv_n) {
+#pragma clang fp contract(off)
+  return sum * inv_n;
+}
+
+// Mean and 1/sqrt(variance + eps) of a row from m, the mean as first summed,
+// and the sums of the deviations d from it and of their squares.  m is off by
+// the roundings of its sum and of 1/n, and rows of one large value show it:
+// 16000 at 1000 channels gave -0.3 instead of 0.  mean(d) is what m is off by.
+DEV void row_stats(float& m, float& rs, const float* s, float inv_n,
+                   float eps) {
+  const float fix = s[0] * inv_n, var = s[1] * inv_n - fix * fix;
+  m += fix;
+  rs = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);       // NaN stays
+}
+
 template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_k(
     const T* __restrict__ x, const float* __restrict__ gamma,
@@ -157,7 +177,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_k(
        base += step, r += step) {
     const bool live = r < rows;
     Vec<T> v[NV];
-    float s[1] = {0.f};
+    float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       v[i] = next[i];
@@ -167,17 +187,18 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_fwd_k(
     }
     if (base + step < rows) fetch(r + step);   // while this one is summed
     row_sum<TPR, 1>(s, red, turn);
-    const float m = s[0] * inv_n;
+    float m = first_mean(s[0], inv_n), rs;
     s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float d = v[i][j] - m;
-        s[0] += (lane + i * TPR) * N + j < n ? d * d : 0.f;
+        const float d = (lane + i * TPR) * N + j < n ? v[i][j] - m : 0.f;
+        s[0] += d;
+        s[1] += d * d;
       }
-    row_sum<TPR, 1>(s, red, turn);
-    const float rs = 1.f / sqrtf(s[0] * inv_n + eps);
+    row_sum<TPR, 2>(s, red, turn);
+    row_stats(m, rs, s, inv_n, eps);
     if (live) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -209,7 +230,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_k(
   const float inv_n = 1.f / (float)n;
   for (long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = x + r * ldx;
-    float s[1] = {0.f};
+    float s[2] = {0.f, 0.f};
     Vec<T> v;
 #pragma unroll 2
     for (int c = threadIdx.x * N; c < n; c += 1024 * N) {
@@ -218,17 +239,20 @@ __global__ __launch_bounds__(1024) void ln_fwd_wide_k(
       for (int j = 0; j < N; ++j) s[0] += v[j];
     }
     row_sum<1024, 1>(s, red, turn);
-    const float m = s[0] * inv_n;
+    float m = first_mean(s[0], inv_n), rs;
     s[0] = 0.f;
 #pragma unroll 2
     for (int c = threadIdx.x * N; c < n; c += 1024 * N) {
       v.load(row, c, n);
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        s[0] += c + j < n ? (v[j] - m) * (v[j] - m) : 0.f;
+      for (int j = 0; j < N; ++j) {
+        const float d = c + j < n ? v[j] - m : 0.f;
+        s[0] += d;
+        s[1] += d * d;
+      }
     }
-    row_sum<1024, 1>(s, red, turn);
-    const float rs = 1.f / sqrtf(s[0] * inv_n + eps);
+    row_sum<1024, 2>(s, red, turn);
+    row_stats(m, rs, s, inv_n, eps);
 #pragma unroll 2
     for (int c = threadIdx.x * N; c < C; c += 1024 * N) {
       float f[N], ga[N], be[N];

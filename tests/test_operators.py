@@ -502,6 +502,35 @@ def test_label_logprobs_nan_first_gpu(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("c", [5, 700, 5000, 40001])
+def test_label_logprobs_gpu_large_maxima(c):
+    """Maxima whose product with log2 e loses from a part of 1 to some 128 in
+    rounding, on either side (fp32's smallest normal power is 2^-126)."""
+    peaks = [1e5, 1.2e7, 3e7, -3e7, 4e8, 2000019456.0, 2000027264.0,
+             2147523840.0, -2000003840.0, -2000011648.0, 1.7e10, 3e38]
+    g = torch.Generator().manual_seed(2)
+    x = torch.tensor(peaks)[:, None].repeat(1, c)
+    steps = torch.randint(0, 4, x.shape, generator=g) * 2.0 ** -23
+    x = x - x.abs() * steps
+    x[:, 3] = torch.tensor(peaks)
+    x[::2, 1] = -math.inf
+    labels = torch.full((len(peaks),), 3)
+    grads = lp_grads(len(peaks), 3)
+    leaf = x.to(dev()).requires_grad_(True)
+    out = OF.label_logprobs(leaf, labels.to(dev()), top=3)
+    (dx,) = torch.autograd.grad(out[:3], leaf, [t.to(dev()) for t in grads])
+    # a logarithm of some hundred classes is below half a step of 3e38 in 64
+    # bits, too: the formula takes what the rows are below their maxima,
+    # which is exact and gives the same probabilities
+    ref, tol = lp_formula(x.double() - x[:, 3:4].double(), labels, c, 3,
+                          grads)
+    assert torch.equal(out[3].cpu(), ref[3])
+    for i, name in enumerate(("logp", "entropy", "top_logp")):
+        close(out[i], ref[i], tol[i], name)
+    close(dx, ref[4], tol[4] + U * ref[4].abs(), "dlogits")
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_label_logprobs_gpu_strides(dtype):
     x, labels = lp_inputs(9, 600, dtype, dev(), n=250)

@@ -273,10 +273,10 @@ __global__ __launch_bounds__(LANES) void lp_fwd_k(
   const float fix = __builtin_amdgcn_exp2f(-off);
   t = (t - off * s) * fix * LN2;
   s *= fix;
-  if (t != t) {
-    // A masked class (0 * -inf), a NaN, or an M near the largest number
-    // that c does not hold: once more, step by step.  Lanes without have
-    // the same sums from both.
+  if (t != t || !(fabsf(off) < 1.f)) {
+    // A masked class (0 * -inf), a NaN, or an M of 2^23 or more, of which c
+    // has lost whole powers of two or which it does not hold: once more, step
+    // by step.  Lanes without have the same sums from both.
     s = t = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)

@@ -211,6 +211,21 @@ def test_layernorm_gpu_rows_of_one_large_value(dtype, value):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layernorm_gpu_overflowing_squares(dtype):
+    """Deviations whose squares fp32 does not hold: the variance is infinite
+    and outputs are beta, as in the CPU's form."""
+    for c in (20, 1000, 20000):
+        x, gamma, beta, _ = ln_inputs((4, c), torch.float32, dev())
+        for t in (x * 1e25 + 1e30, x * 1e24, torch.full_like(x, 1.1e33)):
+            t = t.to(dtype)
+            y = OF.layernorm(t, gamma, beta)
+            assert torch.equal(y, beta.to(dtype).expand_as(y)), c
+            assert torch.equal(OF.layernorm(t.cpu(), gamma.cpu(),
+                                            beta.cpu()), y.cpu())
+
+
+@gpu
 @pytest.mark.parametrize("shape", [(700, 300), (100, 4000)], ids=str)
 def test_layernorm_gpu_same_bits_again(shape):
     args = ln_inputs(shape, torch.bfloat16, dev())

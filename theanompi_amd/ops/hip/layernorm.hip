@@ -140,9 +140,12 @@ DEV float first_mean(float sum, float inv_n) {
 // 16000 at 1000 channels gave -0.3 instead of 0.  mean(d) is what m is off by.
 DEV void row_stats(float& m, float& rs, const float* s, float inv_n,
                    float eps) {
-  const float fix = s[0] * inv_n, var = s[1] * inv_n - fix * fix;
+  const float fix = s[0] * inv_n;
+  float var = s[1] * inv_n;
+  // squares that overflow leave the variance infinite; NaN stays
+  if (var < __builtin_inff()) var = fmaxf(var - fix * fix, 0.f);
   m += fix;
-  rs = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);       // NaN stays
+  rs = 1.f / sqrtf(var + eps);
 }
 
 template <typename T, int TPR, int NV>

@@ -226,6 +226,30 @@ def test_layernorm_gpu_overflowing_squares(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 2, 4, 16, 64, 256, 1024, 4096, 16384])
+def test_layernorm_gpu_gradient_of_large_constant_rows(n, dtype):
+    """Powers of two sum exactly: deviations are 0, 1/std is 1e15, and
+    nothing behind the row's end may count (0 - 2^90 times 1e15 overflows
+    there).  dx is (g - mean g) 1e15, off by the roundings of a sum."""
+    for more in (0, 1, 3, 21, 300):
+        for rows in (5, 600):
+            c = n + more
+            x = torch.full((rows, c), 2.0 ** 90, dtype=dtype, device=dev())
+            _, gamma, beta, dy = ln_inputs((rows, c), dtype, dev())
+            leaf = x.requires_grad_(True)
+            ga = gamma.requires_grad_(True)
+            y = OF.layernorm(leaf, ga, beta, eps=1e-30, n_features=n)
+            dx, dgamma = torch.autograd.grad(y, (leaf, ga), dy)
+            g = dy.double()[:, :n] * gamma.detach().double()[:n]
+            want = (g - g.mean(1, keepdim=True)) * 1e15
+            tol = (DEPTH * U + half(dtype)) * want.abs() + DEPTH * U * (
+                g.abs() + g.abs().mean(1, keepdim=True)) * 1e15
+            close(dx[:, :n], want, tol, (c, rows))
+            assert not dx[:, n:].float().any() and not dgamma.any()
+
+
+@gpu
 @pytest.mark.parametrize("shape", [(700, 300), (100, 4000)], ids=str)
 def test_layernorm_gpu_same_bits_again(shape):
     args = ln_inputs(shape, torch.bfloat16, dev())

@@ -37,13 +37,16 @@ struct Vec {
   // for as the row's last N, by the same instruction as the rest (a path
   // of its own would wait for its load, and for all before it), and moved.
   // `load` is for loops with little more than whole vectors.
+  // NEAR leaves some of the row's own values behind its end, for what meets
+  // gradients of 0 there and has to be finite: (0 - mean)*rstd need not be.
+  template <bool NEAR = false>
   DEV void ask(const T* row, int start, int n) {
     if (n >= N) {
       u = ((const any16*)(row + (start + N <= n ? start : n - N)))->v;
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        t[j] = start + j < n ? row[start + j] : (T)0.f;
+        t[j] = start + j < n ? row[start + j] : NEAR ? row[0] : (T)0.f;
     }
   }
   DEV void settle(int start, int n) {
@@ -51,6 +54,18 @@ struct Vec {
       u = u32x4{0, 0, 0, 0};
     } else if (start + N > n && n >= N) {
       u = move_down(u, (start + N - n) * (int)sizeof(T), 0);
+    }
+  }
+  DEV void settle_near(int start, int n) {
+    if (start < n && start + N > n && n >= N)
+      u = move_down(u, (start + N - n) * (int)sizeof(T), u[3]);
+  }
+  DEV void load_near(const T* row, int start, int n) {
+    if (start + N <= n) {
+      u = ((const any16*)(row + start))->v;
+    } else {
+      ask<true>(row, start, n);
+      settle_near(start, n);
     }
   }
   DEV void load(const T* row, int start, int n) {
@@ -359,7 +374,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
     for (int i = 0; i < NV; ++i) {
       const int c = (lane + i * TPR) * N;
       ny[i].ask(dy + rr * lddy, c, n);
-      nx[i].ask(x + rr * ldx, c, n);
+      nx[i].template ask<true>(x + rr * ldx, c, n);
     }
   };
   fetch(r);
@@ -380,7 +395,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
       const int c = (lane + i * TPR) * N;
       vx[i] = nx[i];
       vy[i] = ny[i];
-      vx[i].settle(c, live ? n : 0);
+      vx[i].settle_near(c, n);
       vy[i].settle(c, live ? n : 0);
     }
     if (base + step < rows) fetch(r + step);
@@ -390,7 +405,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_bwd_k(
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         // behind the row's end dy and gamma are 0, and so is what a row
-        // that is not there adds; x is 0 there, and xh is finite
+        // that is not there adds; x is of the row there, and xh finite
         const float xh = (vx[i][j] - m) * rs, d = vy[i][j];
         if (!FEW) {
           ag[i][j] += d * xh;
@@ -482,7 +497,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide_k(
 #pragma unroll 2
     for (int c = threadIdx.x * N; c < n; c += 1024 * N) {
       g.load(dr, c, n);
-      v.load(xr, c, n);
+      v.load_near(xr, c, n);
       load_param<N>(gamma, c, n, ga);
 #pragma unroll
       for (int j = 0; j < N; ++j) {

@@ -1052,6 +1052,48 @@ def muon_refusals(device):
         assert isinstance(call(steps=steps), ValueError)
 
 
+def muon_shared_memory(device):
+    """Overlaps are refused, whatever their start, and nothing is written;
+    neighbours in one buffer and a gradient for two weights are fine."""
+    def call(change):
+        flat = torch.randn(400, device=device)
+        cut = lambda at, rows=4: flat[at:at + rows * 5].view(  # noqa: E731
+            rows, 5)
+        parts = {"ws": [cut(0), cut(20)], "gs": [cut(40), cut(60)],
+                 "vs": [cut(80), cut(100)],
+                 "outs": [cut(120, 2).view(torch.bfloat16).view(4, 5), None]}
+        change(parts, cut)
+        kept = flat.clone()
+        try:
+            OF.muon_update(parts["ws"], parts["gs"], parts["vs"],
+                           parts["outs"], [0.1] * 2, [0.0] * 2, 0.9,
+                           [1.0] * 2)
+        except ValueError:
+            assert torch.equal(flat, kept)
+            return False
+        return True
+
+    def put(name, i, at):
+        return lambda parts, cut: parts[name].__setitem__(i, cut(at))
+
+    assert call(lambda parts, cut: None)
+    assert call(put("gs", 1, 40))                 # one gradient for two
+    for name, i, at in (("ws", 1, 0), ("ws", 1, 5), ("ws", 0, 15),
+                        ("vs", 0, 101), ("vs", 1, 15), ("gs", 0, 0),
+                        ("gs", 1, 79), ("gs", 0, 99), ("gs", 1, 125),
+                        ("ws", 0, 110), ("vs", 0, 121)):
+        assert not call(put(name, i, at)), (name, i, at)
+
+
+def test_muon_update_shared_memory_cpu():
+    muon_shared_memory("cpu")
+
+
+@gpu
+def test_muon_update_shared_memory_gpu():
+    muon_shared_memory(dev())
+
+
 def test_muon_update_refusals_cpu():
     muon_refusals("cpu")
     OF.muon_update([], [], [], [], [], [], 0.9, [])

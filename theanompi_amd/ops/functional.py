@@ -621,6 +621,22 @@ def orthogonalize(x, steps=5):
         return orthogonalize_ref(x, steps) if x.numel() else x.clone()
 
 
+def _check_apart(written, read):
+    """No memory of ``written`` is another's, or any of ``read``'s (on the
+    GPU the extension looks)."""
+    end = write_end = 0
+    for start, stop, writes in sorted(
+            (t.data_ptr(), t.data_ptr() + t.nbytes, writes)
+            for ts, writes in ((written, True), (read, False))
+            for t in ts if t.numel()):
+        if start < (end if writes else write_end):
+            raise ValueError("a weight, momentum or working copy shares "
+                             "memory with another tensor of the list")
+        end = max(end, stop)
+        if writes:
+            write_end = max(write_end, stop)
+
+
 def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
                 steps=5):
     """Orthogonalised momentum update of a list of weights, in place:
@@ -630,6 +646,7 @@ def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
     ``ws``, ``gs``, ``vs``: float32, contiguous, [rows, cols] or [batch,
     rows, cols] (each matrix of a batch on its own); ``outs``: bf16
     working copies of w, or None in the place of one that is not kept.
+    Weights, momenta and copies share no memory with anything in the list.
     ``phase``: 0 the whole update, 1 the momentum only, 2 the weights
     only (gs are not read and may be None), as in the SGD step.  On the GPU
     every matrix of the list goes through each product in one launch, and
@@ -645,7 +662,6 @@ def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
     _check_steps(steps)
     if not many:
         return
-    seen = set()
     for i in range(many):
         w = ws[i]
         parts = [("w", w), ("v", vs[i])]
@@ -672,13 +688,6 @@ def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
                     or outs[i].device != w.device:
                 raise ValueError(f"out {i} must be contiguous, of its "
                                  "weight's size and on its device")
-        if w.numel():
-            for t in (w, vs[i], outs[i]):
-                if t is not None and t.data_ptr() in seen:
-                    raise ValueError("a weight, momentum or working copy "
-                                     "is in the list twice")
-                if t is not None:
-                    seen.add(t.data_ptr())
     keeps = [1.0 - lr * wd for lr, wd in zip(lrs, wds)]
     rates = [lr * scale for lr, scale in zip(lrs, scales)]
     with torch.no_grad():
@@ -691,6 +700,8 @@ def muon_update(ws, gs, vs, outs, lrs, wds, momentum, scales, phase=0,
                 [none if o is None else o for o in outs], keeps, rates,
                 float(momentum), phase, steps)
             return
+        _check_apart([*ws, *vs, *(o for o in outs if o is not None)],
+                     gs if phase != 2 else [])
         for i in range(many):
             out = outs[i]
             if ws[i].numel():

@@ -1598,6 +1598,38 @@ static torch::Tensor orthogonalize(torch::Tensor x, long steps) {
   return out;
 }
 
+// What is written may share memory with nothing else, what is read with
+// nothing that is written: matrices go through the kernels in any order.
+static void check_apart(const std::vector<torch::Tensor>& ws,
+                        const std::vector<torch::Tensor>& vs,
+                        const std::vector<torch::Tensor>& outs,
+                        const std::vector<torch::Tensor>& gs) {
+  struct Span { const char *start, *stop; bool writes; };
+  std::vector<Span> spans;
+  auto add = [&](const std::vector<torch::Tensor>& ts, bool writes) {
+    for (const auto& t : ts)
+      if (t.numel()) {
+        const char* at = (const char*)t.data_ptr();
+        spans.push_back({at, at + t.nbytes(), writes});
+      }
+  };
+  add(ws, true);
+  add(vs, true);
+  add(outs, true);
+  add(gs, false);
+  std::sort(spans.begin(), spans.end(),
+            [](const Span& a, const Span& b) { return a.start < b.start; });
+  const char *end = nullptr, *write_end = nullptr;
+  for (const Span& s : spans) {
+    if (s.start < (s.writes ? end : write_end))
+      throw pybind11::value_error(
+          "a weight, momentum or working copy shares memory with another "
+          "tensor of the list");
+    end = std::max(end, s.stop);
+    if (s.writes) write_end = std::max(write_end, s.stop);
+  }
+}
+
 // w, v (and the bf16 copies) in place.  Phases as sgd_step's: 0 = full,
 // 1 = momentum only, 2 = weights from the momentum.
 static void muon_update(std::vector<torch::Tensor> ws,
@@ -1635,6 +1667,7 @@ static void muon_update(std::vector<torch::Tensor> ws,
                   "out must have w's shape");
     }
   }
+  check_apart(ws, vs, outs, gs);
   c10::DeviceGuard guard(ws[0].device());
   // One pass for each kind of kernels, NS_MAXP matrices at a time.  Few
   // rows have kernels of their own only where no others take the general

@@ -1241,6 +1241,29 @@ def test_optimizer_by_name():
     assert type(m.opt) is opt.SGDMomentum
 
 
+@pytest.mark.parametrize("optimizer", ["sgd", "muon"])
+def test_wrapped_module_with_an_empty_parameter(optimizer):
+    from theanompi_amd.models.module_adapter import wrap_module
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.none = torch.nn.Parameter(torch.zeros(0, 5))
+            self.fc = torch.nn.Linear(3 * 16 * 16, 10)
+
+        def forward(self, x):
+            return self.fc(x.flatten(1)) + self.none.sum()
+
+    model = wrap_module(Net, batch_size=4, n_classes=10, image_hw=16)
+    m = model({"device": "cpu", "verbose": False, "n_iters": 1,
+               "optimizer": optimizer})
+    m.compile_iter_fns("cdd")
+    before = m.module.fc.weight.detach().clone()
+    m.train_iter(0)
+    m.apply_update()
+    assert not torch.equal(before, m.module.fc.weight)
+
+
 def test_layernorm_layer_cpu():
     from theanompi_amd.models import layers as L
     ln = L.LayerNorm(10)

@@ -25,6 +25,8 @@ exchangers, rules, recorder, checkpoint format — is the framework's.
 That separation is exactly what the reference's Keras wrap demonstrated.
 """
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -80,8 +82,8 @@ class ContractAdapter:
         self.module = self.module_factory().to(self.device)
         self.module.train()
         self.data = self.data_factory()
-        self.recs = [ParamRec(p, name, matrix=(1, p.shape[0], p[0].numel())
-                              if p.dim() > 1 else None)
+        self.recs = [ParamRec(p, name, matrix=None if p.dim() < 2 else
+                              (1, p.shape[0], math.prod(p.shape[1:])))
                      for name, p in self.module.named_parameters()]
         self.params = [r.master for r in self.recs]
         self.vels = [r.vel for r in self.recs]

@@ -1478,6 +1478,49 @@ def test_layernorm_gpu_long_offsets():
 
 
 @gpu
+def test_layernorm_gpu_most_channels():
+    """More channels than one launch of the last sum has threads for.  A
+    lane adds up c / 1024 values, and the sums of 1024 lanes are joined."""
+    c = 2 ** 25 + 37
+    x, gamma, beta, dy = ln_inputs((2, c), torch.float32, dev())
+    leaves = [t.requires_grad_(True) for t in (x, gamma, beta)]
+    y = OF.layernorm(*leaves)
+    got = [y, *torch.autograd.grad(y, leaves, dy)]
+    ref, _ = ln_formula(x.detach(), gamma.detach(), beta.detach(), dy, 1e-5,
+                        c)
+    depth = c // 1024 + 32
+    xh = (ref[0] - beta.detach().double()) / gamma.detach().double()
+    e = depth * U * (xh.abs() + float(x.detach().abs().max()))
+    ga, d = gamma.detach().double().abs(), dy.double().abs()
+    tols = [ga * e + 4 * U * (ref[0].abs() + beta.detach().abs()),
+            d * ga * e + 4 * depth * U * (d * ga + 1 + xh.abs()),
+            (d * e).sum(0) + 4 * U * ref[2].abs(), 4 * U * d.sum(0)]
+    for a, r, t, name in zip(got, ref, tols, ("y", "dx", "dgamma", "dbeta")):
+        close(a, r, t, name)
+    del ref, tols, xh, e
+    with pytest.raises(RuntimeError):
+        OF.layernorm(torch.empty(1, 2 ** 28 + 1, dtype=torch.bfloat16,
+                                 device=dev()),
+                     *(torch.empty(2 ** 28 + 1, device=dev())
+                       for _ in range(2)))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_far_apart_gpu(dtype):
+    """Rows whose offsets 32 bits do not hold, against the formulas."""
+    far = 2 ** 29 - 11                  # elements from row to row
+    for c in (1000, 9001):
+        buf = torch.empty(9 * far + c, dtype=dtype, device=dev())
+        x = buf.as_strided((10, c), (far, 1))
+        new = ln_inputs((10, c), dtype, dev())
+        x.copy_(new[0])
+        ln_check(x, *new[1:])
+        lp_check(x, torch.arange(10, device=dev()) * 7, k=3)
+        del x, buf
+
+
+@gpu
 def test_label_logprobs_gpu_long_offsets():
     rows, c, tail = 17000, 131072, 40
     x = torch.empty(rows, c, dtype=torch.float16, device=dev()).normal_()

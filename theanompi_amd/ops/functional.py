@@ -522,9 +522,9 @@ def layernorm(x, gamma, beta, eps=1e-5, n_features=None):
     [C].  Only the first ``n_features`` channels count (default: all);
     the physical padding behind them is not read, its outputs and
     gradients are 0.  Statistics are kept in float32.  Returns x's shape
-    and type.  Differentiable once in x, gamma and beta; the sums of the
-    latter two have a fixed order, so a repeated call gives the same
-    bits."""
+    and type.  On the GPU a row may have 2^28 channels.  Differentiable once
+    in x, gamma and beta; the sums of the latter two have a fixed order, so a
+    repeated call gives the same bits."""
     _check_float(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x needs at least one channel")

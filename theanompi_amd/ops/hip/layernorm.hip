@@ -23,6 +23,8 @@
 // one trip to memory and the sums over a row.  A training call of few rows
 // takes the host 70 us, 46 of them any operator's trip through autograd.
 
+#include <algorithm>
+
 #include "common.hpp"
 
 namespace {
@@ -540,23 +542,30 @@ __global__ __launch_bounds__(1024) void ln_join_k(
     float* __restrict__ dbeta, int blocks, int C) {
   __shared__ float acc[64][17];
   const int lx = threadIdx.x & 15, ly = threadIdx.x >> 4;
-  const int c = blockIdx.x * 16 + lx;
-  float s = 0.f;
-  if (c < 2 * C)
+  for (int c0 = blockIdx.x * 16; c0 < 2 * C; c0 += gridDim.x * 16) {
+    const int c = c0 + lx;
+    float s = 0.f;
+    if (c < 2 * C)
 #pragma unroll 4
-    for (int b = ly; b < blocks; b += 64) s += part[(long)b * 2 * C + c];
-  acc[ly][lx] = s;
-  __syncthreads();
-  if (threadIdx.x < 16 && c < 2 * C) {
-    s = 0.f;
+      for (int b = ly; b < blocks; b += 64) s += part[(long)b * 2 * C + c];
+    __syncthreads();                 // acc is read
+    acc[ly][lx] = s;
+    __syncthreads();
+    if (threadIdx.x < 16 && c < 2 * C) {
+      s = 0.f;
 #pragma unroll
-    for (int r = 0; r < 64; ++r) s += acc[r][lx];
-    if (c < C)
-      dgamma[c] = s;
-    else
-      dbeta[c - C] = s;
+      for (int r = 0; r < 64; ++r) s += acc[r][lx];
+      if (c < C)
+        dgamma[c] = s;
+      else
+        dbeta[c - C] = s;
+    }
   }
 }
+
+// A launch's threads are counted in 32 bits: 2^22 blocks of 1024 are too
+// many, which rows of 2^25 channels would take.
+constexpr long JOINS = 1L << 20;
 
 // Lanes a row of v vectors, with one vector a lane.
 #define LN_PICK(v, CALL)               \
@@ -673,7 +682,8 @@ hipError_t bwd(const void* dy, const void* x, const float* gamma,
   }
   HIP_KERNEL_ASSERT_OK(hipGetLastError());
   if (shares)
-    hipLaunchKernelGGL(ln_join_k, dim3((unsigned)((2 * C + 15) / 16)),
+    hipLaunchKernelGGL(ln_join_k,
+                       dim3((unsigned)std::min((2L * C + 15) / 16, JOINS)),
                        dim3(1024), 0, stream, part, dgamma, dbeta,
                        (int)shares, C);
   return hipGetLastError();

@@ -1419,10 +1419,9 @@ static bool ns_pairs(const NsArgs& a, long steps) {
 
 // Of two steps the products of m x m are five that follow one another, or
 // six in four launches: what counts is how many follow one another, until
-// two at a time fill the device (us: 512 x 4608 211 -> 188, the weights
-// of a wide residual network 184 -> 170; tiles of 128: 1000 x 8000, 36 of
-// them, 643 -> 593; 1536 x 4096, 78, 669 -> 653; 2000 x 4000, 136, 966 ->
-// 1014; 4096 x 9216, 528, 5505 -> 5932).
+// two at a time fill the device (us: 512 x 4608 213 -> 195; tiles of 128:
+// 1300 x 8000, 66 of them, 771 -> 756; 1900 x 6000, 120, 1034 -> 1048; 2000 x
+// 4000, 136, 930 -> 978; 4096 x 9216, 528, 5752 -> 6185).
 static bool ns_six(const NsArgs& a) {
   if (a.tile == 64) return true;
   long tiles = 0;
@@ -1430,7 +1429,7 @@ static bool ns_six(const NsArgs& a) {
     const long t = (a.p[i].m + 127) / 128;
     tiles += a.p[i].batch * (t * (t + 1) / 2);
   }
-  return tiles <= 128;
+  return tiles <= 96;
 }
 
 // Fills in shapes and workspace of `a` (count problems that have m, n,
@@ -1467,9 +1466,9 @@ static torch::Tensor ns_workspace(NsArgs& a, bool pairs,
       // Blocks a matrix: as many as compute units in all, but each adds up
       // the shares of all of its matrix (0.09 us one), and those of a long
       // one do better with fewer, which have more columns each (1.3 us).
-      // Measured (us) with 8, 16, 32, 64 and 128: 64 x 1536 51, 48, 44, 44,
-      // 44; 64 x 8192 123, 83, 68, 71, 90; 64 x 16384 212, 128, 92, 84, 99;
-      // 64 x 100000 1271, 665, 367, 229, 179.
+      // Measured (us) with 8, 16, 32, 64 and 128: 64 x 1536 72, 60, 63, 62,
+      // 63; 64 x 8192 167, 109, 88, 96, 117; 64 x 16384 283, 169, 123, 111,
+      // 127; 64 x 100000 1697, 884, 480, 297, 228.
       const long cols = p.np / 64;
       const long groups = blocks <= 256 ? cols : (cols * 256 + blocks - 1) / blocks;
       const long most = std::max(24L, (long)(4.0 * std::sqrt((double)cols)));
@@ -1673,7 +1672,7 @@ static void muon_update(std::vector<torch::Tensor> ws,
   // One pass for each kind of kernels, NS_MAXP matrices at a time.  Few
   // rows have kernels of their own only where no others take the general
   // ones: beside those they cost next to nothing (the 17 weights of a
-  // wide residual network: 190 us together, 231 us apart).
+  // wide residual network: 194 us together, 240 us apart).
   bool general = false;
   auto kind = [&](const NsProb& p) {
     const int tile = ns_tile(p);

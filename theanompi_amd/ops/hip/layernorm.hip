@@ -17,10 +17,10 @@
 // behind them (the physical channel padding) is left out of the
 // statistics, and its outputs are zeros.
 //
-// Measured: 802816 x 256 bf16 forward 142 us, 5.8 TB/s, backward 233 + 5
-// us, 5.3 TB/s (a copy of 411 MB here 5.3).  4099 x 1000 f32 forward 11,
-// backward 17 + 5 us; 128 x 4096 bf16 4 + 4.5, 32 x 1024 f16 3.1: a launch,
-// one trip to memory and the sums over a row.  A training call of few rows
+// Measured: 802816 x 256 bf16 forward 149 us, 5.5 TB/s, backward 235 + 5
+// us, 5.2 TB/s (a copy of 411 MB here 5.3).  4099 x 1000 f32 forward 11,
+// backward 14 + 4.4 us; 128 x 4096 bf16 3.7 + 4.6, 32 x 1024 f16 3.1: a
+// launch, one trip to memory and the sums over a row.  A training call of few rows
 // takes the host 70 us, 46 of them any operator's trip through autograd.
 
 #include <algorithm>
@@ -583,13 +583,13 @@ constexpr long JOINS = 1L << 20;
 // Vectors a row may have for registers.  The backward's sums of dgamma and
 // dbeta for two vectors do not fit the 128 registers that 1024 threads have
 // each, but without them it does: rows over 1024 vectors leave them to the
-// column kernel, which reads x and dy again (16384 bf16: 3.15 TB/s of the
+// column kernel, which reads x and dy again (16384 bf16: 2.7 TB/s of the
 // three arrays; with both passes from the wide kernel 2.64).
 constexpr long WIDEST = 2048, WIDEST_SUMS = 1024;
 
 // Threads a compute unit: rows are fetched ahead, and 16 waves do better
-// than 32 (TB/s forward: 256 bf16 5.76, 4.61; 1000 bf16 5.54, 4.40; 512
-// fp32 5.95, 5.25).
+// than 32 (TB/s forward, calls one behind the other: 256 bf16 4.6, 4.4; 1000
+// bf16 4.4, 4.2; 512 fp32 5.5, 5.2).
 constexpr long THREADS = 1024;
 
 template <typename T>
@@ -615,11 +615,11 @@ hipError_t fwd(const void* x, const float* gamma, const float* beta,
                        (T*)y, mean, rstd, rows, C, n, ldx, eps);         \
   } while (0)
   // Three vectors on lanes that they fill, where one would leave a quarter
-  // to a half of the lanes idle (TB/s with three and one: 300 bf16 4.83,
-  // 3.18; 768 bf16 5.25, 4.72; 1500 bf16 5.15, 3.75; 2500 bf16 4.99, 2.95;
-  // 2500 fp32 5.47, 4.78; 9000 bf16 5.38, two 4.36); past 512 vectors 16-bit
-  // types do better with two (5000 bf16: 4.28 with three, 5.23 with two,
-  // 4.46 with one).
+  // to a half of the lanes idle (TB/s with three and one: 300 bf16 4.72,
+  // 2.93; 768 bf16 5.17, 4.20; 1500 bf16 4.91, 3.74; 2500 bf16 4.92, 3.23;
+  // 2500 fp32 5.44, 4.13; 9000 bf16 5.06, two 3.76); past 512 vectors 16-bit
+  // types do better with two (5000 bf16: 4.10 with three, 4.83 with two,
+  // 3.39 with one).
   if (v > 32 && v <= 48) LN_FWD(16, 3);
   else if (v > 64 && v <= 96) LN_FWD(32, 3);
   else if (v > 128 && v <= 192) LN_FWD(64, 3);

@@ -12,9 +12,9 @@
 // segment) in registers, takes maximum and sums from there and writes
 // one partial result; rows of more than one segment are joined by a
 // second kernel, in a fixed order.  2048 x 131072 bf16, top 8: forward
-// 114 + 6 us (4.7 TB/s; its vector instructions, counted, come to half of
-// that, most of it one exp2 an element at a quarter of the rate), backward 170
-// (6.3 TB/s; a copy reaches 4.9 to 6.1 here).  Few rows wait for a chain
+// 123 + 6 us (4.2 TB/s; its vector instructions, counted, come to half of
+// that, most of it one exp2 an element at a quarter of the rate), backward 172
+// (6.2 TB/s; a copy reaches 4.9 to 6.1 here).  Few rows wait for a chain
 // instead: 128 x 1000 5 + 5 us and 1 x 131072 fp32 6 + 4, of which a launch
 // is 1.3 each, and a training call's time is the host's: 70 us, 46 of them
 // any operator's trip through autograd.

@@ -34,12 +34,12 @@
 // in a list: equal lists give equal bits, and a matrix alone others.
 //
 // What bounds it, 5 steps: large matrices, the matrix units: 4096 x 9216
-// takes 5.5 ms, of which 775 us a product with X (1197 TFLOP/s in fp16,
-// where the library's largest fp16 products reach 1340 to 1390), 427 a
-// Gram matrix (1090), 199 one of A and M (1035).  Matrices up to some 2^20
+// takes 5.8 ms, of which 853 us a product with X (1088 TFLOP/s in fp16,
+// where the library's largest fp16 products reach 1340 to 1390), 456 a
+// Gram matrix (1049), 215 one of A and M (988).  Matrices up to some 2^20
 // elements: the 15 to 20 launches, which need one another's results (12 x
-// 333 x 201 128 us, the 17 weights of a wide residual network 168).  One
-// takes 7 to 8 us: 1.3 of launch, 1.1 until a block knows its tile, 1.1
+// 333 x 201 133 us, the 17 weights of a wide residual network 192).  One
+// takes 7 to 9 us: 1.3 of launch, 1.1 until a block knows its tile, 1.1
 // for the first slice, 0.43 a further one of 64, 0.9 to store the sums.
 
 #include <atomic>
@@ -677,10 +677,10 @@ __global__ __launch_bounds__(256) void ns_join_k(const NsArgs a) {
 // `groups` blocks a matrix have a range of X's columns each.  Every block
 // adds up A from all blocks' shares and does the m x m work itself, which
 // costs less than a launch; then it multiplies its columns and leaves its
-// share of the next A.  64 x 576, 5 steps: 37.5 us in 5 kernels (88 in 20 of
-// the general ones), 4 for the squares, 6 to load and for the first
-// shares, 10 for two steps, 7 for one.  They wait, in turn, for a launch,
-// the shares, up to six products that need one another, the columns.
+// share of the next A.  64 x 576, 5 steps: 42.6 us in 6 kernels (twice that
+// in 20 of the general ones), 4 for the squares, 6 to load and for the first
+// shares, 10 for two steps, 7.4 to 8.6 for one.  They wait, in turn, for a
+// launch, the shares, up to six products that need one another, the columns.
 // (Asking for the columns before the products gained nothing here, and
 // lost where a block has many: 64 x 16384 128 -> 139 us.)
 
@@ -692,9 +692,9 @@ constexpr int SLICE = FEW * 64;               // halves of 32 columns
 // neighbours of a row of the result (kept transposed instead, the errors
 // of the chain of products came out twice as large).
 // All four products, the small ones first: an addition in the matrix
-// units seems to cut the sum off, and six of them on the large sum made a
-// step 1.3e-7 off instead of 1.0e-7.  (The smallest, lo * lo, costs 1 us of
-// 36 here and takes a tenth off the errors.)
+// units cuts the sum off, and six of them on the large sum made a step
+// 1.3e-7 off instead of 1.0e-7.  (The smallest, lo * lo, costs 1 us of 43 here
+// and takes a tenth off the errors.)
 DEV void few_terms(const half8 (&f)[2][2][2], const half8 (&g)[2][2][2],
                    f32x4 (&acc)[2][2]) {
 #pragma unroll
@@ -1119,8 +1119,8 @@ hipError_t launch_ns_gemm(NsArgs* a, int mode, hipStream_t stream) {
   // The rest: cut k so that it, too, gives every slot a run of 384 or
   // more, unless the longest run is then less than 768 shorter: a join is
   // a launch of 6 us (us, with the cut and without: 768 x 768 217, 191;
-  // 1000 x 1000 270, 223; but 256 x 2304, 1700 shorter, 153, 206; shortest
-  // run of 192: 128 x 65536 427, of 384 330).
+  // 1000 x 1000 270, 223; but 256 x 2304, 1700 shorter, 163, 208, 4096 x 9216
+  // 5755, 6831; shortest run of 192: 128 x 65536 427, of 384 323).
   rest = tiles - a->whole;
   for (int i = 0; i < a->count; ++i) {
     long skip = a->whole - a->tile0[i];

@@ -14,9 +14,9 @@
 // one stays clear of fp16's smallest step, and a product is three matrix
 // products, hi*hi + hi*lo + lo*hi, in fp32 accumulators, at a third of the
 // fp16 rate, five times the fp32 matrix rate.  Five steps are off by 0.6 to
-// 2.2e-6 (Frobenius norm, relative): 0.4 to 0.9 times what plain fp32 products
-// are from 65 rows on, and up to 1.7 times of some ten rows, whose sums are
-// so short that the two bits show.
+// 2.2e-6 (Frobenius norm, relative): 0.2 to 0.9 times what plain fp32 products
+// are from 65 rows on, and up to 1.7 times (2.1 among longer matrices) of some
+// ten rows, whose sums are so short that the two bits show.
 // The entries stay far below fp16's largest: singular values of X are at
 // most 1.21 over the whole iteration, those of M at most 3.45.
 //
@@ -34,9 +34,9 @@
 // in a list: equal lists give equal bits, and a matrix alone others.
 //
 // What bounds it, 5 steps: large matrices, the matrix units: 4096 x 9216
-// takes 5.8 ms, of which 853 us a product with X (1088 TFLOP/s in fp16,
-// where the library's largest fp16 products reach 1340 to 1390), 456 a
-// Gram matrix (1049), 215 one of A and M (988).  Matrices up to some 2^20
+// takes 5.8 ms, of which 837 us a product with X (1109 TFLOP/s in fp16,
+// where the library's largest fp16 products reach 1340 to 1390), 438 a
+// Gram matrix (1092), 214 one of A and M (995).  Matrices up to some 2^20
 // elements: the 15 to 20 launches, which need one another's results (12 x
 // 333 x 201 133 us, the 17 weights of a wide residual network 192).  One
 // takes 7 to 9 us: 1.3 of launch, 1.1 until a block knows its tile, 1.1
